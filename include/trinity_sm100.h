@@ -144,6 +144,38 @@ TRINITY_SM100_API int trinity_sm100_rmsnorm_bf16(const void* x, const void* gain
 TRINITY_SM100_API int trinity_sm100_softmax_bf16(const void* x, void* y, int64_t rows, int64_t cols, void* stream);
 
 /*
+ * The seam between two blocks of a residual network, in one pass over the rows (FP32 math):
+ *   b = x                                           (post_norm == 0 and no post_gain)
+ *     = x / sqrt(mean(x^2) + post_eps) * post_gain  (otherwise; post_gain may be NULL)
+ *   residual_out = h = residual_scale * residual + gate * b
+ *   out              = h / sqrt(mean(h^2) + eps) * gain
+ * x and the residual are BF16 or FP32 [rows, cols] with any row pitch (elements); residual_out has
+ * the residual's type; gate, gain, post_gain and out are BF16.  gain[cols], post_gain[cols] and
+ * gate may be NULL.  gate is read at row * gate_row_stride + col * gate_col_stride, with a column
+ * stride of 0 or 1 and a row stride of 0 or at least a row: one value for each column, each row
+ * or each element.  out is computed from h before its rounding.  1 <= cols <= 16384.
+ * residual_out may be the residual (or x of its type) and out may be x (or the residual, if BF16),
+ * in the same layout; any other overlap of an output with another operand is not supported.
+ * An all-zero h with eps == 0 gives NaN, as trinity_sm100_rmsnorm_bf16 does.
+ */
+typedef struct trinity_sm100_rmsnorm_residual_args {
+  const void* x;
+  const void* residual;
+  const void* gate;
+  const void* gain;
+  const void* post_gain;
+  void* residual_out;
+  void* out;
+  int64_t rows, cols;
+  int64_t ld_x, ld_residual, ld_residual_out, ld_out;
+  int64_t gate_row_stride, gate_col_stride;
+  int32_t x_dtype, residual_dtype; /* trinity_sm100_dtype */
+  int32_t post_norm;
+  float eps, post_eps, residual_scale;
+} trinity_sm100_rmsnorm_residual_args;
+TRINITY_SM100_API int trinity_sm100_rmsnorm_residual(const trinity_sm100_rmsnorm_residual_args* args, void* stream);
+
+/*
  * Generic pointwise evaluation in FP32 with one rounding at the store.
  *
  *   out[r,c] = f(operands..., constants)        out is [rows, cols] row-major (1-D: rows == 1)

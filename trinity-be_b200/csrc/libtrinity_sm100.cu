@@ -4,6 +4,7 @@
 #include "host_common.cu"
 #include "gemm_tcgen05.cu"
 #include "rownorm.cu"
+#include "block_norm.cu"
 #include "pointwise.cu"
 #include "mla_decode.cu"
 #include "allreduce.cu"

@@ -21,6 +21,7 @@ EXPORTS = (
     "trinity_sm100_gemm_batched_bf16",
     "trinity_sm100_gemm_pair_capacity",
     "trinity_sm100_rmsnorm_bf16",
+    "trinity_sm100_rmsnorm_residual",
     "trinity_sm100_softmax_bf16",
     "trinity_sm100_mla_scratch_bytes",
     "trinity_sm100_mla_default_splits",
@@ -75,6 +76,21 @@ class GemmBatchArgs(ctypes.Structure):
                 ("stride_out", ctypes.c_int64), ("stride_bias", ctypes.c_int64)]
 
 
+class RmsnormResidualArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p), ("residual", ctypes.c_void_p), ("gate", ctypes.c_void_p),
+        ("gain", ctypes.c_void_p), ("post_gain", ctypes.c_void_p),
+        ("residual_out", ctypes.c_void_p), ("out", ctypes.c_void_p),
+        ("rows", ctypes.c_int64), ("cols", ctypes.c_int64),
+        ("ld_x", ctypes.c_int64), ("ld_residual", ctypes.c_int64),
+        ("ld_residual_out", ctypes.c_int64), ("ld_out", ctypes.c_int64),
+        ("gate_row_stride", ctypes.c_int64), ("gate_col_stride", ctypes.c_int64),
+        ("x_dtype", ctypes.c_int32), ("residual_dtype", ctypes.c_int32),
+        ("post_norm", ctypes.c_int32), ("eps", ctypes.c_float), ("post_eps", ctypes.c_float),
+        ("residual_scale", ctypes.c_float),
+    ]
+
+
 class MlaArgs(ctypes.Structure):
     _fields_ = [
         ("q", ctypes.c_void_p), ("cache", ctypes.c_void_p), ("out", ctypes.c_void_p),
@@ -116,6 +132,8 @@ def library():
             lib.trinity_sm100_rmsnorm_bf16.argtypes = [
                 ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
                 ctypes.c_float, ctypes.c_void_p]
+            lib.trinity_sm100_rmsnorm_residual.argtypes = [
+                ctypes.POINTER(RmsnormResidualArgs), ctypes.c_void_p]
             lib.trinity_sm100_softmax_bf16.argtypes = [
                 ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p]
             lib.trinity_sm100_mla_scratch_bytes.argtypes = [ctypes.c_int32] * 4
@@ -158,6 +176,57 @@ def _stream(stream=None):
 def _require(t, dtype, name):
     if not t.is_cuda or t.dtype != dtype:
         raise ValueError(f"{name}: expected a CUDA tensor of {dtype}, got {t.device} {t.dtype}")
+
+
+def _submit(device, stream, operands, launch):
+    """``launch(handle)`` with ``device`` current and ``handle`` the stream to launch on.
+
+    Memory that ``launch`` allocates (outputs, scratch) belongs to that stream.  On a stream other
+    than the device's current one the allocator is told that the operands are in use there and the
+    results here, so neither is handed out again too early; ordering the two streams is left to
+    the caller, as with every torch operation."""
+    if stream is None:
+        if device.index == torch.cuda.current_device():
+            return launch(torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(device):
+            return launch(torch.cuda.current_stream().cuda_stream)
+    if stream.device != device:
+        raise ValueError(f"the stream belongs to {stream.device}, the operands to {device}")
+    with torch.cuda.device(device):
+        here = torch.cuda.current_stream()
+        if stream == here:
+            return launch(here.cuda_stream)
+        with torch.cuda.stream(stream):
+            result = launch(stream.cuda_stream)
+        for t in operands:
+            if t is not None:
+                t.record_stream(stream)
+        for t in result if isinstance(result, tuple) else (result,):
+            if t is not None:
+                t.record_stream(here)
+        return result
+
+
+def _same_device(device, **operands):
+    for name, t in operands.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, the other operands on {device}")
+
+
+def _rows_ok(t):
+    """A [rows, cols] tensor with a unit inner stride (of no meaning when there is one column)."""
+    return t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] == 1)
+
+
+def _pitch(t):
+    """Row pitch of a [rows, cols] tensor in elements (of no meaning when there is one row)."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def _dtype_code(t, name):
+    if not t.is_cuda or t.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"{name}: expected a CUDA tensor of bf16 or fp32, got {t.device} {t.dtype}")
+    return DT_FP32 if t.dtype == torch.float32 else DT_BF16
 
 
 def launch_count():
@@ -280,6 +349,74 @@ def rmsnorm(x, gain=None, eps=0.0, out=None, stream=None):
             x.data_ptr(), gain.data_ptr() if gain is not None else None, out.data_ptr(),
             x.shape[0], x.shape[1], float(eps), _stream(stream)))
     return out
+
+
+def rmsnorm_residual(x, residual, *, gain=None, post_gain=None, post_norm=None, gate=None, residual_scale=1.0,
+                     eps=0.0, post_eps=None, residual_out=None, out=None, stream=None):
+    """The seam between two blocks: ``(h, y)`` with ``h = residual_scale * residual + gate * b`` and
+    ``y = h / sqrt(mean(h^2) + eps) * gain``, where ``b`` is the block's output ``x``, normalised
+    with ``post_eps`` (default ``eps``) and ``post_gain`` if ``post_norm`` (default: if ``post_gain``
+    is given).  See ``trinity_sm100_rmsnorm_residual``.
+
+    ``x`` and ``residual`` are [rows, cols], BF16 or FP32, with a unit inner stride; ``h`` has the
+    residual's type, ``y`` is BF16.  ``gate`` is a BF16 tensor that broadcasts to [rows, cols]:
+    [cols], [1, cols], [rows, 1] or [rows, cols].  ``residual_out=residual`` updates the stream in place."""
+    x_dtype = _dtype_code(x, "x")
+    residual_dtype = _dtype_code(residual, "residual")
+    if residual.shape != x.shape or not _rows_ok(x) or not _rows_ok(residual):
+        raise ValueError("rmsnorm_residual: x and residual must be [rows, cols] with a unit inner stride")
+    rows, cols = x.shape
+    device = x.device
+    for name, t in (("gain", gain), ("post_gain", post_gain)):
+        if t is not None:
+            _require(t, torch.bfloat16, name)
+            if tuple(t.shape) != (cols,) or not t.is_contiguous():
+                raise ValueError(f"rmsnorm_residual: {name} must be [cols]")
+    if post_norm is None:
+        post_norm = post_gain is not None
+    elif not post_norm and post_gain is not None:
+        raise ValueError("rmsnorm_residual: post_gain without the post norm")
+    args = RmsnormResidualArgs()
+    if gate is not None:
+        _require(gate, torch.bfloat16, "gate")
+        try:
+            gate = gate.expand(rows, cols)
+        except RuntimeError:
+            raise ValueError(f"rmsnorm_residual: gate {tuple(gate.shape)} does not broadcast to {(rows, cols)}") from None
+        row_stride, col_stride = gate.stride()
+        if cols == 1:
+            col_stride = 0
+        if rows == 1:
+            row_stride = 0
+        if col_stride not in (0, 1):
+            raise ValueError("rmsnorm_residual: gate must have an inner stride of 0 or 1")
+        args.gate, args.gate_row_stride, args.gate_col_stride = gate.data_ptr(), row_stride, col_stride
+    for name, t, dtype in (("residual_out", residual_out, residual.dtype), ("out", out, torch.bfloat16)):
+        if t is not None:
+            _require(t, dtype, name)
+            if t.shape != x.shape or not _rows_ok(t):
+                raise ValueError(f"rmsnorm_residual: {name} must be [rows, cols] with a unit inner stride")
+    _same_device(device, residual=residual, gain=gain, post_gain=post_gain, gate=gate, residual_out=residual_out,
+                 out=out)
+    args.x, args.residual = x.data_ptr(), residual.data_ptr()
+    args.gain = gain.data_ptr() if gain is not None else None
+    args.post_gain = post_gain.data_ptr() if post_gain is not None else None
+    args.rows, args.cols = rows, cols
+    args.ld_x, args.ld_residual = _pitch(x), _pitch(residual)
+    args.x_dtype, args.residual_dtype = x_dtype, residual_dtype
+    args.post_norm = int(post_norm)
+    args.eps, args.post_eps = eps, eps if post_eps is None else post_eps
+    args.residual_scale = residual_scale
+
+    def launch(handle):
+        h = torch.empty((rows, cols), dtype=residual.dtype, device=device) if residual_out is None else residual_out
+        y = torch.empty((rows, cols), dtype=torch.bfloat16, device=device) if out is None else out
+        args.residual_out, args.out = h.data_ptr(), y.data_ptr()
+        args.ld_residual_out, args.ld_out = _pitch(h), _pitch(y)
+        _check(library().trinity_sm100_rmsnorm_residual(ctypes.byref(args), handle))
+        return h, y
+
+    return _submit(device, stream, (x, residual, gain, post_gain, gate, residual_out, out), launch)
 
 
 def softmax(x, out=None, stream=None):
