@@ -320,6 +320,94 @@ TRINITY_SM100_API int trinity_sm100_mla_decode_bf16(const trinity_sm100_mla* arg
 TRINITY_SM100_API int trinity_sm100_mla_decode_bf16_noalloc(const trinity_sm100_mla* args, void* stream);
 
 /*
+ * A paged key/value cache held in 4 bits, for attention with separate keys and values
+ * (heads / kv_heads query heads to a cached head).
+ *
+ * A row (one position, one cached head) of head_dim channels is cut into groups of `group`
+ * channels.  A group keeps zero = min (exact in BF16) and scale = bf16((max - min) / 15), and for
+ * each channel code = rint((x - zero) / scale), clamped to 0..15, which stands for
+ * zero + scale * code.  A group of equal values has scale 0 and codes 0; one that holds an infinity
+ * or a NaN (or whose max - min overflows) has scale NaN and reads back as NaN.
+ *
+ *   k_codes, v_codes    [pages, kv_heads, page, head_dim / 2]          uint8, channel 2i in the low half
+ *   k_scales, v_scales  [pages, kv_heads, page, head_dim / group, 2]   bf16 (scale, zero)
+ *
+ * all contiguous and 16-byte aligned.  `page` positions to a page, a multiple of 16 (copies are
+ * widest with multiples of 128); head_dim 64 or 128; group 32, 64 or 128, at most head_dim.
+ * Position `slot` of the cache is page slot / page, place slot % page.
+ */
+typedef struct trinity_sm100_kv4_cache {
+  void* k_codes;
+  void* k_scales;
+  void* v_codes;
+  void* v_scales;
+  int32_t pages, kv_heads, page, head_dim, group, reserved;
+} trinity_sm100_kv4_cache;
+
+/* Key and value rows [tokens, kv_heads, head_dim] with any token and head stride (elements, unit
+ * inner stride) and the slot of each token, int64 [tokens]. */
+typedef struct trinity_sm100_kv4_rows {
+  void* k;
+  void* v;
+  const void* slots;
+  int64_t tokens;
+  int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+} trinity_sm100_kv4_rows;
+
+/*
+ * Writes BF16 rows into the cache at their slots.  A negative slot marks a token of a padded batch
+ * that is not written; a slot behind the last page is not written either and sets the device status
+ * word (0x901).  Slots of one call are distinct (of equal ones any may win, row by row).
+ */
+TRINITY_SM100_API int trinity_sm100_kv4_append(const trinity_sm100_kv4_cache* cache,
+                                               const trinity_sm100_kv4_rows* rows, void* stream);
+
+/*
+ * Reads rows back: the values that the codes at the slots stand for, rounded once to out_dtype.
+ * k and v are outputs whose rows start on 16 bytes.  A negative slot reads as zeros; one behind the
+ * last page too, and sets the device status word (0x902).
+ */
+TRINITY_SM100_API int trinity_sm100_kv4_read(const trinity_sm100_kv4_cache* cache, const trinity_sm100_kv4_rows* rows,
+                                             int32_t out_dtype, void* stream);
+
+/*
+ * Attention of one new token per sequence over the cache:
+ *   out[b,h,:] = sum_t softmax_t(scale * q[b,h] . k[b,t,h / (heads / kv_heads)]) v[b,t,...]
+ * over the first lengths[b] positions of sequence b; position t lies in page
+ * page_table[b, t / page], place t % page.
+ *
+ *   q           [batch, heads, head_dim]  bf16, any batch and head stride that keeps rows on 16 bytes
+ *   page_table  int32 [batch, max_pages], row pitch table_stride; only the entries that lengths[b]
+ *               reaches are read
+ *   lengths     int32 [batch], read on the device (a captured launch follows them); below 0 counts as
+ *               0 and above max_pages * page as that
+ *   out         [batch, heads, head_dim]  bf16, contiguous; a sequence of length 0 gets zeros
+ *   lse         NULL or fp32 [batch, heads]: log sum_t exp(scale * q . k[t]) (-inf for length 0), with
+ *               which results over several caches can be joined
+ *   workspace   trinity_sm100_kv4_decode_workspace_bytes() bytes, 16-byte aligned; nothing in it needs
+ *               clearing, calls that may overlap in time need one each
+ *
+ * A page number outside the cache is not followed: page 0 is read in its place and the device status
+ * word is set (0x903).  The sum is taken in an order fixed by the lengths: two launches give the
+ * same bits.
+ */
+typedef struct trinity_sm100_kv4_decode_args {
+  const void* q;
+  const void* page_table;
+  const void* lengths;
+  void* out;
+  void* lse;
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t q_batch_stride, q_head_stride, table_stride;
+  int32_t batch, heads, max_pages;
+  float scale;
+} trinity_sm100_kv4_decode_args;
+TRINITY_SM100_API size_t trinity_sm100_kv4_decode_workspace_bytes(int32_t heads, int32_t kv_heads, int32_t head_dim);
+TRINITY_SM100_API int trinity_sm100_kv4_decode(const trinity_sm100_kv4_cache* cache,
+                                               const trinity_sm100_kv4_decode_args* args, void* stream);
+
+/*
  * Sum all-reduce of a BF16 [rows, cols] matrix across `world` GPUs of one NVLink domain,
  * through peer-mapped memory (no NVSHMEM, no NCCL on the data path).
  *

@@ -1,0 +1,961 @@
+// A paged key/value cache held in 4 bits: writing it, reading it back, and the attention of one new
+// token per sequence over it.
+//
+// Cache format.  A key or value row (one position, one cached head) of D channels is cut into
+// groups of 32, 64 or 128 channels.  A group keeps zero = min (exact in BF16), scale =
+// bf16((max - min) / 15) and for each channel code = rint((x - zero) / scale) in 0..15; a code
+// stands for zero + scale * code.  A group whose values are all equal has scale 0 and codes 0; one
+// that holds an infinity or a NaN has scale NaN and reads back as NaN.
+//   codes  [pages, kv_heads, page, D / 2]         two channels a byte, the even one in the low bits
+//   scales [pages, kv_heads, page, D / group, 2]  BF16 (scale, zero)
+#include <cuda_fp16.h>
+
+#include "host_common.h"
+#include "sm100_ptx.cuh"
+
+namespace trinity_sm100 {
+namespace {
+
+// Device status sites of invalid device-side data (no access is made with it).
+constexpr uint32_t kSiteKv4AppendSlot = 0x901;
+constexpr uint32_t kSiteKv4ReadSlot = 0x902;
+constexpr uint32_t kSiteKv4Page = 0x903;
+
+// ---------------------------------------------------------------- append and read
+//
+// Bound by memory: 2 D bytes read and D / 2 + 4 D / group written per row (append).  A lane owns
+// eight channels (one 16-byte access, one 32-bit word of codes), D / 8 lanes a row, keys and
+// values in one launch; a group's extrema meet by shuffles within its 4, 8 or 16 lanes.
+struct Kv4Rows {
+  const __nv_bfloat16* in[2];      // append: keys, values
+  void* out[2];                    // read: keys, values
+  uint8_t* codes[2];
+  __nv_bfloat162* scales[2];
+  const long long* slots;
+  long long tokens, positions;     // positions = pages * page
+  long long token_stride[2], head_stride[2];
+  int kv_heads, page, group, out_f32;
+};
+
+// Row of the cache that holds head `head` of position `slot`.
+__device__ __forceinline__ long long kv4_row(const Kv4Rows& p, long long slot, int head) {
+  const long long page = slot / p.page;
+  return (page * p.kv_heads + head) * p.page + (slot - page * p.page);
+}
+
+template <int kD, bool kVector>
+__global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4Rows p) {
+  constexpr int kLanes = kD / 8;
+  grid_dependents_may_launch();
+  grid_dependency_wait();
+  const int which = blockIdx.y;
+  const long long index = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) / kLanes;
+  const int lane = threadIdx.x % kLanes;
+  const bool live = index < p.tokens * p.kv_heads;   // shuffles below need every lane of the warp
+  const long long token = live ? index / p.kv_heads : 0;
+  const int head = live ? int(index - token * p.kv_heads) : 0;
+  const long long slot = live ? p.slots[token] : -1;
+  bool write = live && slot >= 0;
+  if (write && slot >= p.positions) {
+    write = false;
+    report_timeout(kSiteKv4AppendSlot);
+  }
+  float v[8];
+  const __nv_bfloat16* src = p.in[which] + token * p.token_stride[which] + head * p.head_stride[which] + lane * 8;
+  if (!write) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+  } else if (kVector) {
+    const uint4 a = __ldcs(reinterpret_cast<const uint4*>(src));
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[2 * e] = bf16_lo(w[e]);
+      v[2 * e + 1] = bf16_hi(w[e]);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = __bfloat162float(src[e]);
+  }
+  float low = v[0], high = v[0];
+  bool bad = false;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    low = fminf(low, v[e]);
+    high = fmaxf(high, v[e]);
+    bad |= !(fabsf(v[e]) < INFINITY);
+  }
+  for (int step = 1; step < p.group / 8; step *= 2) {   // the lanes of a group are neighbours
+    low = fminf(low, __shfl_xor_sync(0xffffffffu, low, step));
+    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, step));
+    bad |= __shfl_xor_sync(0xffffffffu, int(bad), step) != 0;
+  }
+  if (!write) return;
+  const float spread = high - low;
+  bad |= !(spread < INFINITY);
+  const __nv_bfloat16 scale16 = __float2bfloat16(bad ? NAN : spread / 15.0f);
+  const float scale = __bfloat162float(scale16);
+  uint32_t codes = 0;
+  if (scale > 0.0f) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float code = fminf(fmaxf(rintf((v[e] - low) / scale), 0.0f), 15.0f);
+      codes |= static_cast<uint32_t>(code) << (4 * e);
+    }
+  }
+  const long long row = kv4_row(p, slot, head);
+  reinterpret_cast<uint32_t*>(p.codes[which])[row * kLanes + lane] = codes;
+  if (lane % (p.group / 8) == 0) {
+    __nv_bfloat162 pair;
+    pair.x = scale16;
+    pair.y = __float2bfloat16(low);
+    p.scales[which][row * (kD / p.group) + lane * 8 / p.group] = pair;
+  }
+}
+
+// The values that the codes at `slots` stand for, one rounding to the output type (the product
+// scale * code is exact in FP32).  A negative slot reads as zeros.
+template <int kD>
+__global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Rows p) {
+  constexpr int kLanes = kD / 8;
+  grid_dependents_may_launch();
+  grid_dependency_wait();
+  const int which = blockIdx.y;
+  const long long index = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) / kLanes;
+  const int lane = threadIdx.x % kLanes;
+  if (index >= p.tokens * p.kv_heads) return;
+  const long long token = index / p.kv_heads;
+  const int head = int(index - token * p.kv_heads);
+  const long long slot = p.slots[token];
+  float v[8];
+  if (slot >= 0 && slot < p.positions) {
+    const long long row = kv4_row(p, slot, head);
+    const uint32_t codes = reinterpret_cast<const uint32_t*>(p.codes[which])[row * kLanes + lane];
+    const __nv_bfloat162 pair = p.scales[which][row * (kD / p.group) + lane * 8 / p.group];
+    const float scale = __bfloat162float(pair.x), zero = __bfloat162float(pair.y);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = fmaf(static_cast<float>((codes >> (4 * e)) & 15u), scale, zero);
+  } else {
+    if (slot >= 0) report_timeout(kSiteKv4ReadSlot);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+  }
+  const long long at = token * p.token_stride[which] + head * p.head_stride[which] + lane * 8;
+  if (p.out_f32) {
+    float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out[which]) + at);
+    __stcs(dst, make_float4(v[0], v[1], v[2], v[3]));
+    __stcs(dst + 1, make_float4(v[4], v[5], v[6], v[7]));
+  } else {
+    __stcs(reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out[which]) + at),
+           make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                      pack_bf16x2(v[6], v[7])));
+  }
+}
+
+// ---------------------------------------------------------------- attention
+//
+//   s[t] = scale * q . k[t],   out = sum_t exp(s[t] - max s) v[t] / sum_t exp(s[t] - max s)
+//
+// for one query row per sequence and head, heads / kv_heads query heads to a cached head.  Bound by
+// memory (D + 8 D / group bytes a position and cached head) as long as the arithmetic on the codes
+// keeps up, so:
+//
+// * The positions of all (sequence, cached head) rows are cut into tiles of 128 and the tiles, in
+//   order, into equal runs, one for each thread block of a grid that fills the GPU once: whatever the
+//   lengths are (they are read on the device), every SM streams the same share.  A row that one
+//   block holds whole is written at once; the parts of a row that is cut go to the workspace and a
+//   second kernel joins them in block order, so results do not depend on timing.
+// * A producer warp fetches tiles into a ring of stages: codes by tiled TMA with the 32- or 64-byte
+//   swizzle (then the code words that a warp reads lie in distinct banks), scales by bulk copies.
+// * Eight warps take 16 positions of a tile each, with their own running maximum, sum and
+//   accumulator; they meet only at the end of a run's row.
+// * Scores are computed transposed, S^T[16 positions x 8 heads] = K Q^T with mma.sync (m16n8k16):
+//   decoded codes are the A operand straight from registers (tcgen05 would want them written to
+//   shared or tensor memory first, four times the cache bytes), and eight query heads fill a
+//   tile's columns.  The exponentials, transposed in registers, are the B operand of
+//   O^T[channels x 8 heads] += V^T P^T.
+//
+// Key codes enter as FP16: `word & 0x000f000f` read as two FP16 numbers is code * 2^-24 exactly
+// (subnormal; the tensor cores take those at full rate), `& 0x00f000f0` is 16 times that, which the
+// query side takes back.  The query is brought to FP16 with a power of two per head, exactly down
+// to 2^-22 of its largest element.  Scale and zero are applied to the FP32 score.
+// Value codes are decoded to BF16 (128 + code, minus 128, times scale plus zero: one rounding, the
+// rounding that a BF16 cache would have) and the exponentials are rounded to BF16 as the right
+// operand, as in the other attention kernel of this library; both are averaged over positions.
+constexpr int kKv4Tile = 128;          // positions in a stage
+constexpr int kKv4Warps = 8;
+constexpr int kKv4Threads = (kKv4Warps + 1) * 32;
+
+struct Kv4Attend {
+  const __nv_bfloat16* q;
+  const __nv_bfloat162* k_scales;
+  const __nv_bfloat162* v_scales;
+  const int* table;
+  const int* lengths;
+  __nv_bfloat16* out;
+  float* lse;
+  float* parts;          // [blocks][2][8 kNT heads][D] and behind them [blocks][2][8 kNT heads][2]
+  long long q_batch, q_head, table_stride;
+  int batch, heads, kv_heads, group_heads, head_blocks, pages, page, max_pages, box;
+  float scale_log2;
+};
+
+// Where the run of one block starts, and the size of all.
+struct Kv4Start {
+  long long total, tile_base;   // tiles of all rows; tiles before sequence `sequence`
+  int sequence;
+};
+
+__device__ __forceinline__ int kv4_length(const Kv4Attend& p, int b) {
+  const long long most = static_cast<long long>(p.max_pages) * p.page;
+  const int n = p.lengths[b];
+  return n < 0 ? 0 : n > most ? int(most) : n;
+}
+__device__ __forceinline__ int kv4_tiles(int length) { return (length + kKv4Tile - 1) / kKv4Tile; }
+__host__ __device__ __forceinline__ long long kv4_first_tile(long long total, int blocks, int block) {
+  return total * block / blocks;
+}
+// Block whose run holds tile t: the largest i with total * i / blocks <= t.
+__host__ __device__ __forceinline__ int kv4_block_of(long long total, int blocks, long long t) {
+  return int(((t + 1) * blocks - 1) / total);
+}
+
+// All kThreads threads of the block; finds the sequence that holds tile total * block / blocks.
+template <int kThreads>
+__device__ __forceinline__ Kv4Start kv4_locate(const Kv4Attend& p, int blocks, int block, long long* scratch) {
+  constexpr int kWarps = kThreads / 32;
+  const int rows = p.kv_heads * p.head_blocks;
+  const int per = (p.batch + kThreads - 1) / kThreads;
+  const int begin = min(p.batch, int(threadIdx.x) * per), end = min(p.batch, begin + per);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long sum = 0;
+  for (int b = begin; b < end; ++b) sum += static_cast<long long>(kv4_tiles(kv4_length(p, b))) * rows;
+  long long inclusive = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    const long long below = __shfl_up_sync(0xffffffffu, inclusive, o);
+    if (lane >= o) inclusive += below;
+  }
+  if (lane == 31) scratch[warp] = inclusive;
+  __syncthreads();
+  long long base = inclusive - sum, total = 0;
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) base += scratch[w];
+    total += scratch[w];
+  }
+  const long long first = kv4_first_tile(total, blocks, block);
+  if (first >= base && first < base + sum) {   // exactly one thread, if there is any tile
+    int b = begin;
+    for (;; ++b) {
+      const long long n = static_cast<long long>(kv4_tiles(kv4_length(p, b))) * rows;
+      if (first < base + n) break;
+      base += n;
+    }
+    scratch[kWarps] = base;
+    scratch[kWarps + 1] = b;
+  }
+  __syncthreads();
+  Kv4Start s;
+  s.total = total;
+  s.tile_base = scratch[kWarps];
+  s.sequence = int(scratch[kWarps + 1]);
+  return s;
+}
+
+// Walks the rows (sequence, cached head, head block) that a run of tiles covers.
+struct Kv4Walk {
+  long long next, end;       // tiles of the run not yet visited
+  long long base;            // first tile of sequence b
+  int b, length, tiles;
+  // the current piece
+  int row, first, count;     // row within the sequence, first tile of the piece, its tiles
+  __device__ __forceinline__ Kv4Walk(const Kv4Attend& p, const Kv4Start& s, int blocks, int block) {
+    next = kv4_first_tile(s.total, blocks, block);
+    end = kv4_first_tile(s.total, blocks, block + 1);
+    base = s.tile_base;
+    b = s.sequence;
+    length = next < end ? kv4_length(p, b) : 0;
+    tiles = kv4_tiles(length);
+  }
+  __device__ __forceinline__ bool step(const Kv4Attend& p) {
+    if (next >= end) return false;
+    const int rows = p.kv_heads * p.head_blocks;
+    while (next >= base + static_cast<long long>(tiles) * rows) {   // the run ends inside a sequence with tiles
+      base += static_cast<long long>(tiles) * rows;
+      ++b;
+      length = kv4_length(p, b);
+      tiles = kv4_tiles(length);
+    }
+    const int local = int(next - base);
+    row = local / tiles;
+    first = local - row * tiles;
+    const long long left = end - next;
+    count = int(left < tiles - first ? left : tiles - first);
+    next += count;
+    return true;
+  }
+};
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ void lds64(uint32_t a, uint32_t& x, uint32_t& y) {
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(x), "=r"(y) : "r"(a));
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ __nv_bfloat162 as_bf162(uint32_t v) { return *reinterpret_cast<__nv_bfloat162*>(&v); }
+__device__ __forceinline__ uint32_t as_u32(__nv_bfloat162 v) { return *reinterpret_cast<uint32_t*>(&v); }
+
+template <int kD, int kNG>
+__host__ __device__ constexpr int kv4_stage_bytes() {
+  return 2 * kKv4Tile * (kD / 2) + 2 * kKv4Tile * kNG * 4;
+}
+template <int kD, int kNT>
+__host__ __device__ constexpr int kv4_join_bytes() {   // one accumulator per warp, rows padded by four floats, and (maximum, sum)
+  return kKv4Warps * 8 * kNT * ((kD + 4) * 4 + 8);
+}
+template <int kD, int kNG, int kNT>
+__host__ __device__ constexpr int kv4_stages() {
+  // two blocks an SM with eight query heads a block, one with sixteen
+  return ((kNT == 1 ? 113 : 226) * 1024 - 2048 - kv4_join_bytes<kD, kNT>()) / kv4_stage_bytes<kD, kNG>();
+}
+template <int kD, int kNG, int kNT>
+__host__ __device__ constexpr int kv4_smem_bytes() {
+  return 1024 + kv4_stages<kD, kNG, kNT>() * kv4_stage_bytes<kD, kNG>() + kv4_join_bytes<kD, kNT>() + 512;
+}
+
+template <int kD, int kNG, int kNT>
+__global__ void __launch_bounds__(kKv4Threads, kNT == 1 ? 2 : 1)
+kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                  const Kv4Attend p) {
+  constexpr int kRow = kD / 2;                         // bytes of codes a position
+  constexpr int kCodes = kKv4Tile * kRow;
+  constexpr int kScales = kKv4Tile * kNG * 4;
+  constexpr int kStages = kv4_stages<kD, kNG, kNT>();
+  constexpr int kStage = kv4_stage_bytes<kD, kNG>();
+  constexpr int kChunks = kD / 32;                     // 16-byte chunks of a code row
+  constexpr int kMT = kD / 16;                         // channel tiles of the accumulator
+  constexpr int kHeads = 8 * kNT;
+  constexpr int kPitch = kD + 4;
+  static_assert(kStages >= 2, "the ring needs two stages");
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
+  float* join = reinterpret_cast<float*>(smem + kStages * kStage);            // [warp][head][kPitch]
+  float* join_ml = join + kKv4Warps * kHeads * kPitch;                        // [warp][head][2]
+  const uint32_t bars = base + kStages * kStage + kv4_join_bytes<kD, kNT>();
+  auto full = [&](int s) { return bars + 8u * s; };
+  auto empty = [&](int s) { return bars + 8u * (kStages + s); };
+  __shared__ long long locate_scratch[kKv4Threads / 32 + 2];
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), kKv4Warps);
+    }
+    mbar_fence_init();
+    tma_prefetch_desc(&map_k);
+    tma_prefetch_desc(&map_v);
+  }
+  grid_dependency_wait();
+  grid_dependents_may_launch();   // after the wait: the joining kernel may then read the lengths at once
+  const int blocks = gridDim.x, block = blockIdx.x;
+  const Kv4Start start = kv4_locate<kKv4Threads>(p, blocks, block, locate_scratch);   // also orders the barriers
+  Kv4Walk walk(p, start, blocks, block);
+
+  if (warp == kKv4Warps) {
+    // ---------------------------------------------------------- producer
+    uint32_t it = 0;
+    bool ok = true;
+    const int pieces = kKv4Tile / p.box;
+    while (ok && walk.step(p)) {
+      const int kv = walk.row / p.head_blocks;
+      const int* table = p.table + walk.b * p.table_stride;
+      for (int tile = walk.first; tile < walk.first + walk.count; ++tile, ++it) {
+        const int s = it % kStages;
+        ok = __all_sync(0xffffffffu, mbar_wait(empty(s), ((it / kStages) & 1u) ^ 1u, 0x911));
+        if (!ok) break;
+        const int live = min(pieces, (walk.length - tile * kKv4Tile + p.box - 1) / p.box);
+        if (lane == 0) mbar_arrive_expect_tx(full(s), uint32_t(live * p.box) * (2 * kRow + 8 * kNG));
+        __syncwarp();
+        const uint32_t stage = base + s * kStage;
+        for (int c = lane; c < live * 4; c += 32) {
+          const int piece = c >> 2, kind = c & 3;
+          const int position = tile * kKv4Tile + piece * p.box;
+          const int entry = position / p.page;
+          int page = table[entry];
+          if (page < 0 || page >= p.pages) {   // nothing outside the cache is read
+            report_timeout(kSiteKv4Page);
+            page = 0;
+          }
+          const long long row = (static_cast<long long>(page) * p.kv_heads + kv) * p.page + (position - entry * p.page);
+          if (kind < 2)
+            tma_load_3d(stage + kind * kCodes + piece * p.box * kRow, kind ? &map_v : &map_k, full(s), 0, int(row), 0);
+          else
+            bulk_load(stage + 2 * kCodes + (kind - 2) * kScales + piece * p.box * kNG * 4,
+                      (kind == 2 ? p.k_scales : p.v_scales) + row * kNG, uint32_t(p.box) * kNG * 4, full(s));
+        }
+      }
+    }
+    // nothing may still be in flight into this block's shared memory when it ends
+    for (uint32_t back = min(it, uint32_t(kStages)); back > 0; --back)
+      mbar_wait(full((it - back) % kStages), ((it - back) / kStages) & 1u, 0x913);
+  } else {
+    // ---------------------------------------------------------- attention
+    // sequences without a position: nothing to attend to, the output row is zero
+    for (int b = block; b < p.batch; b += blocks) {
+      if (kv4_length(p, b)) continue;
+      for (int i = threadIdx.x; i < p.heads * kD / 8; i += kKv4Warps * 32)
+        reinterpret_cast<uint4*>(p.out)[static_cast<long long>(b) * p.heads * kD / 8 + i] = make_uint4(0, 0, 0, 0);
+      if (p.lse)
+        for (int i = threadIdx.x; i < p.heads; i += kKv4Warps * 32)
+          p.lse[static_cast<long long>(b) * p.heads + i] = -INFINITY;
+    }
+    const int g = lane >> 2, t = lane & 3;
+    // Position within the warp's 16 of row r of a score tile: a permutation of the low three bits, so
+    // that the four positions whose values one load fetches lie in distinct banks.
+    auto position_of = [](int r) {
+      return kD == 128 ? (r & 12) | ((r & 1) << 1) | ((r >> 1) & 1) : (r & 8) | ((r & 1) << 2) | ((r >> 1) & 3);
+    };
+    const int key_row[2] = {warp * 16 + position_of(g), warp * 16 + position_of(g + 8)};
+    const int value_row[4] = {warp * 16 + position_of(2 * t), warp * 16 + position_of(2 * t + 1),
+                              warp * 16 + position_of(2 * t + 8), warp * 16 + position_of(2 * t + 9)};
+    const int value_group = g * (kD / 8) * kNG / kD;
+    uint32_t it = 0;
+    bool ok = true;
+    while (walk.step(p)) {
+      const int kv = walk.row / p.head_blocks, hb = walk.row - kv * p.head_blocks;
+      const int head0 = kv * p.group_heads + hb * kHeads;               // first query head of the block
+      const int heads_here = min(kHeads, p.group_heads - hb * kHeads);
+      // Query fragments: lane (g, t) holds channels 32 j + 8 t + (0..7) of head 8 n + g.
+      uint32_t qf[kNT][kChunks][4];
+      float score_factor[kNT][2], zero_factor[kNT][2][kNG];
+#pragma unroll
+      for (int n = 0; n < kNT; ++n) {
+        float x[kChunks][8], top = 0.0f, sums[kNG];
+#pragma unroll
+        for (int i = 0; i < kNG; ++i) sums[i] = 0.0f;
+        const bool live = n * 8 + g < heads_here;
+        const __nv_bfloat16* src = p.q + walk.b * p.q_batch + (head0 + (live ? n * 8 + g : 0)) * p.q_head;
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j) {
+          const uint4 a = *reinterpret_cast<const uint4*>(src + 32 * j + 8 * t);
+          const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[j][2 * e] = live ? bf16_lo(w[e]) : 0.0f;
+            x[j][2 * e + 1] = live ? bf16_hi(w[e]) : 0.0f;
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            top = fmaxf(top, fabsf(x[j][e]));
+            sums[j * kNG / kChunks] += x[j][e];
+          }
+        }
+#pragma unroll
+        for (int o = 1; o < 4; o *= 2) {
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll
+          for (int i = 0; i < kNG; ++i) sums[i] += __shfl_xor_sync(0xffffffffu, sums[i], o);
+        }
+        // power of two that brings the head's largest element to [2^11, 2^12)
+        int exponent = top > 0.0f && top < INFINITY ? 11 - ilogbf(top) : 0;
+        exponent = min(exponent, 100);
+        const float up = exp2f(static_cast<float>(exponent));
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float f = (e & 1) ? up * 0.0625f : up;      // odd nibbles enter 16 times too large
+            const __half2 h = __floats2half2_rn(x[j][e] * f, x[j][e + 4] * f);
+            qf[n][j][e] = *reinterpret_cast<const uint32_t*>(&h);
+          }
+        // scores: lane (g, t) holds heads 2 t and 2 t + 1 of the tile
+        const float factor = exp2f(static_cast<float>(-exponent)) * p.scale_log2;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          score_factor[n][c] = __shfl_sync(0xffffffffu, factor, 4 * (2 * t + c));
+#pragma unroll
+          for (int i = 0; i < kNG; ++i)
+            zero_factor[n][c][i] = __shfl_sync(0xffffffffu, sums[i], 4 * (2 * t + c)) * p.scale_log2;
+        }
+      }
+      float acc[kNT][kMT][4], top[kNT][2], sum[kNT][2];
+#pragma unroll
+      for (int n = 0; n < kNT; ++n) {
+#pragma unroll
+        for (int i = 0; i < kMT; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[n][i][e] = 0.0f;
+        top[n][0] = top[n][1] = -INFINITY;
+        sum[n][0] = sum[n][1] = 0.0f;
+      }
+      for (int tile = walk.first; tile < walk.first + walk.count; ++tile, ++it) {
+        const int s = it % kStages;
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(full(s), (it / kStages) & 1u, 0x912));
+        const int live = walk.length - tile * kKv4Tile;     // positions of the tile that exist
+        if (ok && warp * 16 < live) {
+          const uint32_t keys = base + s * kStage, values = keys + kCodes;
+          const uint32_t key_scales = values + kCodes, value_scales = key_scales + kScales;
+          float score[kNT][4];
+#pragma unroll
+          for (int n = 0; n < kNT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) score[n][e] = 0.0f;
+#pragma unroll
+          for (int i = 0; i < kNG; ++i) {
+            float dot[kNT][4];
+#pragma unroll
+            for (int n = 0; n < kNT; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) dot[n][e] = 0.0f;
+#pragma unroll
+            for (int jj = 0; jj < kChunks / kNG; ++jj) {
+              const int j = i * (kChunks / kNG) + jj;
+              uint32_t w[2];
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                const int row = key_row[r];
+                const int swizzle = kD == 128 ? (row >> 1) & 3 : (row >> 2) & 1;
+                w[r] = lds32(keys + row * kRow + ((j ^ swizzle) << 4) + t * 4);
+              }
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                const uint32_t a[4] = {w[0] & 0x000f000fu, w[1] & 0x000f000fu, w[0] & 0x00f000f0u, w[1] & 0x00f000f0u};
+#pragma unroll
+                for (int n = 0; n < kNT; ++n) mma_f16(dot[n], a, qf[n][j][2 * half], qf[n][j][2 * half + 1]);
+                w[0] >>= 8;
+                w[1] >>= 8;
+              }
+            }
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const uint32_t pair = lds32(key_scales + (key_row[r] * kNG + i) * 4);
+              const float scale = bf16_lo(pair), zero = bf16_hi(pair);
+#pragma unroll
+              for (int n = 0; n < kNT; ++n)
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+                  score[n][2 * r + c] = fmaf(dot[n][2 * r + c] * 0x1p24f * score_factor[n][c], scale,
+                                             fmaf(zero, zero_factor[n][c][i], score[n][2 * r + c]));
+            }
+          }
+          if (warp * 16 + 16 > live) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+              if (key_row[r] >= live)
+#pragma unroll
+                for (int n = 0; n < kNT; ++n) score[n][2 * r] = score[n][2 * r + 1] = -INFINITY;
+          }
+          // The maximum is raised only when a score exceeds it by more than 2^8: exponentials stay
+          // below 2^8, and most tiles need neither the shuffles nor the rescaling.
+          bool raise = false;
+#pragma unroll
+          for (int n = 0; n < kNT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) raise |= score[n][e] > top[n][e & 1] + 8.0f;
+          if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+            for (int n = 0; n < kNT; ++n)
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                float m = fmaxf(top[n][c], fmaxf(score[n][c], score[n][2 + c]));
+#pragma unroll
+                for (int o = 4; o < 32; o *= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                const float f = m == -INFINITY ? 1.0f : exp2f(top[n][c] - m);
+                top[n][c] = m;
+                sum[n][c] *= f;
+#pragma unroll
+                for (int i = 0; i < kMT; ++i) {
+                  acc[n][i][c] *= f;
+                  acc[n][i][2 + c] *= f;
+                }
+              }
+          }
+          uint32_t pf[kNT][2];
+#pragma unroll
+          for (int n = 0; n < kNT; ++n) {
+            float e[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const float m = top[n][c & 1];
+              e[c] = exp2f(score[n][c] - (m == -INFINITY ? 0.0f : m));
+              sum[n][c & 1] += e[c];
+            }
+            pf[n][0] = transpose_8x8(pack_bf16x2(e[0], e[1]));
+            pf[n][1] = transpose_8x8(pack_bf16x2(e[2], e[3]));
+          }
+          // values: lane (g, t) holds channels kD / 8 * g + (0 ..) of four positions
+          uint32_t pair[4], codes[4][2];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int row = value_row[i];
+            pair[i] = lds32(value_scales + (row * kNG + value_group) * 4);
+            if (warp * 16 + 16 > live && row >= live) pair[i] = 0;     // what lies behind the sequence counts as zero
+            if (kD == 128) {
+              lds64(values + row * kRow + (((g >> 1) ^ ((row >> 1) & 3)) << 4) + (g & 1) * 8, codes[i][0], codes[i][1]);
+            } else {
+              const uint32_t w = lds32(values + row * kRow + (((g >> 2) ^ ((row >> 2) & 1)) << 4) + (g & 3) * 4);
+              codes[i][0] = w;
+              codes[i][1] = w >> 16;
+            }
+          }
+          const __nv_bfloat162 offset = __float2bfloat162_rn(128.0f);
+          __nv_bfloat162 scale2[2], zero2[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            scale2[h] = as_bf162(__byte_perm(pair[2 * h], pair[2 * h + 1], 0x5410));
+            zero2[h] = as_bf162(__byte_perm(pair[2 * h], pair[2 * h + 1], 0x7632));
+          }
+          constexpr int kQuads = kD == 128 ? 2 : 1;          // 16-bit quads of codes in each half row
+#pragma unroll
+          for (int quad = 0; quad < kQuads; ++quad) {
+            uint32_t w[4];                                   // (row g, row g + 8) x (positions 2t.., 2t + 8..)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int r = 0; r < 2; ++r)
+                w[2 * h + r] = __byte_perm(codes[2 * h][r], codes[2 * h + 1][r], quad ? 0x7632 : 0x5410);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t a[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const uint32_t raw = ((w[e] >> (4 * i)) & 0x000f000fu) | 0x43004300u;   // 128 + code
+                a[e] = as_u32(__hfma2(__hsub2(as_bf162(raw), offset), scale2[e >> 1], zero2[e >> 1]));
+              }
+#pragma unroll
+              for (int n = 0; n < kNT; ++n) mma_bf16(acc[n][quad * 4 + i], a, pf[n][0], pf[n][1]);
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty(s));
+      }
+      // ---- the eight warps' parts of this piece meet
+#pragma unroll
+      for (int n = 0; n < kNT; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+          for (int o = 4; o < 32; o *= 2) sum[n][c] += __shfl_xor_sync(0xffffffffu, sum[n][c], o);
+          float* mine = join + (warp * kHeads + n * 8 + 2 * t + c) * kPitch + g * (kD / 8);
+          // channel g * kD / 8 + i of the lower half row, + kD / 16 + i of the upper one
+#pragma unroll
+          for (int i = 0; i < kMT; ++i) {
+            mine[i] = acc[n][i][c];
+            mine[kMT + i] = acc[n][i][2 + c];
+          }
+          if (g == 0) {
+            join_ml[(warp * kHeads + n * 8 + 2 * t + c) * 2] = top[n][c];
+            join_ml[(warp * kHeads + n * 8 + 2 * t + c) * 2 + 1] = sum[n][c];
+          }
+        }
+      asm volatile("bar.sync 1, %0;" ::"n"(kKv4Warps * 32) : "memory");
+      const bool whole = walk.count == walk.tiles;
+      const int slot = walk.first == 0 ? 1 : 0;   // part 0: the row began in an earlier block
+      for (int i = threadIdx.x; i < heads_here * (kD / 4); i += kKv4Warps * 32) {
+        const int head = i / (kD / 4), channel = (i - head * (kD / 4)) * 4;
+        float m = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kKv4Warps; ++w) m = fmaxf(m, join_ml[(w * kHeads + head) * 2]);
+        float total = 0.0f;
+        float4 o = make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int w = 0; w < kKv4Warps; ++w) {
+          const float mw = join_ml[(w * kHeads + head) * 2];
+          const float f = mw == -INFINITY ? (join_ml[(w * kHeads + head) * 2 + 1] == 0.0f ? 0.0f : 1.0f) : exp2f(mw - m);
+          const float4 x = *reinterpret_cast<const float4*>(join + (w * kHeads + head) * kPitch + channel);
+          total = fmaf(join_ml[(w * kHeads + head) * 2 + 1], f, total);
+          o.x = fmaf(x.x, f, o.x);
+          o.y = fmaf(x.y, f, o.y);
+          o.z = fmaf(x.z, f, o.z);
+          o.w = fmaf(x.w, f, o.w);
+        }
+        if (whole) {
+          const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+          const long long at = static_cast<long long>(walk.b) * p.heads + head0 + head;
+          *reinterpret_cast<uint2*>(p.out + at * kD + channel) =
+              make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+          if (p.lse && channel == 0) p.lse[at] = (m + log2f(total)) * 0.69314718055994531f;
+        } else {
+          const long long at = (static_cast<long long>(block) * 2 + slot) * kHeads + head;
+          *reinterpret_cast<float4*>(p.parts + at * kD + channel) = o;
+          if (channel == 0) {
+            float* ml = p.parts + static_cast<long long>(blocks) * 2 * kHeads * kD + at * 2;
+            ml[0] = m;
+            ml[1] = total;
+          }
+        }
+      }
+      asm volatile("bar.sync 1, %0;" ::"n"(kKv4Warps * 32) : "memory");   // the join area is free again
+    }
+  }
+}
+
+// Joins the parts of the rows that the runs cut: block i looks at the boundary between runs i and
+// i + 1 and serves the row there if it is the row's first boundary.  One head per blockIdx.y.
+template <int kD>
+__global__ void __launch_bounds__(kD) kv4_join_kernel(const Kv4Attend p, int blocks, int heads_per_block) {
+  __shared__ long long scratch[kD / 32 + 2];
+  grid_dependents_may_launch();
+  const int boundary = blockIdx.x + 1;
+  const Kv4Start s = kv4_locate<kD>(p, blocks, boundary, scratch);   // reads only the lengths
+  grid_dependency_wait();
+  const long long tile = kv4_first_tile(s.total, blocks, boundary);
+  if (s.total == 0 || tile >= s.total) return;
+  const int tiles = kv4_tiles(kv4_length(p, s.sequence));
+  const int row = int((tile - s.tile_base) / tiles);
+  const long long begin = s.tile_base + static_cast<long long>(row) * tiles;
+  if (begin == tile) return;                                          // the boundary falls between two rows
+  const int first = kv4_block_of(s.total, blocks, begin), last = kv4_block_of(s.total, blocks, begin + tiles - 1);
+  if (kv4_first_tile(s.total, blocks, boundary - 1) > begin) return;  // not the first boundary inside the row
+  const int kv = row / p.head_blocks, hb = row - kv * p.head_blocks;
+  const int head = blockIdx.y;
+  if (hb * heads_per_block + head >= p.group_heads) return;
+  const float* ml = p.parts + static_cast<long long>(blocks) * 2 * heads_per_block * kD;
+  float m = -INFINITY;
+  auto part_of = [&](int c) { return (static_cast<long long>(c) * 2 + (c == first ? 1 : 0)) * heads_per_block + head; };
+  auto held = [&](int c) { return kv4_first_tile(s.total, blocks, c) != kv4_first_tile(s.total, blocks, c + 1); };
+  for (int c = first; c <= last; ++c)
+    if (held(c)) m = fmaxf(m, ml[part_of(c) * 2]);
+  float total = 0.0f, o = 0.0f;
+#pragma unroll 4
+  for (int c = first; c <= last; ++c) {
+    if (!held(c)) continue;
+    const float mc = ml[part_of(c) * 2], lc = ml[part_of(c) * 2 + 1];
+    const float f = mc == -INFINITY ? (lc == 0.0f ? 0.0f : 1.0f) : exp2f(mc - m);
+    total = fmaf(lc, f, total);
+    o = fmaf(p.parts[part_of(c) * kD + threadIdx.x], f, o);
+  }
+  const long long at = static_cast<long long>(s.sequence) * p.heads + kv * p.group_heads + hb * heads_per_block + head;
+  p.out[at * kD + threadIdx.x] = __float2bfloat16(total == 0.0f ? 0.0f : o / total);
+  if (p.lse && threadIdx.x == 0) p.lse[at] = (m + log2f(total)) * 0.69314718055994531f;
+}
+
+int check_kv4_cache(const char* what, const trinity_sm100_kv4_cache& c) {
+  if (!c.k_codes || !c.k_scales || !c.v_codes || !c.v_scales) return fail(TRINITY_SM100_E_INVALID, "%s: null cache pointer", what);
+  if (!aligned16(c.k_codes) || !aligned16(c.k_scales) || !aligned16(c.v_codes) || !aligned16(c.v_scales))
+    return fail(TRINITY_SM100_E_INVALID, "%s: cache pointers must be 16-byte aligned", what);
+  if (c.head_dim != 64 && c.head_dim != 128)
+    return fail(TRINITY_SM100_E_UNSUPPORTED, "%s: head_dim %d (64 and 128 are supported)", what, c.head_dim);
+  if ((c.group != 32 && c.group != 64 && c.group != 128) || c.group > c.head_dim)
+    return fail(TRINITY_SM100_E_UNSUPPORTED, "%s: groups of %d channels (32, 64 and 128, at most head_dim)", what, c.group);
+  if (c.pages <= 0 || c.kv_heads <= 0 || c.page <= 0) return fail(TRINITY_SM100_E_INVALID, "%s: empty cache", what);
+  if (c.page % 16) return fail(TRINITY_SM100_E_UNSUPPORTED, "%s: a page of %d positions (multiples of 16)", what, c.page);
+  if (static_cast<long long>(c.pages) * c.kv_heads > INT32_MAX / c.page)
+    return fail(TRINITY_SM100_E_UNSUPPORTED, "%s: the cache has 2^31 rows or more", what);
+  return 0;
+}
+
+Kv4Rows kv4_rows(const trinity_sm100_kv4_cache& c, const trinity_sm100_kv4_rows& r) {
+  Kv4Rows p = {};
+  p.codes[0] = static_cast<uint8_t*>(c.k_codes);
+  p.codes[1] = static_cast<uint8_t*>(c.v_codes);
+  p.scales[0] = static_cast<__nv_bfloat162*>(c.k_scales);
+  p.scales[1] = static_cast<__nv_bfloat162*>(c.v_scales);
+  p.slots = reinterpret_cast<const long long*>(r.slots);
+  p.tokens = r.tokens;
+  p.positions = static_cast<long long>(c.pages) * c.page;
+  p.token_stride[0] = r.k_token_stride;
+  p.token_stride[1] = r.v_token_stride;
+  p.head_stride[0] = r.k_head_stride;
+  p.head_stride[1] = r.v_head_stride;
+  p.kv_heads = c.kv_heads;
+  p.page = c.page;
+  p.group = c.group;
+  return p;
+}
+
+int check_kv4_rows(const char* what, const trinity_sm100_kv4_cache& c, const trinity_sm100_kv4_rows& r) {
+  if (int rc = check_kv4_cache(what, c)) return rc;
+  if (!r.k || !r.v || !r.slots) return fail(TRINITY_SM100_E_INVALID, "%s: null pointer", what);
+  if (r.tokens <= 0) return fail(TRINITY_SM100_E_INVALID, "%s: empty extent", what);
+  if (r.tokens > INT32_MAX / (16 * c.kv_heads)) return fail(TRINITY_SM100_E_UNSUPPORTED, "%s: too many tokens", what);
+  if (reinterpret_cast<uintptr_t>(r.slots) % 8) return fail(TRINITY_SM100_E_INVALID, "%s: slots must be 8-byte aligned", what);
+  return 0;
+}
+
+template <int kD, int kNG, int kNT>
+int launch_kv4_attend(const Kv4Attend& p, const CUtensorMap& map_k, const CUtensorMap& map_v, int blocks, cudaStream_t stream) {
+  static unsigned long long opted = 0;
+  constexpr int kSmem = kv4_smem_bytes<kD, kNG, kNT>();
+  static_assert(kSmem <= 232448, "exceeds the 227 KB shared-memory limit");
+  auto kernel = kv4_attend_kernel<kD, kNG, kNT>;
+  if (int rc = opt_in_shared_memory(reinterpret_cast<const void*>(kernel), kSmem, &opted, "kv4_decode")) return rc;
+  {
+    KernelLaunch launch(dim3(blocks), dim3(kKv4Threads), kSmem, stream);
+    cudaError_t e = cudaLaunchKernelEx(&launch.config, kernel, map_k, map_v, p);
+    if (e != cudaSuccess) return fail(TRINITY_SM100_E_CUDA, "kv4_attend launch: %s", cudaGetErrorString(e));
+    count_launch();
+  }
+  if (blocks > 1) {
+    KernelLaunch launch(dim3(blocks - 1, 8 * kNT), dim3(kD), 0, stream);
+    cudaError_t e = cudaLaunchKernelEx(&launch.config, kv4_join_kernel<kD>, p, blocks, 8 * kNT);
+    if (e != cudaSuccess) return fail(TRINITY_SM100_E_CUDA, "kv4_join launch: %s", cudaGetErrorString(e));
+    count_launch();
+  }
+  return check_launch("kv4_decode");
+}
+
+int kv4_blocks(int sm_count, int group_heads) { return group_heads > 8 ? sm_count : 2 * sm_count; }
+
+}  // namespace
+}  // namespace trinity_sm100
+
+using namespace trinity_sm100;
+
+extern "C" int trinity_sm100_kv4_append(const trinity_sm100_kv4_cache* cache, const trinity_sm100_kv4_rows* rows,
+                                        void* stream_handle) {
+  if (!cache || !rows) return fail(TRINITY_SM100_E_INVALID, "kv4_append: null argument block");
+  const trinity_sm100_kv4_rows& r = *rows;
+  if (int rc = check_kv4_rows("kv4_append", *cache, r)) return rc;
+  if (reinterpret_cast<uintptr_t>(r.k) % 2 || reinterpret_cast<uintptr_t>(r.v) % 2)
+    return fail(TRINITY_SM100_E_INVALID, "kv4_append: a pointer is not aligned to its element type");
+  if (int rc = require_sm100(nullptr)) return rc;
+  Kv4Rows p = kv4_rows(*cache, r);
+  p.in[0] = static_cast<const __nv_bfloat16*>(r.k);
+  p.in[1] = static_cast<const __nv_bfloat16*>(r.v);
+  // 16-byte loads where every row starts on 16 bytes
+  const bool vectors = aligned16(r.k) && aligned16(r.v) && r.k_token_stride % 8 == 0 && r.v_token_stride % 8 == 0 &&
+                       r.k_head_stride % 8 == 0 && r.v_head_stride % 8 == 0;
+  const long long threads = r.tokens * cache->kv_heads * (cache->head_dim / 8);
+  KernelLaunch launch(dim3(unsigned((threads + 255) / 256), 2), dim3(256), 0, static_cast<cudaStream_t>(stream_handle));
+  cudaError_t e;
+  if (cache->head_dim == 128)
+    e = vectors ? cudaLaunchKernelEx(&launch.config, kv4_append_kernel<128, true>, p)
+                : cudaLaunchKernelEx(&launch.config, kv4_append_kernel<128, false>, p);
+  else
+    e = vectors ? cudaLaunchKernelEx(&launch.config, kv4_append_kernel<64, true>, p)
+                : cudaLaunchKernelEx(&launch.config, kv4_append_kernel<64, false>, p);
+  if (e != cudaSuccess) return fail(TRINITY_SM100_E_CUDA, "kv4_append launch: %s", cudaGetErrorString(e));
+  count_launch();
+  return check_launch("kv4_append");
+}
+
+extern "C" int trinity_sm100_kv4_read(const trinity_sm100_kv4_cache* cache, const trinity_sm100_kv4_rows* rows,
+                                      int32_t out_dtype, void* stream_handle) {
+  if (!cache || !rows) return fail(TRINITY_SM100_E_INVALID, "kv4_read: null argument block");
+  const trinity_sm100_kv4_rows& r = *rows;
+  if (int rc = check_kv4_rows("kv4_read", *cache, r)) return rc;
+  if (out_dtype != TRINITY_SM100_BF16 && out_dtype != TRINITY_SM100_FP32)
+    return fail(TRINITY_SM100_E_INVALID, "kv4_read: unknown output dtype %d", out_dtype);
+  const int unit = out_dtype == TRINITY_SM100_FP32 ? 4 : 8;
+  if (!aligned16(r.k) || !aligned16(r.v) || r.k_token_stride % unit || r.v_token_stride % unit || r.k_head_stride % unit ||
+      r.v_head_stride % unit)
+    return fail(TRINITY_SM100_E_INVALID, "kv4_read: output rows must start on 16 bytes");
+  if (int rc = require_sm100(nullptr)) return rc;
+  Kv4Rows p = kv4_rows(*cache, r);
+  p.out[0] = r.k;
+  p.out[1] = r.v;
+  p.out_f32 = out_dtype == TRINITY_SM100_FP32;
+  const long long threads = r.tokens * cache->kv_heads * (cache->head_dim / 8);
+  KernelLaunch launch(dim3(unsigned((threads + 255) / 256), 2), dim3(256), 0, static_cast<cudaStream_t>(stream_handle));
+  cudaError_t e = cache->head_dim == 128 ? cudaLaunchKernelEx(&launch.config, kv4_read_kernel<128>, p)
+                                         : cudaLaunchKernelEx(&launch.config, kv4_read_kernel<64>, p);
+  if (e != cudaSuccess) return fail(TRINITY_SM100_E_CUDA, "kv4_read launch: %s", cudaGetErrorString(e));
+  count_launch();
+  return check_launch("kv4_read");
+}
+
+extern "C" size_t trinity_sm100_kv4_decode_workspace_bytes(int32_t heads, int32_t kv_heads, int32_t head_dim) {
+  int sm_count = 0;
+  if (heads <= 0 || kv_heads <= 0 || head_dim <= 0 || heads % kv_heads || require_sm100(&sm_count)) return 0;
+  const int group_heads = heads / kv_heads;
+  return size_t(kv4_blocks(sm_count, group_heads)) * 2 * (group_heads > 8 ? 16 : 8) * (size_t(head_dim) + 2) * 4;
+}
+
+extern "C" int trinity_sm100_kv4_decode(const trinity_sm100_kv4_cache* cache, const trinity_sm100_kv4_decode_args* args,
+                                        void* stream_handle) {
+  if (!cache || !args) return fail(TRINITY_SM100_E_INVALID, "kv4_decode: null argument block");
+  const trinity_sm100_kv4_cache& c = *cache;
+  const trinity_sm100_kv4_decode_args& a = *args;
+  if (int rc = check_kv4_cache("kv4_decode", c)) return rc;
+  if (!a.q || !a.out || !a.page_table || !a.lengths || !a.workspace) return fail(TRINITY_SM100_E_INVALID, "kv4_decode: null pointer");
+  if (a.batch <= 0 || a.heads <= 0 || a.max_pages <= 0) return fail(TRINITY_SM100_E_INVALID, "kv4_decode: empty extent");
+  if (a.heads % c.kv_heads)
+    return fail(TRINITY_SM100_E_INVALID, "kv4_decode: %d query heads do not divide over %d cached ones", a.heads, c.kv_heads);
+  if (a.table_stride < a.max_pages) return fail(TRINITY_SM100_E_INVALID, "kv4_decode: table stride smaller than its row");
+  if (!aligned16(a.q) || a.q_batch_stride % 8 || a.q_head_stride % 8)
+    return fail(TRINITY_SM100_E_INVALID, "kv4_decode: query rows must start on 16 bytes");
+  if (!aligned16(a.out) || !aligned16(a.workspace)) return fail(TRINITY_SM100_E_INVALID, "kv4_decode: pointers must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(a.page_table) % 4 || reinterpret_cast<uintptr_t>(a.lengths) % 4 ||
+      reinterpret_cast<uintptr_t>(a.lse) % 4)
+    return fail(TRINITY_SM100_E_INVALID, "kv4_decode: a pointer is not aligned to its element type");
+  if (static_cast<long long>(a.max_pages) * c.page > INT32_MAX - kKv4Tile)
+    return fail(TRINITY_SM100_E_UNSUPPORTED, "kv4_decode: a table row covers 2^31 positions or more");
+  int sm_count = 0;
+  if (int rc = require_sm100(&sm_count)) return rc;
+  const size_t need = trinity_sm100_kv4_decode_workspace_bytes(a.heads, c.kv_heads, c.head_dim);
+  if (a.workspace_bytes < need)
+    return fail(TRINITY_SM100_E_INVALID, "kv4_decode: workspace of %zu bytes, %zu needed", a.workspace_bytes, need);
+  Kv4Attend p;
+  p.q = static_cast<const __nv_bfloat16*>(a.q);
+  p.k_scales = static_cast<const __nv_bfloat162*>(c.k_scales);
+  p.v_scales = static_cast<const __nv_bfloat162*>(c.v_scales);
+  p.table = static_cast<const int*>(a.page_table);
+  p.lengths = static_cast<const int*>(a.lengths);
+  p.out = static_cast<__nv_bfloat16*>(a.out);
+  p.lse = static_cast<float*>(a.lse);
+  p.parts = static_cast<float*>(a.workspace);
+  p.q_batch = a.q_batch_stride;
+  p.q_head = a.q_head_stride;
+  p.table_stride = a.table_stride;
+  p.batch = a.batch;
+  p.heads = a.heads;
+  p.kv_heads = c.kv_heads;
+  p.group_heads = a.heads / c.kv_heads;
+  const int block_heads = p.group_heads > 8 ? 16 : 8;
+  p.head_blocks = (p.group_heads + block_heads - 1) / block_heads;
+  p.pages = c.pages;
+  p.page = c.page;
+  p.max_pages = a.max_pages;
+  p.box = kKv4Tile;                     // positions a copy fetches: the largest power of two that pages and tiles share
+  while (c.page % p.box) p.box /= 2;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  CUtensorMap map_k, map_v;
+  const uint64_t rows = static_cast<uint64_t>(c.pages) * c.kv_heads * c.page;
+  const int row_bytes = c.head_dim / 2;
+  if (int rc = make_tensor_map_3d(&map_k, c.k_codes, 2, row_bytes / 2, rows, 1, row_bytes, row_bytes * rows, row_bytes / 2, p.box, 1, row_bytes))
+    return rc;
+  if (int rc = make_tensor_map_3d(&map_v, c.v_codes, 2, row_bytes / 2, rows, 1, row_bytes, row_bytes * rows, row_bytes / 2, p.box, 1, row_bytes))
+    return rc;
+  const int blocks = kv4_blocks(sm_count, p.group_heads);
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
+  const int groups = c.head_dim / c.group;
+#define TRINITY_KV4(D, NG) \
+  return block_heads == 8 ? launch_kv4_attend<D, NG, 1>(p, map_k, map_v, blocks, stream) \
+                          : launch_kv4_attend<D, NG, 2>(p, map_k, map_v, blocks, stream);
+  if (c.head_dim == 128) {
+    if (groups == 1) TRINITY_KV4(128, 1)
+    if (groups == 2) TRINITY_KV4(128, 2)
+    TRINITY_KV4(128, 4)
+  }
+  if (groups == 1) TRINITY_KV4(64, 1)
+  TRINITY_KV4(64, 2)
+#undef TRINITY_KV4
+}

@@ -7,5 +7,6 @@
 #include "block_norm.cu"
 #include "pointwise.cu"
 #include "mla_decode.cu"
+#include "kv4.cu"
 #include "allreduce.cu"
 #include "allgather.cu"

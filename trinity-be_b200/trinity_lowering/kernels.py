@@ -30,6 +30,10 @@ EXPORTS = (
     "trinity_sm100_mla_schedule_segment",
     "trinity_sm100_mla_decode_bf16",
     "trinity_sm100_mla_decode_bf16_noalloc",
+    "trinity_sm100_kv4_append",
+    "trinity_sm100_kv4_read",
+    "trinity_sm100_kv4_decode_workspace_bytes",
+    "trinity_sm100_kv4_decode",
     "trinity_sm100_allreduce_flag_words",
     "trinity_sm100_allreduce_bf16",
     "trinity_sm100_allgather_bf16",
@@ -101,6 +105,36 @@ class MlaArgs(ctypes.Structure):
     ]
 
 
+class Kv4CacheArgs(ctypes.Structure):
+    _fields_ = [
+        ("k_codes", ctypes.c_void_p), ("k_scales", ctypes.c_void_p),
+        ("v_codes", ctypes.c_void_p), ("v_scales", ctypes.c_void_p),
+        ("pages", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("page", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("group", ctypes.c_int32), ("reserved", ctypes.c_int32),
+    ]
+
+
+class Kv4RowsArgs(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("slots", ctypes.c_void_p),
+        ("tokens", ctypes.c_int64),
+        ("k_token_stride", ctypes.c_int64), ("k_head_stride", ctypes.c_int64),
+        ("v_token_stride", ctypes.c_int64), ("v_head_stride", ctypes.c_int64),
+    ]
+
+
+class Kv4DecodeArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("page_table", ctypes.c_void_p), ("lengths", ctypes.c_void_p),
+        ("out", ctypes.c_void_p), ("lse", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+        ("q_batch_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64),
+        ("table_stride", ctypes.c_int64),
+        ("batch", ctypes.c_int32), ("heads", ctypes.c_int32), ("max_pages", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+    ]
+
+
 class AllReduceArgs(ctypes.Structure):
     _fields_ = [
         ("peers", ctypes.POINTER(ctypes.c_void_p)), ("flags", ctypes.POINTER(ctypes.c_void_p)),
@@ -143,6 +177,14 @@ def library():
             lib.trinity_sm100_mla_decode_bf16.argtypes = [ctypes.POINTER(MlaArgs), ctypes.c_void_p]
             lib.trinity_sm100_mla_decode_bf16_noalloc.argtypes = [
                 ctypes.POINTER(MlaArgs), ctypes.c_void_p]
+            lib.trinity_sm100_kv4_append.argtypes = [
+                ctypes.POINTER(Kv4CacheArgs), ctypes.POINTER(Kv4RowsArgs), ctypes.c_void_p]
+            lib.trinity_sm100_kv4_read.argtypes = [
+                ctypes.POINTER(Kv4CacheArgs), ctypes.POINTER(Kv4RowsArgs), ctypes.c_int32, ctypes.c_void_p]
+            lib.trinity_sm100_kv4_decode_workspace_bytes.argtypes = [ctypes.c_int32] * 3
+            lib.trinity_sm100_kv4_decode_workspace_bytes.restype = ctypes.c_size_t
+            lib.trinity_sm100_kv4_decode.argtypes = [
+                ctypes.POINTER(Kv4CacheArgs), ctypes.POINTER(Kv4DecodeArgs), ctypes.c_void_p]
             lib.trinity_sm100_allreduce_flag_words.restype = ctypes.c_size_t
             lib.trinity_sm100_allreduce_bf16.argtypes = [
                 ctypes.POINTER(AllReduceArgs), ctypes.c_void_p]
@@ -498,6 +540,154 @@ def mla_decode_noalloc(q, cache, scale, d_v=512, kv_splits=0, out=None, stream=N
     with torch.cuda.device(q.device):
         _check(library().trinity_sm100_mla_decode_bf16_noalloc(ctypes.byref(args), _stream(stream)))
     return out
+
+
+class Kv4Cache:
+    """A paged key/value cache held in 4 bits (see ``trinity_sm100_kv4_cache`` for the format):
+    codes uint8 [pages, kv_heads, page, head_dim / 2], scales BF16 [pages, kv_heads, page,
+    head_dim / group, 2] with (scale, zero) pairs.  ``kv4_cache`` makes an empty one."""
+
+    def __init__(self, k_codes, k_scales, v_codes, v_scales):
+        if k_codes.dim() != 4 or k_scales.dim() != 5 or k_scales.shape[4] != 2:
+            raise ValueError("Kv4Cache: codes are [pages, kv_heads, page, head_dim / 2], "
+                             "scales [pages, kv_heads, page, head_dim / group, 2]")
+        pages, kv_heads, page, half = k_codes.shape
+        groups = k_scales.shape[3]
+        if (k_scales.shape[:3] != k_codes.shape[:3] or v_codes.shape != k_codes.shape
+                or v_scales.shape != k_scales.shape or groups == 0 or (2 * half) % groups):
+            raise ValueError("Kv4Cache: codes and scales disagree")
+        for name, t, dtype in (("k_codes", k_codes, torch.uint8), ("v_codes", v_codes, torch.uint8),
+                               ("k_scales", k_scales, torch.bfloat16), ("v_scales", v_scales, torch.bfloat16)):
+            _require(t, dtype, name)
+            if not t.is_contiguous() or t.device != k_codes.device:
+                raise ValueError(f"Kv4Cache: {name} must be contiguous and on {k_codes.device}")
+        self.k_codes, self.k_scales, self.v_codes, self.v_scales = k_codes, k_scales, v_codes, v_scales
+        self.pages, self.kv_heads, self.page = pages, kv_heads, page
+        self.head_dim, self.group = 2 * half, 2 * half // groups
+        self.device = k_codes.device
+        self.args = Kv4CacheArgs(k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(),
+                                 pages, kv_heads, page, self.head_dim, self.group, 0)
+
+    @property
+    def tensors(self):
+        return self.k_codes, self.k_scales, self.v_codes, self.v_scales
+
+
+def kv4_cache(pages, kv_heads, page, head_dim, group=None, device="cuda"):
+    """An empty ``Kv4Cache`` of ``pages`` pages of ``page`` positions, quantised in groups of
+    ``group`` channels (default: the whole head)."""
+    group = head_dim if group is None else group
+    if group <= 0 or head_dim % group:
+        raise ValueError(f"kv4_cache: groups of {group} do not divide {head_dim} channels")
+    codes = [torch.zeros((pages, kv_heads, page, head_dim // 2), dtype=torch.uint8, device=device) for _ in range(2)]
+    scales = [torch.zeros((pages, kv_heads, page, head_dim // group, 2), dtype=torch.bfloat16, device=device)
+              for _ in range(2)]
+    return Kv4Cache(codes[0], scales[0], codes[1], scales[1])
+
+
+def _kv4_rows(what, cache, k, v, slots):
+    expected = (slots.shape[0] if slots.dim() == 1 else -1, cache.kv_heads, cache.head_dim)
+    if tuple(k.shape) != expected or tuple(v.shape) != expected or k.stride(2) != 1 or v.stride(2) != 1:
+        raise ValueError(f"{what}: k and v must be [tokens, {cache.kv_heads}, {cache.head_dim}] with a unit inner "
+                         "stride and slots [tokens]")
+    _require(slots, torch.int64, "slots")
+    if not slots.is_contiguous():
+        raise ValueError(f"{what}: slots must be contiguous")
+    _same_device(cache.device, k=k, v=v, slots=slots)
+    return Kv4RowsArgs(k.data_ptr(), v.data_ptr(), slots.data_ptr(), expected[0], k.stride(0), k.stride(1),
+                       v.stride(0), v.stride(1))
+
+
+def kv4_append(cache, k, v, slots, stream=None):
+    """Quantises the BF16 rows ``k`` and ``v`` [tokens, kv_heads, head_dim] (views with any token and
+    head stride) into ``cache`` at positions ``slots`` (int64 [tokens]; distinct; negative: token not
+    written); see ``trinity_sm100_kv4_append``."""
+    _require(k, torch.bfloat16, "k")
+    _require(v, torch.bfloat16, "v")
+    args = _kv4_rows("kv4_append", cache, k, v, slots)
+
+    def launch(handle):
+        _check(library().trinity_sm100_kv4_append(ctypes.byref(cache.args), ctypes.byref(args), handle))
+
+    _submit(cache.device, stream, (k, v, slots, *cache.tensors), launch)
+
+
+def kv4_read(cache, slots, *, dtype=torch.bfloat16, k_out=None, v_out=None, stream=None):
+    """The keys and values [tokens, kv_heads, head_dim] that ``cache`` holds at positions ``slots``
+    (int64 [tokens]; negative: zeros), in BF16 or FP32; see ``trinity_sm100_kv4_read``."""
+    if (k_out is None) != (v_out is None):
+        raise ValueError("kv4_read: give both outputs or none")
+    if k_out is not None:
+        dtype = k_out.dtype
+        if v_out.dtype != dtype:
+            raise ValueError("kv4_read: the outputs differ in type")
+    if dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("kv4_read: dtype must be bf16 or fp32")
+    code = DT_FP32 if dtype == torch.float32 else DT_BF16
+
+    def launch(handle):
+        if k_out is None:
+            shape = (slots.shape[0] if slots.dim() == 1 else -1, cache.kv_heads, cache.head_dim)
+            if shape[0] < 0:
+                raise ValueError("kv4_read: slots must be [tokens]")
+            k, v = (torch.empty(shape, dtype=dtype, device=cache.device) for _ in range(2))
+        else:
+            k, v = k_out, v_out
+        args = _kv4_rows("kv4_read", cache, k, v, slots)
+        _check(library().trinity_sm100_kv4_read(ctypes.byref(cache.args), ctypes.byref(args), code, handle))
+        return k, v
+
+    return _submit(cache.device, stream, (slots, k_out, v_out, *cache.tensors), launch)
+
+
+def kv4_decode_workspace_bytes(heads, kv_heads, head_dim):
+    """Bytes of workspace that ``kv4_decode`` needs on the current device."""
+    return int(library().trinity_sm100_kv4_decode_workspace_bytes(heads, kv_heads, head_dim))
+
+
+def kv4_decode(q, cache, page_table, lengths, scale, *, out=None, lse=None, workspace=None, stream=None):
+    """Attention of one new token per sequence over a 4-bit paged cache: ``out[b, h] =
+    softmax_t(scale * q[b, h] . k[b, t]) v[b, t]`` over the first ``lengths[b]`` positions, which lie in
+    the pages ``page_table[b]``; see ``trinity_sm100_kv4_decode``.
+
+    ``q`` is BF16 [batch, heads, head_dim] (views allowed), ``page_table`` int32 [batch, max_pages],
+    ``lengths`` int32 [batch] on the device.  ``lse`` (FP32 [batch, heads]) receives the logarithm of
+    the sum of exponentials.  ``workspace`` (uint8, ``kv4_decode_workspace_bytes``) is allocated per
+    call unless given; calls that may overlap need one each."""
+    _require(q, torch.bfloat16, "q")
+    _require(page_table, torch.int32, "page_table")
+    _require(lengths, torch.int32, "lengths")
+    device = cache.device
+    if q.dim() != 3 or q.shape[2] != cache.head_dim or q.stride(2) != 1:
+        raise ValueError(f"kv4_decode: q must be [batch, heads, {cache.head_dim}] with a unit inner stride")
+    batch, heads, head_dim = q.shape
+    if (page_table.dim() != 2 or page_table.shape[0] != batch or page_table.stride(1) != 1 and page_table.shape[1] != 1
+            or tuple(lengths.shape) != (batch,) or not lengths.is_contiguous()):
+        raise ValueError("kv4_decode: page_table must be [batch, max_pages] and lengths [batch]")
+    if out is not None:
+        _require(out, torch.bfloat16, "out")
+        if out.shape != q.shape or not out.is_contiguous():
+            raise ValueError("kv4_decode: out must be a contiguous [batch, heads, head_dim] tensor")
+    if lse is not None:
+        _require(lse, torch.float32, "lse")
+        if tuple(lse.shape) != (batch, heads) or not lse.is_contiguous():
+            raise ValueError("kv4_decode: lse must be a contiguous [batch, heads] tensor")
+    _same_device(device, q=q, page_table=page_table, lengths=lengths, out=out, lse=lse, workspace=workspace)
+
+    def launch(handle):
+        o = torch.empty((batch, heads, head_dim), dtype=torch.bfloat16, device=device) if out is None else out
+        room = workspace
+        if room is None:
+            room = torch.empty(kv4_decode_workspace_bytes(heads, cache.kv_heads, head_dim), dtype=torch.uint8,
+                               device=device)
+        args = Kv4DecodeArgs(q.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), o.data_ptr(),
+                             lse.data_ptr() if lse is not None else None, room.data_ptr(),
+                             room.numel() * room.element_size(), q.stride(0), q.stride(1),
+                             _pitch(page_table), batch, heads, page_table.shape[1], scale)
+        _check(library().trinity_sm100_kv4_decode(ctypes.byref(cache.args), ctypes.byref(args), handle))
+        return o
+
+    return _submit(device, stream, (q, page_table, lengths, out, lse, workspace, *cache.tensors), launch)
 
 
 def allreduce_flag_words():
