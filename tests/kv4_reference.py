@@ -38,11 +38,14 @@ def filled_cache(kernels, pages, kv_heads, page, head_dim, group, seed, device="
 def attend(q, cache, table, lengths, scale):
     """out, lse and the bound of the error of out, in 64 bits.
 
-    The exponentials are rounded to BF16 (2^-8 each) but summed unrounded, the decoded values are
-    rounded to BF16 (2^-8): 2^-7 of sum w |v|.  A score is a sum of at most 128 products of
-    exact FP16 numbers and of the zero's part, in FP32: each of at most 128 + 8 additions rounds by
-    2^-24 of at most the sum of magnitudes, which moves a weight by as much (times two: numerator
-    and denominator).  Exponentials, rescalings and joins add a few 2^-22 more: 2^-18 covers them.
+    A value is zero + scale * code; a weight times its scale is rounded to FP16 (2^-11), of at most
+    15 of which each code takes, everything else is FP32.  A score is a sum of at most 128 products of
+    exact FP16 numbers and of the zero's part: each of at most 128 + 8 additions rounds by 2^-24 of
+    at most the sum of magnitudes, which moves a weight by as much (times two: numerator and
+    denominator).  Exponentials, sums over the positions, rescalings and joins add a few 2^-22 more:
+    2^-18 covers them.  All of that is relative to sum w (15 scale + |zero|).
+    A weight times scale smaller than FP16's normal numbers is off by 2^-25 where the largest scale is
+    more than 1/2 and the largest weight at least 2^7: less than length * 2^-27 of the largest scale.
     An exponential below FP32's smallest normal number, 2^-126 of one at the row's maximum, may come
     out as zero (so that a row whose heaviest value is exactly 0 has no smaller relative error):
     length * 2^-126 of the largest value, absolutely.
@@ -66,7 +69,10 @@ def attend(q, cache, table, lengths, scale):
             moved = 2 * 136 * 2.0 ** -24 * abs(scale) * qh.abs().sum(1, keepdim=True) * size + 2.0 ** -18
             w = torch.softmax(scores, -1)
             out[b, heads] = w @ v
-            bound[b, heads] = (2.0 ** -7 + moved) * (w @ v.abs()) + length * 2.0 ** -126 * v.abs().amax()
+            pairs = cache.v_scales[pages, h].flatten(0, 1)[:length].double()
+            reach = (15 * pairs[..., 0].abs() + pairs[..., 1].abs()).repeat_interleave(cache.group, 1)
+            bound[b, heads] = ((2.0 ** -11 + moved) * (w @ reach) + length * 2.0 ** -27 * pairs[..., 0].abs().amax()
+                               + length * 2.0 ** -126 * v.abs().amax())
             lse[b, heads] = torch.logsumexp(scores, -1)
     return out, lse, bound + 2.0 ** -8 * (out.abs() + bound)
 

@@ -165,26 +165,34 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Rows p) {
 //   lengths are (they are read on the device), every SM streams the same share.  A row that one
 //   block holds whole is written at once; the parts of a row that is cut go to the workspace and a
 //   second kernel joins them in block order, so results do not depend on timing.
-// * A producer warp fetches tiles into a ring of stages: codes by tiled TMA with the 32- or 64-byte
-//   swizzle (then the code words that a warp reads lie in distinct banks), scales by bulk copies.
+// * Tiles are fetched into a ring of stages: codes by tiled TMA as rows of 128 bytes (two or four
+//   positions) with the 128-byte swizzle, so that the code rows that ldmatrix reads lie in distinct
+//   banks; scales by bulk copies.
 // * Eight warps take 16 positions of a tile each, with their own running maximum, sum and
-//   accumulator; they meet only at the end of a run's row.
+//   accumulator; they meet only at the end of a run's row.  The warps refill the ring in turn (a
+//   warp of its own for that would cost a quarter of the registers: an SM's four schedulers
+//   would hold five warps of two blocks instead of four).
 // * Scores are computed transposed, S^T[16 positions x 8 heads] = K Q^T with mma.sync (m16n8k16):
 //   decoded codes are the A operand straight from registers (tcgen05 would want them written to
 //   shared or tensor memory first, four times the cache bytes), and eight query heads fill a
 //   tile's columns.  The exponentials, transposed in registers, are the B operand of
-//   O^T[channels x 8 heads] += V^T P^T.
+//   O^T[channels x 8 heads] += V^T P^T, whose A operand ldmatrix.trans delivers as pairs of
+//   positions with four channels each.
 //
-// Key codes enter as FP16: `word & 0x000f000f` read as two FP16 numbers is code * 2^-24 exactly
-// (subnormal; the tensor cores take those at full rate), `& 0x00f000f0` is 16 times that, which the
-// query side takes back.  The query is brought to FP16 with a power of two per head, exactly down
-// to 2^-22 of its largest element.  Scale and zero are applied to the FP32 score.
-// Value codes are decoded to BF16 (128 + code, minus 128, times scale plus zero: one rounding, the
-// rounding that a BF16 cache would have) and the exponentials are rounded to BF16 as the right
-// operand, as in the other attention kernel of this library; both are averaged over positions.
+// Codes are never converted: `word & 0x000f000f` read as two FP16 numbers is code * 2^-24 exactly
+// (subnormal; the tensor cores take those at full rate), `& 0x00f000f0` is 16 times that, and a
+// shift by 8 gives the other two pairs: five integer instructions for eight codes.  Scales and
+// zeros are applied outside the products:
+// * keys: s = scale_k * (q . codes) + zero_k * (sum of q), per group, in FP32.  The query enters as
+//   FP16 times a power of two per head, exactly down to 2^-22 of its largest element.
+// * values: out = sum_t (p_t scale_v[t]) codes[t] + sum_t p_t zero_v[t], per group; the second sum is
+//   FP32.  p_t scale_v[t] enters as FP16 (2^-12, far below the output's rounding): p_t is at most 2^15
+//   (see the maximum below) and scale_v is divided by a power of two, a running bound of the
+//   scales seen, which the accumulators follow like they follow the maximum.
 constexpr int kKv4Tile = 128;          // positions in a stage
 constexpr int kKv4Warps = 8;
-constexpr int kKv4Threads = (kKv4Warps + 1) * 32;
+constexpr uint32_t kKv4Lag = 2;
+constexpr int kKv4Threads = kKv4Warps * 32;
 
 struct Kv4Attend {
   const __nv_bfloat16* q;
@@ -268,7 +276,9 @@ struct Kv4Walk {
   long long base;            // first tile of sequence b
   int b, length, tiles;
   // the current piece
-  int row, first, count;     // row within the sequence, first tile of the piece, its tiles
+  int row, first, count;     // row within the sequence, first tile of the piece, its tiles (0: the run is over)
+  int tile;                  // for next_tile
+  Kv4Walk() = default;
   __device__ __forceinline__ Kv4Walk(const Kv4Attend& p, const Kv4Start& s, int blocks, int block) {
     next = kv4_first_tile(s.total, blocks, block);
     end = kv4_first_tile(s.total, blocks, block + 1);
@@ -278,7 +288,10 @@ struct Kv4Walk {
     tiles = kv4_tiles(length);
   }
   __device__ __forceinline__ bool step(const Kv4Attend& p) {
-    if (next >= end) return false;
+    if (next >= end) {
+      count = 0;
+      return false;
+    }
     const int rows = p.kv_heads * p.head_blocks;
     while (next >= base + static_cast<long long>(tiles) * rows) {   // the run ends inside a sequence with tiles
       base += static_cast<long long>(tiles) * rows;
@@ -292,8 +305,10 @@ struct Kv4Walk {
     const long long left = end - next;
     count = int(left < tiles - first ? left : tiles - first);
     next += count;
+    tile = first;
     return true;
   }
+  __device__ __forceinline__ bool next_tile(const Kv4Attend& p) { return ++tile < first + count || step(p); }
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -302,33 +317,41 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-__device__ __forceinline__ uint32_t lds32(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
-  return v;
+__device__ __forceinline__ float exp2_approx(float x) {   // 2^-22 relative; results below 2^-126 are 0
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
-__device__ __forceinline__ void lds64(uint32_t a, uint32_t& x, uint32_t& y) {
-  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(x), "=r"(y) : "r"(a));
+template <bool kTrans>
+__device__ __forceinline__ void load_matrices(uint32_t a, uint32_t (&r)[4]) {
+  if (kTrans)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
+}
+// The (scale, zero) pairs of one position.
+template <int kNG>
+__device__ __forceinline__ void load_pairs(uint32_t a, uint32_t (&r)[kNG]) {
+  if (kNG == 1)
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r[0]) : "r"(a));
+  else if (kNG == 2)
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1 % kNG]) : "r"(a));
+  else
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1 % kNG]), "=r"(r[2 % kNG]), "=r"(r[3 % kNG]) : "r"(a));
 }
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
                "l"(src), "r"(bytes), "r"(bar)
                : "memory");
 }
-__device__ __forceinline__ __nv_bfloat162 as_bf162(uint32_t v) { return *reinterpret_cast<__nv_bfloat162*>(&v); }
-__device__ __forceinline__ uint32_t as_u32(__nv_bfloat162 v) { return *reinterpret_cast<uint32_t*>(&v); }
-
 template <int kD, int kNG>
 __host__ __device__ constexpr int kv4_stage_bytes() {
   return 2 * kKv4Tile * (kD / 2) + 2 * kKv4Tile * kNG * 4;
@@ -370,12 +393,17 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   auto full = [&](int s) { return bars + 8u * s; };
   auto empty = [&](int s) { return bars + 8u * (kStages + s); };
   __shared__ long long locate_scratch[kKv4Threads / 32 + 2];
+  __shared__ Kv4Walk ahead_state[kKv4Lag];
+  __shared__ int ahead_pages[kKv4Lag][kKv4Tile / 16];
+  __shared__ uint32_t fetched[kStages];                    // tiles fetched into a stage so far
+  static_assert(kStages > int(kKv4Lag), "a tile must be on its way before it is waited for");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(full(s), 1);
       mbar_init(empty(s), kKv4Warps);
+      fetched[s] = 0;
     }
     mbar_fence_init();
     tma_prefetch_desc(&map_k);
@@ -387,44 +415,67 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   const Kv4Start start = kv4_locate<kKv4Threads>(p, blocks, block, locate_scratch);   // also orders the barriers
   Kv4Walk walk(p, start, blocks, block);
 
-  if (warp == kKv4Warps) {
-    // ---------------------------------------------------------- producer
-    uint32_t it = 0;
-    bool ok = true;
-    const int pieces = kKv4Tile / p.box;
-    while (ok && walk.step(p)) {
-      const int kv = walk.row / p.head_blocks;
-      const int* table = p.table + walk.b * p.table_stride;
-      for (int tile = walk.first; tile < walk.first + walk.count; ++tile, ++it) {
-        const int s = it % kStages;
-        ok = __all_sync(0xffffffffu, mbar_wait(empty(s), ((it / kStages) & 1u) ^ 1u, 0x911));
-        if (!ok) break;
-        const int live = min(pieces, (walk.length - tile * kKv4Tile + p.box - 1) / p.box);
-        if (lane == 0) mbar_arrive_expect_tx(full(s), uint32_t(live * p.box) * (2 * kRow + 8 * kNG));
-        __syncwarp();
-        const uint32_t stage = base + s * kStage;
-        for (int c = lane; c < live * 4; c += 32) {
-          const int piece = c >> 2, kind = c & 3;
-          const int position = tile * kKv4Tile + piece * p.box;
-          const int entry = position / p.page;
-          int page = table[entry];
-          if (page < 0 || page >= p.pages) {   // nothing outside the cache is read
-            report_timeout(kSiteKv4Page);
-            page = 0;
-          }
-          const long long row = (static_cast<long long>(page) * p.kv_heads + kv) * p.page + (position - entry * p.page);
-          if (kind < 2)
-            tma_load_3d(stage + kind * kCodes + piece * p.box * kRow, kind ? &map_v : &map_k, full(s), 0, int(row), 0);
-          else
-            bulk_load(stage + 2 * kCodes + (kind - 2) * kScales + piece * p.box * kNG * 4,
-                      (kind == 2 ? p.k_scales : p.v_scales) + row * kNG, uint32_t(p.box) * kNG * 4, full(s));
-        }
+  // ---------------------------------------------------------- refilling the ring
+  // At tile i one warp, number i modulo the warps, fetches tile i - kKv4Lag + kStages once all warps are
+  // through with tile i - kKv4Lag.  What it needs for that (where the tile lies, its page numbers) lies in
+  // slot i modulo kKv4Lag of shared memory, written by the warp that fetched at tile i - kKv4Lag before
+  // it said that it was through with that tile: the wait that frees the stage also orders the slot.
+  // It then leaves in the slot the tile kKv4Lag further on and starts the copy of its page numbers,
+  // which has landed before it says that it is through with tile i.
+  auto issue = [&](const Kv4Walk& at, int s, const int* pages) {     // one warp: a tile's copies into stage s
+    const int kv = at.row / p.head_blocks;
+    const int live = min(kKv4Tile / p.box, (at.length - at.tile * kKv4Tile + p.box - 1) / p.box);
+    if (lane == 0) {
+      mbar_arrive_expect_tx(full(s), uint32_t(live * p.box) * (2 * kRow + 8 * kNG));
+      ++fetched[s];
+    }
+    __syncwarp();
+    const uint32_t stage = base + s * kStage;
+    if (lane < live * 4) {
+      const int piece = lane >> 2, kind = lane & 3;
+      const int position = at.tile * kKv4Tile + piece * p.box, entry = position / p.page;
+      int page = pages ? pages[piece] : p.table[at.b * p.table_stride + entry];
+      if (page < 0 || page >= p.pages) {   // nothing outside the cache is read
+        report_timeout(kSiteKv4Page);
+        page = 0;
+      }
+      const long long row = (static_cast<long long>(page) * p.kv_heads + kv) * p.page + (position - entry * p.page);
+      if (kind < 2)
+        tma_load_3d(stage + kind * kCodes + piece * p.box * kRow, kind ? &map_v : &map_k, full(s), 0, int(row * kRow / 128), 0);
+      else
+        bulk_load(stage + 2 * kCodes + (kind - 2) * kScales + piece * p.box * kNG * 4,
+                  (kind == 2 ? p.k_scales : p.v_scales) + row * kNG, uint32_t(p.box) * kNG * 4, full(s));
+    }
+  };
+  auto look_ahead = [&](const Kv4Walk& at, int slot) {     // one warp: leaves `at` in the slot as the tile to fetch next
+    __syncwarp();
+    if (lane == 0) ahead_state[slot] = at;
+    if (at.count > 0) {
+      const int live = min(kKv4Tile / p.box, (at.length - at.tile * kKv4Tile + p.box - 1) / p.box);
+      if (lane < live)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(&ahead_pages[slot][lane])),
+                     "l"(p.table + at.b * p.table_stride + (at.tile * kKv4Tile + lane * p.box) / p.page)
+                     : "memory");
+    }
+  };
+  {
+    // the first tiles: every warp finds and fetches its own
+    Kv4Walk at = walk;
+    int behind = 0;
+    bool some = at.step(p);
+    for (int s = warp; s < kStages && some; s += kKv4Warps) {
+      for (; behind < s && some; ++behind) some = at.next_tile(p);
+      if (some) issue(at, s, nullptr);
+    }
+    if (warp == 0) {
+      for (; behind < kStages && some; ++behind) some = at.next_tile(p);
+      for (int slot = 0; slot < int(kKv4Lag); ++slot) {
+        look_ahead(at, slot);
+        if (some) some = at.next_tile(p);
       }
     }
-    // nothing may still be in flight into this block's shared memory when it ends
-    for (uint32_t back = min(it, uint32_t(kStages)); back > 0; --back)
-      mbar_wait(full((it - back) % kStages), ((it - back) / kStages) & 1u, 0x913);
-  } else {
+  }
+  {
     // ---------------------------------------------------------- attention
     // sequences without a position: nothing to attend to, the output row is zero
     for (int b = block; b < p.batch; b += blocks) {
@@ -436,15 +487,11 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           p.lse[static_cast<long long>(b) * p.heads + i] = -INFINITY;
     }
     const int g = lane >> 2, t = lane & 3;
-    // Position within the warp's 16 of row r of a score tile: a permutation of the low three bits, so
-    // that the four positions whose values one load fetches lie in distinct banks.
-    auto position_of = [](int r) {
-      return kD == 128 ? (r & 12) | ((r & 1) << 1) | ((r >> 1) & 1) : (r & 8) | ((r & 1) << 2) | ((r >> 1) & 3);
-    };
-    const int key_row[2] = {warp * 16 + position_of(g), warp * 16 + position_of(g + 8)};
-    const int value_row[4] = {warp * 16 + position_of(2 * t), warp * 16 + position_of(2 * t + 1),
-                              warp * 16 + position_of(2 * t + 8), warp * 16 + position_of(2 * t + 9)};
-    const int value_group = g * (kD / 8) * kNG / kD;
+    // ldmatrix: lane l gives the address of row l & 7 of matrix l >> 3, which are (positions 0-7, 8-15) x
+    // (an even, the next odd 16-byte chunk); chunks are swizzled, chunk ^ bits 7-9 of the offset.
+    const uint32_t matrix_row = (warp * 16 + ((lane >> 3) & 1) * 8 + (lane & 7)) * kRow + (lane >> 4) * 16;
+    const uint32_t matrix_offset = matrix_row ^ (((matrix_row >> 7) & 7) << 4);
+    const int position[2] = {warp * 16 + g, warp * 16 + g + 8};     // rows of the lane's scores
     uint32_t it = 0;
     bool ok = true;
     while (walk.step(p)) {
@@ -504,91 +551,143 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
             zero_factor[n][c][i] = __shfl_sync(0xffffffffu, sums[i], 4 * (2 * t + c)) * p.scale_log2;
         }
       }
-      float acc[kNT][kMT][4], top[kNT][2], sum[kNT][2];
+      float acc[kNT][kMT][4], zeros[kNT][2][kNG], ref[kNT][2], sum[kNT][2];
+      float limit = 0.0f, inverse_limit = 0.0f;        // power of two above every value scale so far
 #pragma unroll
       for (int n = 0; n < kNT; ++n) {
 #pragma unroll
         for (int i = 0; i < kMT; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[n][i][e] = 0.0f;
-        top[n][0] = top[n][1] = -INFINITY;
-        sum[n][0] = sum[n][1] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          ref[n][c] = -INFINITY;
+          sum[n][c] = 0.0f;
+#pragma unroll
+          for (int i = 0; i < kNG; ++i) zeros[n][c][i] = 0.0f;
+        }
       }
       for (int tile = walk.first; tile < walk.first + walk.count; ++tile, ++it) {
         const int s = it % kStages;
+        if (ok && it >= kKv4Lag && warp == int(it % kKv4Warps)) {
+          const uint32_t old = it - kKv4Lag;
+          ok = __all_sync(0xffffffffu, mbar_wait(empty(old % kStages), (old / kStages) & 1u, 0x911));
+          if (ok) {
+            Kv4Walk at = ahead_state[it % kKv4Lag];
+            if (at.count > 0) {
+              issue(at, old % kStages, ahead_pages[it % kKv4Lag]);
+              bool some = true;
+              for (uint32_t i = 0; i < kKv4Lag && some; ++i) some = at.next_tile(p);
+              look_ahead(at, it % kKv4Lag);
+            }
+          }
+        }
         if (ok) ok = __all_sync(0xffffffffu, mbar_wait(full(s), (it / kStages) & 1u, 0x912));
         const int live = walk.length - tile * kKv4Tile;     // positions of the tile that exist
         if (ok && warp * 16 < live) {
           const uint32_t keys = base + s * kStage, values = keys + kCodes;
           const uint32_t key_scales = values + kCodes, value_scales = key_scales + kScales;
           float score[kNT][4];
-#pragma unroll
-          for (int n = 0; n < kNT; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) score[n][e] = 0.0f;
-#pragma unroll
-          for (int i = 0; i < kNG; ++i) {
-            float dot[kNT][4];
+          {
+            float dot[kNT][kNG][4];
 #pragma unroll
             for (int n = 0; n < kNT; ++n)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) dot[n][e] = 0.0f;
+              for (int i = 0; i < kNG; ++i)
 #pragma unroll
-            for (int jj = 0; jj < kChunks / kNG; ++jj) {
-              const int j = i * (kChunks / kNG) + jj;
-              uint32_t w[2];
+                for (int e = 0; e < 4; ++e) dot[n][i][e] = 0.0f;
 #pragma unroll
-              for (int r = 0; r < 2; ++r) {
-                const int row = key_row[r];
-                const int swizzle = kD == 128 ? (row >> 1) & 3 : (row >> 2) & 1;
-                w[r] = lds32(keys + row * kRow + ((j ^ swizzle) << 4) + t * 4);
-              }
+            for (int jj = 0; jj < kChunks / 2; ++jj) {
+              uint32_t w[4];
+              load_matrices<false>((keys + matrix_offset) ^ (jj << 5), w);
 #pragma unroll
-              for (int half = 0; half < 2; ++half) {
-                const uint32_t a[4] = {w[0] & 0x000f000fu, w[1] & 0x000f000fu, w[0] & 0x00f000f0u, w[1] & 0x00f000f0u};
+              for (int q = 0; q < 2; ++q) {
+                const int j = 2 * jj + q, i = j * kNG / kChunks;
 #pragma unroll
-                for (int n = 0; n < kNT; ++n) mma_f16(dot[n], a, qf[n][j][2 * half], qf[n][j][2 * half + 1]);
-                w[0] >>= 8;
-                w[1] >>= 8;
+                for (int half = 0; half < 2; ++half) {
+                  const uint32_t lo = half ? w[2 * q] >> 8 : w[2 * q], hi = half ? w[2 * q + 1] >> 8 : w[2 * q + 1];
+                  const uint32_t a[4] = {lo & 0x000f000fu, hi & 0x000f000fu, lo & 0x00f000f0u, hi & 0x00f000f0u};
+#pragma unroll
+                  for (int n = 0; n < kNT; ++n) mma_f16(dot[n][i], a, qf[n][j][2 * half], qf[n][j][2 * half + 1]);
+                }
               }
             }
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-              const uint32_t pair = lds32(key_scales + (key_row[r] * kNG + i) * 4);
-              const float scale = bf16_lo(pair), zero = bf16_hi(pair);
+              uint32_t pair[kNG];
+              load_pairs<kNG>(key_scales + position[r] * (kNG * 4), pair);
 #pragma unroll
               for (int n = 0; n < kNT; ++n)
 #pragma unroll
-                for (int c = 0; c < 2; ++c)
-                  score[n][2 * r + c] = fmaf(dot[n][2 * r + c] * 0x1p24f * score_factor[n][c], scale,
-                                             fmaf(zero, zero_factor[n][c][i], score[n][2 * r + c]));
+                for (int c = 0; c < 2; ++c) {
+                  float x = dot[n][0][2 * r + c] * bf16_lo(pair[0]), z = bf16_hi(pair[0]) * zero_factor[n][c][0];
+#pragma unroll
+                  for (int i = 1; i < kNG; ++i) {
+                    x = fmaf(dot[n][i][2 * r + c], bf16_lo(pair[i]), x);
+                    z = fmaf(bf16_hi(pair[i]), zero_factor[n][c][i], z);
+                  }
+                  score[n][2 * r + c] = fmaf(x * 0x1p24f, score_factor[n][c], z);
+                }
             }
           }
+          uint32_t value_pair[2][kNG];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) load_pairs<kNG>(value_scales + position[r] * (kNG * 4), value_pair[r]);
           if (warp * 16 + 16 > live) {
+            // what lies behind the sequence, NaN included, weighs nothing
 #pragma unroll
             for (int r = 0; r < 2; ++r)
-              if (key_row[r] >= live)
+              if (position[r] >= live) {
 #pragma unroll
                 for (int n = 0; n < kNT; ++n) score[n][2 * r] = score[n][2 * r + 1] = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < kNG; ++i) value_pair[r][i] = 0;
+              }
           }
-          // The maximum is raised only when a score exceeds it by more than 2^8: exponentials stay
-          // below 2^8, and most tiles need neither the shuffles nor the rescaling.
+          // The reference point of a head's exponentials is 2^7 below the largest score when it was last
+          // set, and is set again only when a score exceeds that one by 2^8 or more (most tiles need
+          // neither the shuffles nor the rescaling): exponentials stay below 2^15, and FP16 keeps
+          // those down to 2^-31 of the largest.
           bool raise = false;
 #pragma unroll
           for (int n = 0; n < kNT; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) raise |= score[n][e] > top[n][e & 1] + 8.0f;
+            for (int e = 0; e < 4; ++e) raise |= score[n][e] > ref[n][e & 1] + 15.0f;
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int i = 0; i < kNG; ++i) raise |= bf16_lo(value_pair[r][i]) > limit;
           if (__any_sync(0xffffffffu, raise)) {
+            float most = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+              for (int i = 0; i < kNG; ++i) most = fmaxf(most, bf16_lo(value_pair[r][i]));
+#pragma unroll
+            for (int o = 4; o < 32; o *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+            float rescale = 1.0f;
+            if (most > limit) {
+              const uint32_t power = min((__float_as_uint(most) & 0x7f800000u) + 0x00800000u, 0x7e800000u);
+              inverse_limit = __uint_as_float(0x7f000000u - power);      // 2^-k for limit 2^k
+              rescale = limit * inverse_limit;
+              limit = __uint_as_float(power);
+            }
 #pragma unroll
             for (int n = 0; n < kNT; ++n)
 #pragma unroll
               for (int c = 0; c < 2; ++c) {
-                float m = fmaxf(top[n][c], fmaxf(score[n][c], score[n][2 + c]));
+                float m = fmaxf(score[n][c], score[n][2 + c]);
 #pragma unroll
                 for (int o = 4; o < 32; o *= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                const float f = m == -INFINITY ? 1.0f : exp2f(top[n][c] - m);
-                top[n][c] = m;
+                float f = 1.0f;
+                if (m - 7.0f > ref[n][c]) {
+                  f = exp2_approx(ref[n][c] - (m - 7.0f));
+                  ref[n][c] = m - 7.0f;
+                }
                 sum[n][c] *= f;
+#pragma unroll
+                for (int i = 0; i < kNG; ++i) zeros[n][c][i] *= f;
+                f *= rescale;
 #pragma unroll
                 for (int i = 0; i < kMT; ++i) {
                   acc[n][i][c] *= f;
@@ -596,63 +695,48 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
                 }
               }
           }
-          uint32_t pf[kNT][2];
+          float weight[kNT][4];
 #pragma unroll
-          for (int n = 0; n < kNT; ++n) {
-            float e[4];
+          for (int n = 0; n < kNT; ++n)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const float m = top[n][c & 1];
-              e[c] = exp2f(score[n][c] - (m == -INFINITY ? 0.0f : m));
-              sum[n][c & 1] += e[c];
+            for (int e = 0; e < 4; ++e) {
+              weight[n][e] = exp2_approx(score[n][e] - ref[n][e & 1]);
+              sum[n][e & 1] += weight[n][e];
             }
-            pf[n][0] = transpose_8x8(pack_bf16x2(e[0], e[1]));
-            pf[n][1] = transpose_8x8(pack_bf16x2(e[2], e[3]));
-          }
-          // values: lane (g, t) holds channels kD / 8 * g + (0 ..) of four positions
-          uint32_t pair[4], codes[4][2];
+          uint32_t pf[kNT][kNG][2];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int row = value_row[i];
-            pair[i] = lds32(value_scales + (row * kNG + value_group) * 4);
-            if (warp * 16 + 16 > live && row >= live) pair[i] = 0;     // what lies behind the sequence counts as zero
-            if (kD == 128) {
-              lds64(values + row * kRow + (((g >> 1) ^ ((row >> 1) & 3)) << 4) + (g & 1) * 8, codes[i][0], codes[i][1]);
-            } else {
-              const uint32_t w = lds32(values + row * kRow + (((g >> 2) ^ ((row >> 2) & 1)) << 4) + (g & 3) * 4);
-              codes[i][0] = w;
-              codes[i][1] = w >> 16;
-            }
-          }
-          const __nv_bfloat162 offset = __float2bfloat162_rn(128.0f);
-          __nv_bfloat162 scale2[2], zero2[2];
+          for (int i = 0; i < kNG; ++i)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            scale2[h] = as_bf162(__byte_perm(pair[2 * h], pair[2 * h + 1], 0x5410));
-            zero2[h] = as_bf162(__byte_perm(pair[2 * h], pair[2 * h + 1], 0x7632));
-          }
-          constexpr int kQuads = kD == 128 ? 2 : 1;          // 16-bit quads of codes in each half row
+            for (int r = 0; r < 2; ++r) {
+              const float scale = bf16_lo(value_pair[r][i]) * inverse_limit, zero = bf16_hi(value_pair[r][i]);
 #pragma unroll
-          for (int quad = 0; quad < kQuads; ++quad) {
-            uint32_t w[4];                                   // (row g, row g + 8) x (positions 2t.., 2t + 8..)
+              for (int n = 0; n < kNT; ++n) {
+                const __half2 h = __floats2half2_rn(weight[n][2 * r] * scale, weight[n][2 * r + 1] * scale);
+                pf[n][i][r] = transpose_8x8(*reinterpret_cast<const uint32_t*>(&h));
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-              for (int r = 0; r < 2; ++r)
-                w[2 * h + r] = __byte_perm(codes[2 * h][r], codes[2 * h + 1][r], quad ? 0x7632 : 0x5410);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint32_t a[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const uint32_t raw = ((w[e] >> (4 * i)) & 0x000f000fu) | 0x43004300u;   // 128 + code
-                a[e] = as_u32(__hfma2(__hsub2(as_bf162(raw), offset), scale2[e >> 1], zero2[e >> 1]));
+                for (int c = 0; c < 2; ++c) zeros[n][c][i] = fmaf(weight[n][2 * r + c], zero, zeros[n][c][i]);
               }
+            }
+          // A chunk of 32 channels: lane (g, t) holds channels 4 g .. 4 g + 3 of positions 2 t, 2 t + 1 (and + 8);
+          // two tiles of 16 channels, row g the even and row g + 8 the odd channel (16 times too large).
 #pragma unroll
-              for (int n = 0; n < kNT; ++n) mma_bf16(acc[n][quad * 4 + i], a, pf[n][0], pf[n][1]);
+          for (int jj = 0; jj < kChunks / 2; ++jj) {
+            uint32_t w[4];
+            load_matrices<true>((values + matrix_offset) ^ (jj << 5), w);
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              const int j = 2 * jj + q, i = j * kNG / kChunks;
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                const uint32_t lo = half ? w[2 * q] >> 8 : w[2 * q], hi = half ? w[2 * q + 1] >> 8 : w[2 * q + 1];
+                const uint32_t a[4] = {lo & 0x000f000fu, lo & 0x00f000f0u, hi & 0x000f000fu, hi & 0x00f000f0u};
+#pragma unroll
+                for (int n = 0; n < kNT; ++n) mma_f16(acc[n][2 * j + half], a, pf[n][i][0], pf[n][i][1]);
+              }
             }
           }
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");    // page numbers, if this warp asked for any
         __syncwarp();
         if (lane == 0) mbar_arrive(empty(s));
       }
@@ -663,19 +747,25 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         for (int c = 0; c < 2; ++c) {
 #pragma unroll
           for (int o = 4; o < 32; o *= 2) sum[n][c] += __shfl_xor_sync(0xffffffffu, sum[n][c], o);
-          float* mine = join + (warp * kHeads + n * 8 + 2 * t + c) * kPitch + g * (kD / 8);
-          // channel g * kD / 8 + i of the lower half row, + kD / 16 + i of the upper one
 #pragma unroll
-          for (int i = 0; i < kMT; ++i) {
-            mine[i] = acc[n][i][c];
-            mine[kMT + i] = acc[n][i][2 + c];
+          for (int i = 0; i < kNG; ++i)
+#pragma unroll
+            for (int o = 4; o < 32; o *= 2) zeros[n][c][i] += __shfl_xor_sync(0xffffffffu, zeros[n][c][i], o);
+          float* mine = join + (warp * kHeads + n * 8 + 2 * t + c) * kPitch + g * 4;
+          const float even = limit * 0x1p24f, odd = limit * 0x1p20f;
+#pragma unroll
+          for (int j = 0; j < kChunks; ++j) {
+            const float zero = zeros[n][c][j * kNG / kChunks];
+            *reinterpret_cast<float4*>(mine + 32 * j) =
+                make_float4(fmaf(acc[n][2 * j][c], even, zero), fmaf(acc[n][2 * j][2 + c], odd, zero),
+                            fmaf(acc[n][2 * j + 1][c], even, zero), fmaf(acc[n][2 * j + 1][2 + c], odd, zero));
           }
           if (g == 0) {
-            join_ml[(warp * kHeads + n * 8 + 2 * t + c) * 2] = top[n][c];
+            join_ml[(warp * kHeads + n * 8 + 2 * t + c) * 2] = ref[n][c];
             join_ml[(warp * kHeads + n * 8 + 2 * t + c) * 2 + 1] = sum[n][c];
           }
         }
-      asm volatile("bar.sync 1, %0;" ::"n"(kKv4Warps * 32) : "memory");
+      __syncthreads();
       const bool whole = walk.count == walk.tiles;
       const int slot = walk.first == 0 ? 1 : 0;   // part 0: the row began in an earlier block
       for (int i = threadIdx.x; i < heads_here * (kD / 4); i += kKv4Warps * 32) {
@@ -712,8 +802,12 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           }
         }
       }
-      asm volatile("bar.sync 1, %0;" ::"n"(kKv4Warps * 32) : "memory");   // the join area is free again
+      __syncthreads();   // the join area is free again
     }
+    // After a wait that gave up, nothing may still be in flight into this block's shared memory.
+    if (__syncthreads_or(!ok))
+      for (int s = 0; s < kStages; ++s)
+        if (fetched[s]) mbar_wait(full(s), (fetched[s] - 1) & 1u, 0x913);
   }
 }
 
@@ -938,12 +1032,10 @@ extern "C" int trinity_sm100_kv4_decode(const trinity_sm100_kv4_cache* cache, co
   while (c.page % p.box) p.box /= 2;
   p.scale_log2 = a.scale * 1.4426950408889634f;
   CUtensorMap map_k, map_v;
-  const uint64_t rows = static_cast<uint64_t>(c.pages) * c.kv_heads * c.page;
-  const int row_bytes = c.head_dim / 2;
-  if (int rc = make_tensor_map_3d(&map_k, c.k_codes, 2, row_bytes / 2, rows, 1, row_bytes, row_bytes * rows, row_bytes / 2, p.box, 1, row_bytes))
-    return rc;
-  if (int rc = make_tensor_map_3d(&map_v, c.v_codes, 2, row_bytes / 2, rows, 1, row_bytes, row_bytes * rows, row_bytes / 2, p.box, 1, row_bytes))
-    return rc;
+  const uint64_t lines = static_cast<uint64_t>(c.pages) * c.kv_heads * c.page * (c.head_dim / 2) / 128;
+  const uint32_t box_lines = p.box * (c.head_dim / 2) / 128;
+  if (int rc = make_tensor_map_3d(&map_k, c.k_codes, 2, 64, lines, 1, 128, 128 * lines, 64, box_lines, 1, 128)) return rc;
+  if (int rc = make_tensor_map_3d(&map_v, c.v_codes, 2, 64, lines, 1, 128, 128 * lines, 64, box_lines, 1, 128)) return rc;
   const int blocks = kv4_blocks(sm_count, p.group_heads);
   cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
   const int groups = c.head_dim / c.group;
