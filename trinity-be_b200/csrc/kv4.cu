@@ -168,10 +168,10 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Rows p) {
 // * Tiles are fetched into a ring of stages: codes by tiled TMA as rows of 128 bytes (two or four
 //   positions) with the 128-byte swizzle, so that the code rows that ldmatrix reads lie in distinct
 //   banks; scales by bulk copies.
-// * Eight warps take 16 positions of a tile each, with their own running maximum, sum and
-//   accumulator; they meet only at the end of a run's row.  The warps refill the ring in turn (a
-//   warp of its own for that would cost a quarter of the registers: an SM's four schedulers
-//   would hold five warps of two blocks instead of four).
+// * Four warps take twice 16 positions of a tile each (two independent chains of products), with
+//   their own running maximum, sum and accumulator; they meet only at the end of a run's row.  The
+//   warps refill the ring in turn: a warp of its own for that would cost registers that the others
+//   need.
 // * Scores are computed transposed, S^T[16 positions x 8 heads] = K Q^T with mma.sync (m16n8k16):
 //   decoded codes are the A operand straight from registers (tcgen05 would want them written to
 //   shared or tensor memory first, four times the cache bytes), and eight query heads fill a
@@ -190,7 +190,9 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Rows p) {
 //   (see the maximum below) and scale_v is divided by a power of two, a running bound of the
 //   scales seen, which the accumulators follow like they follow the maximum.
 constexpr int kKv4Tile = 128;          // positions in a stage
-constexpr int kKv4Warps = 8;
+constexpr int kKv4Warps = 4;
+constexpr int kKv4Sub = kKv4Tile / (16 * kKv4Warps);   // groups of 16 positions a warp takes of each tile
+constexpr int kKv4PerSm = 3;           // resident blocks: twelve warps of 168 registers
 constexpr uint32_t kKv4Lag = 2;
 constexpr int kKv4Threads = kKv4Warps * 32;
 
@@ -202,16 +204,18 @@ struct Kv4Attend {
   const int* lengths;
   __nv_bfloat16* out;
   float* lse;
-  float* parts;          // [blocks][2][8 kNT heads][D] and behind them [blocks][2][8 kNT heads][2]
+  // Workspace: of each block two parts (sums, then maximum and total), and the row it leaves unfinished.
+  float* parts;          // [blocks][2][8 kNT heads][D], behind them [blocks][2][8 kNT heads][2]
+  int4* cuts;            // [blocks] {sequence, row in it, last block that holds a part, 1} or {.., 0}
   long long q_batch, q_head, table_stride;
-  int batch, heads, kv_heads, group_heads, head_blocks, pages, page, max_pages, box;
+  int batch, heads, kv_heads, group_heads, head_blocks, pages, page, max_pages, box, box_shift, page_shift;
   float scale_log2;
 };
 
 // Where the run of one block starts, and the size of all.
 struct Kv4Start {
   long long total, tile_base;   // tiles of all rows; tiles before sequence `sequence`
-  int sequence;
+  int sequence, runs;           // runs: blocks that have one
 };
 
 __device__ __forceinline__ int kv4_length(const Kv4Attend& p, int b) {
@@ -219,16 +223,21 @@ __device__ __forceinline__ int kv4_length(const Kv4Attend& p, int b) {
   const int n = p.lengths[b];
   return n < 0 ? 0 : n > most ? int(most) : n;
 }
-__device__ __forceinline__ int kv4_tiles(int length) { return (length + kKv4Tile - 1) / kKv4Tile; }
-__host__ __device__ __forceinline__ long long kv4_first_tile(long long total, int blocks, int block) {
-  return total * block / blocks;
+__device__ __forceinline__ int kv4_page_of(const Kv4Attend& p, int position) {
+  return p.page_shift >= 0 ? position >> p.page_shift : position / p.page;
 }
-// Block whose run holds tile t: the largest i with total * i / blocks <= t.
-__host__ __device__ __forceinline__ int kv4_block_of(long long total, int blocks, long long t) {
-  return int(((t + 1) * blocks - 1) / total);
+__device__ __forceinline__ int kv4_tiles(int length) { return (length + kKv4Tile - 1) / kKv4Tile; }
+// First tile of a block's run; `runs` is at most the number of tiles, so that no run is empty.
+__device__ __forceinline__ long long kv4_first_tile(long long total, int runs, int block) {
+  if (total < (1 << 20)) return uint32_t(total) * uint32_t(block) / uint32_t(runs);   // (runs are below 2^11)
+  return total * block / runs;
+}
+// Block whose run holds tile t: the largest i with total * i / runs <= t.
+__device__ __forceinline__ int kv4_block_of(long long total, int runs, long long t) {
+  return int(((t + 1) * runs - 1) / total);
 }
 
-// All kThreads threads of the block; finds the sequence that holds tile total * block / blocks.
+// All threads of the block; finds the sequence in which its run begins.
 template <int kThreads>
 __device__ __forceinline__ Kv4Start kv4_locate(const Kv4Attend& p, int blocks, int block, long long* scratch) {
   constexpr int kWarps = kThreads / 32;
@@ -251,7 +260,8 @@ __device__ __forceinline__ Kv4Start kv4_locate(const Kv4Attend& p, int blocks, i
     if (w < warp) base += scratch[w];
     total += scratch[w];
   }
-  const long long first = kv4_first_tile(total, blocks, block);
+  const int runs = total < blocks ? int(total) : blocks;
+  const long long first = block < runs ? kv4_first_tile(total, runs, block) : -1;
   if (first >= base && first < base + sum) {   // exactly one thread, if there is any tile
     int b = begin;
     for (;; ++b) {
@@ -267,6 +277,7 @@ __device__ __forceinline__ Kv4Start kv4_locate(const Kv4Attend& p, int blocks, i
   s.total = total;
   s.tile_base = scratch[kWarps];
   s.sequence = int(scratch[kWarps + 1]);
+  s.runs = runs;
   return s;
 }
 
@@ -277,11 +288,15 @@ struct Kv4Walk {
   int b, length, tiles;
   // the current piece
   int row, first, count;     // row within the sequence, first tile of the piece, its tiles (0: the run is over)
+  int kv, hb;                // cached head and head block of the row
   int tile;                  // for next_tile
   Kv4Walk() = default;
-  __device__ __forceinline__ Kv4Walk(const Kv4Attend& p, const Kv4Start& s, int blocks, int block) {
-    next = kv4_first_tile(s.total, blocks, block);
-    end = kv4_first_tile(s.total, blocks, block + 1);
+  __device__ __forceinline__ Kv4Walk(const Kv4Attend& p, const Kv4Start& s, int block) {
+    next = end = 0;
+    if (block < s.runs) {
+      next = kv4_first_tile(s.total, s.runs, block);
+      end = kv4_first_tile(s.total, s.runs, block + 1);
+    }
     base = s.tile_base;
     b = s.sequence;
     length = next < end ? kv4_length(p, b) : 0;
@@ -306,6 +321,8 @@ struct Kv4Walk {
     count = int(left < tiles - first ? left : tiles - first);
     next += count;
     tile = first;
+    kv = p.head_blocks == 1 ? row : row / p.head_blocks;
+    hb = row - kv * p.head_blocks;
     return true;
   }
   __device__ __forceinline__ bool next_tile(const Kv4Attend& p) { return ++tile < first + count || step(p); }
@@ -356,22 +373,27 @@ template <int kD, int kNG>
 __host__ __device__ constexpr int kv4_stage_bytes() {
   return 2 * kKv4Tile * (kD / 2) + 2 * kKv4Tile * kNG * 4;
 }
+template <int kD>
+__host__ __device__ constexpr int kv4_join_bytes() {   // four heads' accumulators per warp, rows padded by four floats, and (maximum, sum)
+  return kKv4Warps * 4 * ((kD + 4) * 4 + 8);
+}
 template <int kD, int kNT>
-__host__ __device__ constexpr int kv4_join_bytes() {   // one accumulator per warp, rows padded by four floats, and (maximum, sum)
-  return kKv4Warps * 8 * kNT * ((kD + 4) * 4 + 8);
+__host__ __device__ constexpr int kv4_query_bytes() {
+  return kNT * (kD / 32) * 32 * 16;
 }
 template <int kD, int kNG, int kNT>
 __host__ __device__ constexpr int kv4_stages() {
-  // two blocks an SM with eight query heads a block, one with sixteen
-  return ((kNT == 1 ? 113 : 226) * 1024 - 2048 - kv4_join_bytes<kD, kNT>()) / kv4_stage_bytes<kD, kNG>();
+  // what a third of an SM's 228 KB leaves beside the system's 1 KB a block, static variables and alignment
+  return (228 * 1024 / kKv4PerSm - 3072 - kv4_join_bytes<kD>() - kv4_query_bytes<kD, kNT>()) / kv4_stage_bytes<kD, kNG>();
 }
 template <int kD, int kNG, int kNT>
 __host__ __device__ constexpr int kv4_smem_bytes() {
-  return 1024 + kv4_stages<kD, kNG, kNT>() * kv4_stage_bytes<kD, kNG>() + kv4_join_bytes<kD, kNT>() + 512;
+  return 1024 + kv4_stages<kD, kNG, kNT>() * kv4_stage_bytes<kD, kNG>() + kv4_query_bytes<kD, kNT>() +
+         kv4_join_bytes<kD>() + 256;
 }
 
 template <int kD, int kNG, int kNT>
-__global__ void __launch_bounds__(kKv4Threads, kNT == 1 ? 2 : 1)
+__global__ void __launch_bounds__(kKv4Threads, kKv4PerSm)
 kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                   const Kv4Attend p) {
   constexpr int kRow = kD / 2;                         // bytes of codes a position
@@ -387,9 +409,11 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
-  float* join = reinterpret_cast<float*>(smem + kStages * kStage);            // [warp][head][kPitch]
-  float* join_ml = join + kKv4Warps * kHeads * kPitch;                        // [warp][head][2]
-  const uint32_t bars = base + kStages * kStage + kv4_join_bytes<kD, kNT>();
+  uint4 (*query)[kChunks][32] = reinterpret_cast<uint4 (*)[kChunks][32]>(smem + kStages * kStage);   // [tile of heads][chunk][lane]
+  float* join = reinterpret_cast<float*>(smem + kStages * kStage + kv4_query_bytes<kD, kNT>());       // [warp][head][kPitch]
+  float* join_ml = join + kKv4Warps * 4 * kPitch;                                                     // [warp][head][2]
+  const uint32_t bars = base + kStages * kStage + kv4_query_bytes<kD, kNT>() + kv4_join_bytes<kD>();
+  __shared__ float factors[kHeads][1 + kNG];     // of a head's scores: scale, and zero per group
   auto full = [&](int s) { return bars + 8u * s; };
   auto empty = [&](int s) { return bars + 8u * (kStages + s); };
   __shared__ long long locate_scratch[kKv4Threads / 32 + 2];
@@ -410,10 +434,10 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     tma_prefetch_desc(&map_v);
   }
   grid_dependency_wait();
-  grid_dependents_may_launch();   // after the wait: the joining kernel may then read the lengths at once
+  grid_dependents_may_launch();
   const int blocks = gridDim.x, block = blockIdx.x;
   const Kv4Start start = kv4_locate<kKv4Threads>(p, blocks, block, locate_scratch);   // also orders the barriers
-  Kv4Walk walk(p, start, blocks, block);
+  Kv4Walk walk(p, start, block);
 
   // ---------------------------------------------------------- refilling the ring
   // At tile i one warp, number i modulo the warps, fetches tile i - kKv4Lag + kStages once all warps are
@@ -423,23 +447,22 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   // It then leaves in the slot the tile kKv4Lag further on and starts the copy of its page numbers,
   // which has landed before it says that it is through with tile i.
   auto issue = [&](const Kv4Walk& at, int s, const int* pages) {     // one warp: a tile's copies into stage s
-    const int kv = at.row / p.head_blocks;
-    const int live = min(kKv4Tile / p.box, (at.length - at.tile * kKv4Tile + p.box - 1) / p.box);
+    const int live = (min(kKv4Tile, at.length - at.tile * kKv4Tile) + p.box - 1) >> p.box_shift;
     if (lane == 0) {
-      mbar_arrive_expect_tx(full(s), uint32_t(live * p.box) * (2 * kRow + 8 * kNG));
+      mbar_arrive_expect_tx(full(s), uint32_t(live << p.box_shift) * (2 * kRow + 8 * kNG));
       ++fetched[s];
     }
     __syncwarp();
     const uint32_t stage = base + s * kStage;
     if (lane < live * 4) {
       const int piece = lane >> 2, kind = lane & 3;
-      const int position = at.tile * kKv4Tile + piece * p.box, entry = position / p.page;
+      const int position = at.tile * kKv4Tile + (piece << p.box_shift), entry = kv4_page_of(p, position);
       int page = pages ? pages[piece] : p.table[at.b * p.table_stride + entry];
       if (page < 0 || page >= p.pages) {   // nothing outside the cache is read
         report_timeout(kSiteKv4Page);
         page = 0;
       }
-      const long long row = (static_cast<long long>(page) * p.kv_heads + kv) * p.page + (position - entry * p.page);
+      const long long row = (static_cast<long long>(page) * p.kv_heads + at.kv) * p.page + (position - entry * p.page);
       if (kind < 2)
         tma_load_3d(stage + kind * kCodes + piece * p.box * kRow, kind ? &map_v : &map_k, full(s), 0, int(row * kRow / 128), 0);
       else
@@ -451,10 +474,10 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     __syncwarp();
     if (lane == 0) ahead_state[slot] = at;
     if (at.count > 0) {
-      const int live = min(kKv4Tile / p.box, (at.length - at.tile * kKv4Tile + p.box - 1) / p.box);
+      const int live = (min(kKv4Tile, at.length - at.tile * kKv4Tile) + p.box - 1) >> p.box_shift;
       if (lane < live)
         asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(&ahead_pages[slot][lane])),
-                     "l"(p.table + at.b * p.table_stride + (at.tile * kKv4Tile + lane * p.box) / p.page)
+                     "l"(p.table + at.b * p.table_stride + kv4_page_of(p, at.tile * kKv4Tile + (lane << p.box_shift)))
                      : "memory");
     }
   };
@@ -480,38 +503,38 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     // sequences without a position: nothing to attend to, the output row is zero
     for (int b = block; b < p.batch; b += blocks) {
       if (kv4_length(p, b)) continue;
-      for (int i = threadIdx.x; i < p.heads * kD / 8; i += kKv4Warps * 32)
+      for (int i = threadIdx.x; i < p.heads * kD / 8; i += kKv4Threads)
         reinterpret_cast<uint4*>(p.out)[static_cast<long long>(b) * p.heads * kD / 8 + i] = make_uint4(0, 0, 0, 0);
       if (p.lse)
-        for (int i = threadIdx.x; i < p.heads; i += kKv4Warps * 32)
+        for (int i = threadIdx.x; i < p.heads; i += kKv4Threads)
           p.lse[static_cast<long long>(b) * p.heads + i] = -INFINITY;
     }
     const int g = lane >> 2, t = lane & 3;
     // ldmatrix: lane l gives the address of row l & 7 of matrix l >> 3, which are (positions 0-7, 8-15) x
     // (an even, the next odd 16-byte chunk); chunks are swizzled, chunk ^ bits 7-9 of the offset.
     const uint32_t matrix_row = (warp * 16 + ((lane >> 3) & 1) * 8 + (lane & 7)) * kRow + (lane >> 4) * 16;
+    constexpr uint32_t kSubBytes = kKv4Warps * 16 * kRow;       // a multiple of 1024: the swizzle repeats
     const uint32_t matrix_offset = matrix_row ^ (((matrix_row >> 7) & 7) << 4);
-    const int position[2] = {warp * 16 + g, warp * 16 + g + 8};     // rows of the lane's scores
+    const int position0 = warp * 16 + g;                        // first row of the lane's scores
     uint32_t it = 0;
-    bool ok = true;
+    bool ok = true, last_cut = false;
     while (walk.step(p)) {
-      const int kv = walk.row / p.head_blocks, hb = walk.row - kv * p.head_blocks;
-      const int head0 = kv * p.group_heads + hb * kHeads;               // first query head of the block
-      const int heads_here = min(kHeads, p.group_heads - hb * kHeads);
-      // Query fragments: lane (g, t) holds channels 32 j + 8 t + (0..7) of head 8 n + g.
-      uint32_t qf[kNT][kChunks][4];
-      float score_factor[kNT][2], zero_factor[kNT][2][kNG];
-#pragma unroll
-      for (int n = 0; n < kNT; ++n) {
+      const int head0 = walk.kv * p.group_heads + walk.hb * kHeads;     // first query head of the block
+      const int heads_here = min(kHeads, p.group_heads - walk.hb * kHeads);
+      if (warp < kNT) {
+        // Query fragments of eight heads: lane (g, t) prepares channels 32 j + 8 t + (0..7) of head
+        // 8 warp + g, which are the words it will read back.
         float x[kChunks][8], top = 0.0f, sums[kNG];
 #pragma unroll
         for (int i = 0; i < kNG; ++i) sums[i] = 0.0f;
-        const bool live = n * 8 + g < heads_here;
-        const __nv_bfloat16* src = p.q + walk.b * p.q_batch + (head0 + (live ? n * 8 + g : 0)) * p.q_head;
+        const bool live = warp * 8 + g < heads_here;
+        const __nv_bfloat16* src = p.q + walk.b * p.q_batch + (head0 + (live ? warp * 8 + g : 0)) * p.q_head;
+        uint4 raw[kChunks];
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j) raw[j] = *reinterpret_cast<const uint4*>(src + 32 * j + 8 * t);
 #pragma unroll
         for (int j = 0; j < kChunks; ++j) {
-          const uint4 a = *reinterpret_cast<const uint4*>(src + 32 * j + 8 * t);
-          const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+          const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             x[j][2 * e] = live ? bf16_lo(w[e]) : 0.0f;
@@ -534,23 +557,32 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         exponent = min(exponent, 100);
         const float up = exp2f(static_cast<float>(exponent));
 #pragma unroll
-        for (int j = 0; j < kChunks; ++j)
+        for (int j = 0; j < kChunks; ++j) {
+          uint32_t w[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float f = (e & 1) ? up * 0.0625f : up;      // odd nibbles enter 16 times too large
             const __half2 h = __floats2half2_rn(x[j][e] * f, x[j][e + 4] * f);
-            qf[n][j][e] = *reinterpret_cast<const uint32_t*>(&h);
+            w[e] = *reinterpret_cast<const uint32_t*>(&h);
           }
-        // scores: lane (g, t) holds heads 2 t and 2 t + 1 of the tile
-        const float factor = exp2f(static_cast<float>(-exponent)) * p.scale_log2;
+          query[warp][j][lane] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        if (t == 0) {
+          factors[warp * 8 + g][0] = exp2f(static_cast<float>(-exponent)) * p.scale_log2;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          score_factor[n][c] = __shfl_sync(0xffffffffu, factor, 4 * (2 * t + c));
-#pragma unroll
-          for (int i = 0; i < kNG; ++i)
-            zero_factor[n][c][i] = __shfl_sync(0xffffffffu, sums[i], 4 * (2 * t + c)) * p.scale_log2;
+          for (int i = 0; i < kNG; ++i) factors[warp * 8 + g][1 + i] = sums[i] * p.scale_log2;
         }
       }
+      __syncthreads();
+      float score_factor[kNT][2], zero_factor[kNT][2][kNG];    // lane (g, t): heads 2 t and 2 t + 1 of a tile
+#pragma unroll
+      for (int n = 0; n < kNT; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          score_factor[n][c] = factors[n * 8 + 2 * t + c][0];
+#pragma unroll
+          for (int i = 0; i < kNG; ++i) zero_factor[n][c][i] = factors[n * 8 + 2 * t + c][1 + i];
+        }
       float acc[kNT][kMT][4], zeros[kNT][2][kNG], ref[kNT][2], sum[kNT][2];
       float limit = 0.0f, inverse_limit = 0.0f;        // power of two above every value scale so far
 #pragma unroll
@@ -587,62 +619,73 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         if (ok && warp * 16 < live) {
           const uint32_t keys = base + s * kStage, values = keys + kCodes;
           const uint32_t key_scales = values + kCodes, value_scales = key_scales + kScales;
-          float score[kNT][4];
-          {
-            float dot[kNT][kNG][4];
+          float dot[kKv4Sub][kNT][kNG][4];
+#pragma unroll
+          for (int u = 0; u < kKv4Sub; ++u)
 #pragma unroll
             for (int n = 0; n < kNT; ++n)
 #pragma unroll
               for (int i = 0; i < kNG; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) dot[n][i][e] = 0.0f;
+                for (int e = 0; e < 4; ++e) dot[u][n][i][e] = 0.0f;
 #pragma unroll
-            for (int jj = 0; jj < kChunks / 2; ++jj) {
-              uint32_t w[4];
-              load_matrices<false>((keys + matrix_offset) ^ (jj << 5), w);
+          for (int jj = 0; jj < kChunks / 2; ++jj) {
+            uint32_t w[kKv4Sub][4];
 #pragma unroll
-              for (int q = 0; q < 2; ++q) {
-                const int j = 2 * jj + q, i = j * kNG / kChunks;
+            for (int u = 0; u < kKv4Sub; ++u) load_matrices<false>((keys + u * kSubBytes + matrix_offset) ^ (jj << 5), w[u]);
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              const int j = 2 * jj + q, i = j * kNG / kChunks;
+              uint4 qf[kNT];
+#pragma unroll
+              for (int n = 0; n < kNT; ++n) qf[n] = query[n][j][lane];
+#pragma unroll
+              for (int u = 0; u < kKv4Sub; ++u)
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                  const uint32_t lo = half ? w[2 * q] >> 8 : w[2 * q], hi = half ? w[2 * q + 1] >> 8 : w[2 * q + 1];
+                  const uint32_t lo = half ? w[u][2 * q] >> 8 : w[u][2 * q], hi = half ? w[u][2 * q + 1] >> 8 : w[u][2 * q + 1];
                   const uint32_t a[4] = {lo & 0x000f000fu, hi & 0x000f000fu, lo & 0x00f000f0u, hi & 0x00f000f0u};
 #pragma unroll
-                  for (int n = 0; n < kNT; ++n) mma_f16(dot[n][i], a, qf[n][j][2 * half], qf[n][j][2 * half + 1]);
+                  for (int n = 0; n < kNT; ++n)
+                    mma_f16(dot[u][n][i], a, half ? qf[n].z : qf[n].x, half ? qf[n].w : qf[n].y);
                 }
-              }
             }
+          }
+          float score[kKv4Sub][kNT][4];
+          uint32_t value_pair[kKv4Sub][2][kNG];
+#pragma unroll
+          for (int u = 0; u < kKv4Sub; ++u)
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
+              const int position = u * (kKv4Warps * 16) + position0 + 8 * r;
               uint32_t pair[kNG];
-              load_pairs<kNG>(key_scales + position[r] * (kNG * 4), pair);
+              load_pairs<kNG>(key_scales + position * (kNG * 4), pair);
+              load_pairs<kNG>(value_scales + position * (kNG * 4), value_pair[u][r]);
 #pragma unroll
               for (int n = 0; n < kNT; ++n)
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                  float x = dot[n][0][2 * r + c] * bf16_lo(pair[0]), z = bf16_hi(pair[0]) * zero_factor[n][c][0];
+                  float x = dot[u][n][0][2 * r + c] * bf16_lo(pair[0]), z = bf16_hi(pair[0]) * zero_factor[n][c][0];
 #pragma unroll
                   for (int i = 1; i < kNG; ++i) {
-                    x = fmaf(dot[n][i][2 * r + c], bf16_lo(pair[i]), x);
+                    x = fmaf(dot[u][n][i][2 * r + c], bf16_lo(pair[i]), x);
                     z = fmaf(bf16_hi(pair[i]), zero_factor[n][c][i], z);
                   }
-                  score[n][2 * r + c] = fmaf(x * 0x1p24f, score_factor[n][c], z);
+                  score[u][n][2 * r + c] = fmaf(x * 0x1p24f, score_factor[n][c], z);
                 }
             }
-          }
-          uint32_t value_pair[2][kNG];
-#pragma unroll
-          for (int r = 0; r < 2; ++r) load_pairs<kNG>(value_scales + position[r] * (kNG * 4), value_pair[r]);
-          if (warp * 16 + 16 > live) {
+          if (live < kKv4Tile) {
             // what lies behind the sequence, NaN included, weighs nothing
 #pragma unroll
-            for (int r = 0; r < 2; ++r)
-              if (position[r] >= live) {
+            for (int u = 0; u < kKv4Sub; ++u)
 #pragma unroll
-                for (int n = 0; n < kNT; ++n) score[n][2 * r] = score[n][2 * r + 1] = -INFINITY;
+              for (int r = 0; r < 2; ++r)
+                if (u * (kKv4Warps * 16) + position0 + 8 * r >= live) {
 #pragma unroll
-                for (int i = 0; i < kNG; ++i) value_pair[r][i] = 0;
-              }
+                  for (int n = 0; n < kNT; ++n) score[u][n][2 * r] = score[u][n][2 * r + 1] = -INFINITY;
+#pragma unroll
+                  for (int i = 0; i < kNG; ++i) value_pair[u][r][i] = 0;
+                }
           }
           // The reference point of a head's exponentials is 2^7 below the largest score when it was last
           // set, and is set again only when a score exceeds that one by 2^8 or more (most tiles need
@@ -650,19 +693,24 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           // those down to 2^-31 of the largest.
           bool raise = false;
 #pragma unroll
-          for (int n = 0; n < kNT; ++n)
+          for (int u = 0; u < kKv4Sub; ++u) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) raise |= score[n][e] > ref[n][e & 1] + 15.0f;
+            for (int n = 0; n < kNT; ++n)
 #pragma unroll
-          for (int r = 0; r < 2; ++r)
-#pragma unroll
-            for (int i = 0; i < kNG; ++i) raise |= bf16_lo(value_pair[r][i]) > limit;
-          if (__any_sync(0xffffffffu, raise)) {
-            float most = 0.0f;
+              for (int e = 0; e < 4; ++e) raise |= score[u][n][e] > ref[n][e & 1] + 15.0f;
 #pragma unroll
             for (int r = 0; r < 2; ++r)
 #pragma unroll
-              for (int i = 0; i < kNG; ++i) most = fmaxf(most, bf16_lo(value_pair[r][i]));
+              for (int i = 0; i < kNG; ++i) raise |= bf16_lo(value_pair[u][r][i]) > limit;
+          }
+          if (__any_sync(0xffffffffu, raise)) {
+            float most = 0.0f;
+#pragma unroll
+            for (int u = 0; u < kKv4Sub; ++u)
+#pragma unroll
+              for (int r = 0; r < 2; ++r)
+#pragma unroll
+                for (int i = 0; i < kNG; ++i) most = fmaxf(most, bf16_lo(value_pair[u][r][i]));
 #pragma unroll
             for (int o = 4; o < 32; o *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
             float rescale = 1.0f;
@@ -676,7 +724,9 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
             for (int n = 0; n < kNT; ++n)
 #pragma unroll
               for (int c = 0; c < 2; ++c) {
-                float m = fmaxf(score[n][c], score[n][2 + c]);
+                float m = -INFINITY;
+#pragma unroll
+                for (int u = 0; u < kKv4Sub; ++u) m = fmaxf(m, fmaxf(score[u][n][c], score[u][n][2 + c]));
 #pragma unroll
                 for (int o = 4; o < 32; o *= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
                 float f = 1.0f;
@@ -695,43 +745,46 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
                 }
               }
           }
-          float weight[kNT][4];
 #pragma unroll
-          for (int n = 0; n < kNT; ++n)
+          for (int u = 0; u < kKv4Sub; ++u) {
+            float (&weight)[kNT][4] = score[u];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              weight[n][e] = exp2_approx(score[n][e] - ref[n][e & 1]);
-              sum[n][e & 1] += weight[n][e];
-            }
-          uint32_t pf[kNT][kNG][2];
+            for (int n = 0; n < kNT; ++n)
 #pragma unroll
-          for (int i = 0; i < kNG; ++i)
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              const float scale = bf16_lo(value_pair[r][i]) * inverse_limit, zero = bf16_hi(value_pair[r][i]);
-#pragma unroll
-              for (int n = 0; n < kNT; ++n) {
-                const __half2 h = __floats2half2_rn(weight[n][2 * r] * scale, weight[n][2 * r + 1] * scale);
-                pf[n][i][r] = transpose_8x8(*reinterpret_cast<const uint32_t*>(&h));
-#pragma unroll
-                for (int c = 0; c < 2; ++c) zeros[n][c][i] = fmaf(weight[n][2 * r + c], zero, zeros[n][c][i]);
+              for (int e = 0; e < 4; ++e) {
+                weight[n][e] = exp2_approx(score[u][n][e] - ref[n][e & 1]);
+                sum[n][e & 1] += weight[n][e];
               }
-            }
-          // A chunk of 32 channels: lane (g, t) holds channels 4 g .. 4 g + 3 of positions 2 t, 2 t + 1 (and + 8);
-          // two tiles of 16 channels, row g the even and row g + 8 the odd channel (16 times too large).
+            uint32_t pf[kNT][kNG][2];
 #pragma unroll
-          for (int jj = 0; jj < kChunks / 2; ++jj) {
-            uint32_t w[4];
-            load_matrices<true>((values + matrix_offset) ^ (jj << 5), w);
+            for (int i = 0; i < kNG; ++i)
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              const int j = 2 * jj + q, i = j * kNG / kChunks;
+              for (int r = 0; r < 2; ++r) {
+                const float scale = bf16_lo(value_pair[u][r][i]) * inverse_limit, zero = bf16_hi(value_pair[u][r][i]);
 #pragma unroll
-              for (int half = 0; half < 2; ++half) {
-                const uint32_t lo = half ? w[2 * q] >> 8 : w[2 * q], hi = half ? w[2 * q + 1] >> 8 : w[2 * q + 1];
-                const uint32_t a[4] = {lo & 0x000f000fu, lo & 0x00f000f0u, hi & 0x000f000fu, hi & 0x00f000f0u};
+                for (int n = 0; n < kNT; ++n) {
+                  const __half2 h = __floats2half2_rn(weight[n][2 * r] * scale, weight[n][2 * r + 1] * scale);
+                  pf[n][i][r] = transpose_8x8(*reinterpret_cast<const uint32_t*>(&h));
 #pragma unroll
-                for (int n = 0; n < kNT; ++n) mma_f16(acc[n][2 * j + half], a, pf[n][i][0], pf[n][i][1]);
+                  for (int c = 0; c < 2; ++c) zeros[n][c][i] = fmaf(weight[n][2 * r + c], zero, zeros[n][c][i]);
+                }
+              }
+            // A chunk of 32 channels: lane (g, t) holds channels 4 g .. 4 g + 3 of positions 2 t, 2 t + 1 (and + 8);
+            // two tiles of 16 channels, row g the even and row g + 8 the odd channel (16 times too large).
+#pragma unroll
+            for (int jj = 0; jj < kChunks / 2; ++jj) {
+              uint32_t w[4];
+              load_matrices<true>((values + u * kSubBytes + matrix_offset) ^ (jj << 5), w);
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {
+                const int j = 2 * jj + q, i = j * kNG / kChunks;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                  const uint32_t lo = half ? w[2 * q] >> 8 : w[2 * q], hi = half ? w[2 * q + 1] >> 8 : w[2 * q + 1];
+                  const uint32_t a[4] = {lo & 0x000f000fu, lo & 0x00f000f0u, hi & 0x000f000fu, hi & 0x00f000f0u};
+#pragma unroll
+                  for (int n = 0; n < kNT; ++n) mma_f16(acc[n][2 * j + half], a, pf[n][i][0], pf[n][i][1]);
+                }
               }
             }
           }
@@ -740,18 +793,22 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         __syncwarp();
         if (lane == 0) mbar_arrive(empty(s));
       }
-      // ---- the eight warps' parts of this piece meet
+      // ---- the warps' parts of this piece meet, four heads (those of one accumulator column) at a time
+      const bool whole = walk.count == walk.tiles;
+      last_cut = walk.first == 0 && !whole;
+      const int slot = walk.first == 0 ? 1 : 0;   // part 0: the row began in an earlier block
 #pragma unroll
       for (int n = 0; n < kNT; ++n)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
+          if (n | c) __syncthreads();
 #pragma unroll
           for (int o = 4; o < 32; o *= 2) sum[n][c] += __shfl_xor_sync(0xffffffffu, sum[n][c], o);
 #pragma unroll
           for (int i = 0; i < kNG; ++i)
 #pragma unroll
             for (int o = 4; o < 32; o *= 2) zeros[n][c][i] += __shfl_xor_sync(0xffffffffu, zeros[n][c][i], o);
-          float* mine = join + (warp * kHeads + n * 8 + 2 * t + c) * kPitch + g * 4;
+          float* mine = join + (warp * 4 + t) * kPitch + g * 4;
           const float even = limit * 0x1p24f, odd = limit * 0x1p20f;
 #pragma unroll
           for (int j = 0; j < kChunks; ++j) {
@@ -761,48 +818,56 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
                             fmaf(acc[n][2 * j + 1][c], even, zero), fmaf(acc[n][2 * j + 1][2 + c], odd, zero));
           }
           if (g == 0) {
-            join_ml[(warp * kHeads + n * 8 + 2 * t + c) * 2] = ref[n][c];
-            join_ml[(warp * kHeads + n * 8 + 2 * t + c) * 2 + 1] = sum[n][c];
+            join_ml[(warp * 4 + t) * 2] = ref[n][c];
+            join_ml[(warp * 4 + t) * 2 + 1] = sum[n][c];
+          }
+          __syncthreads();
+          static_assert(kKv4Threads == 4 * 32 && kD / 4 <= 32, "a thread joins four channels of one head");
+          const int place = threadIdx.x / (kD / 4), channel = (threadIdx.x - place * (kD / 4)) * 4;
+          const int head = 8 * n + 2 * place + c;
+          if (place >= 4 || head >= heads_here) continue;
+          float m = -INFINITY;
+#pragma unroll
+          for (int w = 0; w < kKv4Warps; ++w) m = fmaxf(m, join_ml[(w * 4 + place) * 2]);
+          float total = 0.0f;
+          float4 o = make_float4(0, 0, 0, 0);
+#pragma unroll
+          for (int w = 0; w < kKv4Warps; ++w) {
+            const float mw = join_ml[(w * 4 + place) * 2], lw = join_ml[(w * 4 + place) * 2 + 1];
+            const float f = mw == -INFINITY ? (lw == 0.0f ? 0.0f : 1.0f) : exp2f(mw - m);
+            const float4 x = *reinterpret_cast<const float4*>(join + (w * 4 + place) * kPitch + channel);
+            total = fmaf(lw, f, total);
+            o.x = fmaf(x.x, f, o.x);
+            o.y = fmaf(x.y, f, o.y);
+            o.z = fmaf(x.z, f, o.z);
+            o.w = fmaf(x.w, f, o.w);
+          }
+          if (whole) {
+            const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+            const long long at = static_cast<long long>(walk.b) * p.heads + head0 + head;
+            *reinterpret_cast<uint2*>(p.out + at * kD + channel) =
+                make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+            if (p.lse && channel == 0) p.lse[at] = (m + log2f(total)) * 0.69314718055994531f;
+          } else {
+            const long long at = (static_cast<long long>(block) * 2 + slot) * kHeads + head;
+            *reinterpret_cast<float4*>(p.parts + at * kD + channel) = o;
+            if (channel == 0) {
+              float* ml = p.parts + static_cast<long long>(blocks) * 2 * kHeads * kD + at * 2;
+              ml[0] = m;
+              ml[1] = total;
+            }
           }
         }
-      __syncthreads();
-      const bool whole = walk.count == walk.tiles;
-      const int slot = walk.first == 0 ? 1 : 0;   // part 0: the row began in an earlier block
-      for (int i = threadIdx.x; i < heads_here * (kD / 4); i += kKv4Warps * 32) {
-        const int head = i / (kD / 4), channel = (i - head * (kD / 4)) * 4;
-        float m = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < kKv4Warps; ++w) m = fmaxf(m, join_ml[(w * kHeads + head) * 2]);
-        float total = 0.0f;
-        float4 o = make_float4(0, 0, 0, 0);
-#pragma unroll
-        for (int w = 0; w < kKv4Warps; ++w) {
-          const float mw = join_ml[(w * kHeads + head) * 2];
-          const float f = mw == -INFINITY ? (join_ml[(w * kHeads + head) * 2 + 1] == 0.0f ? 0.0f : 1.0f) : exp2f(mw - m);
-          const float4 x = *reinterpret_cast<const float4*>(join + (w * kHeads + head) * kPitch + channel);
-          total = fmaf(join_ml[(w * kHeads + head) * 2 + 1], f, total);
-          o.x = fmaf(x.x, f, o.x);
-          o.y = fmaf(x.y, f, o.y);
-          o.z = fmaf(x.z, f, o.z);
-          o.w = fmaf(x.w, f, o.w);
-        }
-        if (whole) {
-          const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-          const long long at = static_cast<long long>(walk.b) * p.heads + head0 + head;
-          *reinterpret_cast<uint2*>(p.out + at * kD + channel) =
-              make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
-          if (p.lse && channel == 0) p.lse[at] = (m + log2f(total)) * 0.69314718055994531f;
-        } else {
-          const long long at = (static_cast<long long>(block) * 2 + slot) * kHeads + head;
-          *reinterpret_cast<float4*>(p.parts + at * kD + channel) = o;
-          if (channel == 0) {
-            float* ml = p.parts + static_cast<long long>(blocks) * 2 * kHeads * kD + at * 2;
-            ml[0] = m;
-            ml[1] = total;
-          }
-        }
+      // (the next piece writes the join area behind the barrier that follows its query)
+    }
+    // The row that this run began and did not end, for the joining kernel.
+    if (threadIdx.x == 0) {
+      int4 cut = make_int4(0, 0, 0, 0);
+      if (last_cut) {
+        const long long row_end = walk.base + static_cast<long long>(walk.row + 1) * walk.tiles;
+        cut = make_int4(walk.b, walk.row, kv4_block_of(start.total, start.runs, row_end - 1), 1);
       }
-      __syncthreads();   // the join area is free again
+      p.cuts[block] = cut;
     }
     // After a wait that gave up, nothing may still be in flight into this block's shared memory.
     if (__syncthreads_or(!ok))
@@ -811,44 +876,89 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   }
 }
 
-// Joins the parts of the rows that the runs cut: block i looks at the boundary between runs i and
-// i + 1 and serves the row there if it is the row's first boundary.  One head per blockIdx.y.
-template <int kD>
-__global__ void __launch_bounds__(kD) kv4_join_kernel(const Kv4Attend p, int blocks, int heads_per_block) {
-  __shared__ long long scratch[kD / 32 + 2];
+// Joins the parts of the row that block blockIdx.x began and did not end.  A warp takes one head and
+// every kGroups-th part, lanes the channels; the groups meet in shared memory, all in a fixed order.
+constexpr int kKv4JoinThreads = 1024;
+template <int kD, int kHeads>
+__global__ void __launch_bounds__(kKv4JoinThreads) kv4_join_kernel(const Kv4Attend p, int blocks) {
+  constexpr int kGroups = kKv4JoinThreads / 32 / kHeads, kPerLane = kD / 32;
+  __shared__ float sums[kGroups][kHeads][kD], ml_shared[kGroups][kHeads][2];
   grid_dependents_may_launch();
-  const int boundary = blockIdx.x + 1;
-  const Kv4Start s = kv4_locate<kD>(p, blocks, boundary, scratch);   // reads only the lengths
   grid_dependency_wait();
-  const long long tile = kv4_first_tile(s.total, blocks, boundary);
-  if (s.total == 0 || tile >= s.total) return;
-  const int tiles = kv4_tiles(kv4_length(p, s.sequence));
-  const int row = int((tile - s.tile_base) / tiles);
-  const long long begin = s.tile_base + static_cast<long long>(row) * tiles;
-  if (begin == tile) return;                                          // the boundary falls between two rows
-  const int first = kv4_block_of(s.total, blocks, begin), last = kv4_block_of(s.total, blocks, begin + tiles - 1);
-  if (kv4_first_tile(s.total, blocks, boundary - 1) > begin) return;  // not the first boundary inside the row
-  const int kv = row / p.head_blocks, hb = row - kv * p.head_blocks;
-  const int head = blockIdx.y;
-  if (hb * heads_per_block + head >= p.group_heads) return;
-  const float* ml = p.parts + static_cast<long long>(blocks) * 2 * heads_per_block * kD;
-  float m = -INFINITY;
-  auto part_of = [&](int c) { return (static_cast<long long>(c) * 2 + (c == first ? 1 : 0)) * heads_per_block + head; };
-  auto held = [&](int c) { return kv4_first_tile(s.total, blocks, c) != kv4_first_tile(s.total, blocks, c + 1); };
-  for (int c = first; c <= last; ++c)
-    if (held(c)) m = fmaxf(m, ml[part_of(c) * 2]);
-  float total = 0.0f, o = 0.0f;
-#pragma unroll 4
-  for (int c = first; c <= last; ++c) {
-    if (!held(c)) continue;
-    const float mc = ml[part_of(c) * 2], lc = ml[part_of(c) * 2 + 1];
-    const float f = mc == -INFINITY ? (lc == 0.0f ? 0.0f : 1.0f) : exp2f(mc - m);
-    total = fmaf(lc, f, total);
-    o = fmaf(p.parts[part_of(c) * kD + threadIdx.x], f, o);
+  const int4 cut = p.cuts[blockIdx.x];
+  if (!cut.w) return;
+  const int first = blockIdx.x, last = cut.z;
+  const int head = (threadIdx.x >> 5) % kHeads, group = (threadIdx.x >> 5) / kHeads, lane = threadIdx.x & 31;
+  const float* parts_ml = p.parts + static_cast<long long>(blocks) * 2 * kHeads * kD;
+  float m = -INFINITY, total = 0.0f, o[kPerLane];
+#pragma unroll
+  for (int e = 0; e < kPerLane; ++e) o[e] = 0.0f;
+  constexpr int kBatch = 8;      // parts whose loads are in flight together
+  for (int c0 = first + group; c0 <= last; c0 += kBatch * kGroups) {
+    float x[kBatch][kPerLane], mc[kBatch], lc[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int c = c0 + u * kGroups;
+      const long long at = (static_cast<long long>(c) * 2 + (c == first ? 1 : 0)) * kHeads + head;
+      mc[u] = -INFINITY;
+      lc[u] = 0.0f;
+#pragma unroll
+      for (int e = 0; e < kPerLane; ++e) x[u][e] = 0.0f;
+      if (c <= last) {
+        const float2 ml = *reinterpret_cast<const float2*>(parts_ml + at * 2);
+        mc[u] = ml.x;
+        lc[u] = ml.y;
+        if (kPerLane == 4) {
+          const float4 v = *reinterpret_cast<const float4*>(p.parts + at * kD + lane * 4);
+          x[u][0] = v.x; x[u][1] = v.y; x[u][2 % kPerLane] = v.z; x[u][3 % kPerLane] = v.w;
+        } else {
+          const float2 v = *reinterpret_cast<const float2*>(p.parts + at * kD + lane * 2);
+          x[u][0] = v.x; x[u][1] = v.y;
+        }
+      }
+    }
+    float top = m;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) top = fmaxf(top, mc[u]);
+    const float back = m == -INFINITY ? (total == 0.0f ? 0.0f : 1.0f) : exp2f(m - top);
+    total *= back;
+#pragma unroll
+    for (int e = 0; e < kPerLane; ++e) o[e] *= back;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const float f = mc[u] == -INFINITY ? (lc[u] == 0.0f ? 0.0f : 1.0f) : exp2f(mc[u] - top);
+      total = fmaf(lc[u], f, total);
+#pragma unroll
+      for (int e = 0; e < kPerLane; ++e) o[e] = fmaf(x[u][e], f, o[e]);
+    }
+    m = top;
   }
-  const long long at = static_cast<long long>(s.sequence) * p.heads + kv * p.group_heads + hb * heads_per_block + head;
-  p.out[at * kD + threadIdx.x] = __float2bfloat16(total == 0.0f ? 0.0f : o / total);
-  if (p.lse && threadIdx.x == 0) p.lse[at] = (m + log2f(total)) * 0.69314718055994531f;
+#pragma unroll
+  for (int e = 0; e < kPerLane; ++e) sums[group][head][lane * kPerLane + e] = o[e];
+  if (lane == 0) {
+    ml_shared[group][head][0] = m;
+    ml_shared[group][head][1] = total;
+  }
+  __syncthreads();
+  const int kv = cut.y / p.head_blocks, hb = cut.y - kv * p.head_blocks;
+  const int head0 = kv * p.group_heads + hb * kHeads;
+  for (int i = threadIdx.x; i < kHeads * kD; i += kKv4JoinThreads) {
+    const int h = i / kD, channel = i - h * kD;
+    if (hb * kHeads + h >= p.group_heads) break;
+    float top = -INFINITY, all = 0.0f, sum = 0.0f;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) top = fmaxf(top, ml_shared[g][h][0]);
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      const float mg = ml_shared[g][h][0], lg = ml_shared[g][h][1];
+      const float f = mg == -INFINITY ? (lg == 0.0f ? 0.0f : 1.0f) : exp2f(mg - top);
+      all = fmaf(lg, f, all);
+      sum = fmaf(sums[g][h][channel], f, sum);
+    }
+    const long long at = static_cast<long long>(cut.x) * p.heads + head0 + h;
+    p.out[at * kD + channel] = __float2bfloat16(all == 0.0f ? 0.0f : sum / all);
+    if (p.lse && channel == 0) p.lse[at] = (top + log2f(all)) * 0.69314718055994531f;
+  }
 }
 
 int check_kv4_cache(const char* what, const trinity_sm100_kv4_cache& c) {
@@ -908,15 +1018,15 @@ int launch_kv4_attend(const Kv4Attend& p, const CUtensorMap& map_k, const CUtens
     count_launch();
   }
   if (blocks > 1) {
-    KernelLaunch launch(dim3(blocks - 1, 8 * kNT), dim3(kD), 0, stream);
-    cudaError_t e = cudaLaunchKernelEx(&launch.config, kv4_join_kernel<kD>, p, blocks, 8 * kNT);
+    KernelLaunch launch(dim3(blocks), dim3(kKv4JoinThreads), 0, stream);
+    cudaError_t e = cudaLaunchKernelEx(&launch.config, kv4_join_kernel<kD, 8 * kNT>, p, blocks);
     if (e != cudaSuccess) return fail(TRINITY_SM100_E_CUDA, "kv4_join launch: %s", cudaGetErrorString(e));
     count_launch();
   }
   return check_launch("kv4_decode");
 }
 
-int kv4_blocks(int sm_count, int group_heads) { return group_heads > 8 ? sm_count : 2 * sm_count; }
+int kv4_blocks(int sm_count) { return kKv4PerSm * sm_count; }
 
 }  // namespace
 }  // namespace trinity_sm100
@@ -980,7 +1090,8 @@ extern "C" size_t trinity_sm100_kv4_decode_workspace_bytes(int32_t heads, int32_
   int sm_count = 0;
   if (heads <= 0 || kv_heads <= 0 || head_dim <= 0 || heads % kv_heads || require_sm100(&sm_count)) return 0;
   const int group_heads = heads / kv_heads;
-  return size_t(kv4_blocks(sm_count, group_heads)) * 2 * (group_heads > 8 ? 16 : 8) * (size_t(head_dim) + 2) * 4;
+  const size_t blocks = kv4_blocks(sm_count);
+  return blocks * 2 * (group_heads > 8 ? 16 : 8) * (size_t(head_dim) + 2) * 4 + blocks * sizeof(int4);
 }
 
 extern "C" int trinity_sm100_kv4_decode(const trinity_sm100_kv4_cache* cache, const trinity_sm100_kv4_decode_args* args,
@@ -1030,13 +1141,16 @@ extern "C" int trinity_sm100_kv4_decode(const trinity_sm100_kv4_cache* cache, co
   p.max_pages = a.max_pages;
   p.box = kKv4Tile;                     // positions a copy fetches: the largest power of two that pages and tiles share
   while (c.page % p.box) p.box /= 2;
+  p.box_shift = __builtin_ctz(p.box);
+  p.page_shift = (c.page & (c.page - 1)) == 0 ? __builtin_ctz(c.page) : -1;
   p.scale_log2 = a.scale * 1.4426950408889634f;
   CUtensorMap map_k, map_v;
   const uint64_t lines = static_cast<uint64_t>(c.pages) * c.kv_heads * c.page * (c.head_dim / 2) / 128;
   const uint32_t box_lines = p.box * (c.head_dim / 2) / 128;
   if (int rc = make_tensor_map_3d(&map_k, c.k_codes, 2, 64, lines, 1, 128, 128 * lines, 64, box_lines, 1, 128)) return rc;
   if (int rc = make_tensor_map_3d(&map_v, c.v_codes, 2, 64, lines, 1, 128, 128 * lines, 64, box_lines, 1, 128)) return rc;
-  const int blocks = kv4_blocks(sm_count, p.group_heads);
+  const int blocks = kv4_blocks(sm_count);
+  p.cuts = reinterpret_cast<int4*>(p.parts + static_cast<size_t>(blocks) * 2 * block_heads * (c.head_dim + 2));
   cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
   const int groups = c.head_dim / c.group;
 #define TRINITY_KV4(D, NG) \
