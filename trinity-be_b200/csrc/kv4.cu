@@ -161,8 +161,9 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Rows p) {
 // keeps up, so:
 //
 // * The positions of all (sequence, cached head) rows are cut into tiles of 128 and the tiles, in
-//   order, into equal runs, one for each thread block of a grid that fills the GPU once: whatever the
-//   lengths are (they are read on the device), every SM streams the same share.  A row that one
+//   order, into equal runs, one for each thread block of a grid that fills the GPU once (a row
+//   counts two tiles more than it has: what its start and end cost): whatever the lengths are (they
+//   are read on the device), every SM has the same share.  A row that one
 //   block holds whole is written at once; the parts of a row that is cut go to the workspace and a
 //   second kernel joins them in block order, so results do not depend on timing.
 // * Tiles are fetched into a ring of stages: codes by tiled TMA as rows of 128 bytes (two or four
@@ -192,7 +193,10 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Rows p) {
 constexpr int kKv4Tile = 128;          // positions in a stage
 constexpr int kKv4Warps = 4;
 constexpr int kKv4Sub = kKv4Tile / (16 * kKv4Warps);   // groups of 16 positions a warp takes of each tile
-constexpr int kKv4PerSm = 3;           // resident blocks: twelve warps of 168 registers
+constexpr int kKv4RowUnits = 2;
+// Resident blocks an SM: three (twelve warps of 168 registers), or two where sixteen heads with four
+// groups of scales each need more registers and shared memory.
+__host__ __device__ constexpr int kv4_per_sm(int groups, int head_tiles) { return groups * head_tiles > 4 ? 2 : 3; }
 constexpr uint32_t kKv4Lag = 2;
 constexpr int kKv4Threads = kKv4Warps * 32;
 
@@ -214,7 +218,7 @@ struct Kv4Attend {
 
 // Where the run of one block starts, and the size of all.
 struct Kv4Start {
-  long long total, tile_base;   // tiles of all rows; tiles before sequence `sequence`
+  long long total, base;        // units of all rows; units before sequence `sequence`
   int sequence, runs;           // runs: blocks that have one
 };
 
@@ -226,13 +230,17 @@ __device__ __forceinline__ int kv4_length(const Kv4Attend& p, int b) {
 __device__ __forceinline__ int kv4_page_of(const Kv4Attend& p, int position) {
   return p.page_shift >= 0 ? position >> p.page_shift : position / p.page;
 }
-__device__ __forceinline__ int kv4_tiles(int length) { return (length + kKv4Tile - 1) / kKv4Tile; }
-// First tile of a block's run; `runs` is at most the number of tiles, so that no run is empty.
-__device__ __forceinline__ long long kv4_first_tile(long long total, int runs, int block) {
+// Units of work of a row: its tiles, and what starting and ending a row costs beside them (none for an
+// empty sequence).  The runs are equal in units.
+__device__ __forceinline__ int kv4_units(int length) {
+  return length ? (length + kKv4Tile - 1) / kKv4Tile + kKv4RowUnits : 0;
+}
+// First unit of a block's run; `runs` is at most the number of units, so that no run is empty.
+__device__ __forceinline__ long long kv4_first_unit(long long total, int runs, int block) {
   if (total < (1 << 20)) return uint32_t(total) * uint32_t(block) / uint32_t(runs);   // (runs are below 2^11)
   return total * block / runs;
 }
-// Block whose run holds tile t: the largest i with total * i / runs <= t.
+// Block whose run holds unit t: the largest i with total * i / runs <= t.
 __device__ __forceinline__ int kv4_block_of(long long total, int runs, long long t) {
   return int(((t + 1) * runs - 1) / total);
 }
@@ -246,7 +254,7 @@ __device__ __forceinline__ Kv4Start kv4_locate(const Kv4Attend& p, int blocks, i
   const int begin = min(p.batch, int(threadIdx.x) * per), end = min(p.batch, begin + per);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   long long sum = 0;
-  for (int b = begin; b < end; ++b) sum += static_cast<long long>(kv4_tiles(kv4_length(p, b))) * rows;
+  for (int b = begin; b < end; ++b) sum += static_cast<long long>(kv4_units(kv4_length(p, b))) * rows;
   long long inclusive = sum;
 #pragma unroll
   for (int o = 1; o < 32; o *= 2) {
@@ -261,11 +269,11 @@ __device__ __forceinline__ Kv4Start kv4_locate(const Kv4Attend& p, int blocks, i
     total += scratch[w];
   }
   const int runs = total < blocks ? int(total) : blocks;
-  const long long first = block < runs ? kv4_first_tile(total, runs, block) : -1;
+  const long long first = block < runs ? kv4_first_unit(total, runs, block) : -1;
   if (first >= base && first < base + sum) {   // exactly one thread, if there is any tile
     int b = begin;
     for (;; ++b) {
-      const long long n = static_cast<long long>(kv4_tiles(kv4_length(p, b))) * rows;
+      const long long n = static_cast<long long>(kv4_units(kv4_length(p, b))) * rows;
       if (first < base + n) break;
       base += n;
     }
@@ -275,7 +283,7 @@ __device__ __forceinline__ Kv4Start kv4_locate(const Kv4Attend& p, int blocks, i
   __syncthreads();
   Kv4Start s;
   s.total = total;
-  s.tile_base = scratch[kWarps];
+  s.base = scratch[kWarps];
   s.sequence = int(scratch[kWarps + 1]);
   s.runs = runs;
   return s;
@@ -283,9 +291,9 @@ __device__ __forceinline__ Kv4Start kv4_locate(const Kv4Attend& p, int blocks, i
 
 // Walks the rows (sequence, cached head, head block) that a run of tiles covers.
 struct Kv4Walk {
-  long long next, end;       // tiles of the run not yet visited
-  long long base;            // first tile of sequence b
-  int b, length, tiles;
+  long long next, end;       // units of the run not yet visited
+  long long base;            // first unit of sequence b
+  int b, length, units, tiles;
   // the current piece
   int row, first, count;     // row within the sequence, first tile of the piece, its tiles (0: the run is over)
   int kv, hb;                // cached head and head block of the row
@@ -294,13 +302,13 @@ struct Kv4Walk {
   __device__ __forceinline__ Kv4Walk(const Kv4Attend& p, const Kv4Start& s, int block) {
     next = end = 0;
     if (block < s.runs) {
-      next = kv4_first_tile(s.total, s.runs, block);
-      end = kv4_first_tile(s.total, s.runs, block + 1);
+      next = kv4_first_unit(s.total, s.runs, block);
+      end = kv4_first_unit(s.total, s.runs, block + 1);
     }
-    base = s.tile_base;
+    base = s.base;
     b = s.sequence;
     length = next < end ? kv4_length(p, b) : 0;
-    tiles = kv4_tiles(length);
+    units = kv4_units(length);
   }
   __device__ __forceinline__ bool step(const Kv4Attend& p) {
     if (next >= end) {
@@ -308,18 +316,28 @@ struct Kv4Walk {
       return false;
     }
     const int rows = p.kv_heads * p.head_blocks;
-    while (next >= base + static_cast<long long>(tiles) * rows) {   // the run ends inside a sequence with tiles
-      base += static_cast<long long>(tiles) * rows;
-      ++b;
-      length = kv4_length(p, b);
-      tiles = kv4_tiles(length);
+    for (;;) {
+      while (next >= base + static_cast<long long>(units) * rows) {   // the run ends inside a sequence with tiles
+        base += static_cast<long long>(units) * rows;
+        ++b;
+        length = kv4_length(p, b);
+        units = kv4_units(length);
+      }
+      const int local = int(next - base);
+      row = local / units;
+      const int from = local - row * units;
+      const long long left = end - next;
+      const int to = int(left < units - from ? from + left : units);
+      next += to - from;
+      tiles = units - kKv4RowUnits;
+      first = max(0, from - kKv4RowUnits);
+      count = to - kKv4RowUnits - first;
+      if (count > 0) break;
+      if (next >= end) {
+        count = 0;
+        return false;
+      }
     }
-    const int local = int(next - base);
-    row = local / tiles;
-    first = local - row * tiles;
-    const long long left = end - next;
-    count = int(left < tiles - first ? left : tiles - first);
-    next += count;
     tile = first;
     kv = p.head_blocks == 1 ? row : row / p.head_blocks;
     hb = row - kv * p.head_blocks;
@@ -329,7 +347,7 @@ struct Kv4Walk {
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -379,12 +397,12 @@ __host__ __device__ constexpr int kv4_join_bytes() {   // four heads' accumulato
 }
 template <int kD, int kNT>
 __host__ __device__ constexpr int kv4_query_bytes() {
-  return kNT * (kD / 32) * 32 * 16;
+  return 2 * kNT * (kD / 32) * 32 * 16;
 }
 template <int kD, int kNG, int kNT>
 __host__ __device__ constexpr int kv4_stages() {
-  // what a third of an SM's 228 KB leaves beside the system's 1 KB a block, static variables and alignment
-  return (228 * 1024 / kKv4PerSm - 3072 - kv4_join_bytes<kD>() - kv4_query_bytes<kD, kNT>()) / kv4_stage_bytes<kD, kNG>();
+  // what a block's share of an SM's 228 KB leaves beside the system's 1 KB a block, static variables and alignment
+  return (228 * 1024 / kv4_per_sm(kNG, kNT) - 3072 - kv4_join_bytes<kD>() - kv4_query_bytes<kD, kNT>()) / kv4_stage_bytes<kD, kNG>();
 }
 template <int kD, int kNG, int kNT>
 __host__ __device__ constexpr int kv4_smem_bytes() {
@@ -393,7 +411,7 @@ __host__ __device__ constexpr int kv4_smem_bytes() {
 }
 
 template <int kD, int kNG, int kNT>
-__global__ void __launch_bounds__(kKv4Threads, kKv4PerSm)
+__global__ void __launch_bounds__(kKv4Threads, kv4_per_sm(kNG, kNT))
 kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                   const Kv4Attend p) {
   constexpr int kRow = kD / 2;                         // bytes of codes a position
@@ -410,6 +428,7 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
   uint4 (*query)[kChunks][32] = reinterpret_cast<uint4 (*)[kChunks][32]>(smem + kStages * kStage);   // [tile of heads][chunk][lane]
+  uint4 (*raw_query)[kChunks][32] = query + kNT;                                                      // the same, as it came
   float* join = reinterpret_cast<float*>(smem + kStages * kStage + kv4_query_bytes<kD, kNT>());       // [warp][head][kPitch]
   float* join_ml = join + kKv4Warps * 4 * kPitch;                                                     // [warp][head][2]
   const uint32_t bars = base + kStages * kStage + kv4_query_bytes<kD, kNT>() + kv4_join_bytes<kD>();
@@ -518,7 +537,25 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     const int position0 = warp * 16 + g;                        // first row of the lane's scores
     uint32_t it = 0;
     bool ok = true, last_cut = false;
-    while (walk.step(p)) {
+    // The query rows of a piece are copied to shared memory while the piece before it is worked on.
+    auto fetch_query = [&](const Kv4Walk& at) {
+      if (warp >= kNT) return;
+      const int in_block = warp * 8 + g, in_group = at.hb * kHeads + in_block;
+      const __nv_bfloat16* src = p.q + at.b * p.q_batch +
+                                 (at.kv * p.group_heads + (in_group < p.group_heads ? in_group : 0)) * p.q_head;
+#pragma unroll
+      for (int j = 0; j < kChunks; ++j)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(smem_u32(&raw_query[warp][j][lane])),
+                     "l"(src + 32 * j + 8 * t)
+                     : "memory");
+    };
+    bool more = walk.step(p);
+    if (more) {
+      fetch_query(walk);
+      asm volatile("cp.async.wait_all;" ::: "memory");
+    }
+    Kv4Walk after = walk;
+    for (; more; walk = after) {
       const int head0 = walk.kv * p.group_heads + walk.hb * kHeads;     // first query head of the block
       const int heads_here = min(kHeads, p.group_heads - walk.hb * kHeads);
       if (warp < kNT) {
@@ -528,10 +565,9 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 #pragma unroll
         for (int i = 0; i < kNG; ++i) sums[i] = 0.0f;
         const bool live = warp * 8 + g < heads_here;
-        const __nv_bfloat16* src = p.q + walk.b * p.q_batch + (head0 + (live ? warp * 8 + g : 0)) * p.q_head;
-        uint4 raw[kChunks];
+        uint4 raw[kChunks];      // written by this very lane, which has waited for its copies
 #pragma unroll
-        for (int j = 0; j < kChunks; ++j) raw[j] = *reinterpret_cast<const uint4*>(src + 32 * j + 8 * t);
+        for (int j = 0; j < kChunks; ++j) raw[j] = raw_query[warp][j][lane];
 #pragma unroll
         for (int j = 0; j < kChunks; ++j) {
           const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
@@ -573,6 +609,8 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           for (int i = 0; i < kNG; ++i) factors[warp * 8 + g][1 + i] = sums[i] * p.scale_log2;
         }
       }
+      more = after.step(p);
+      if (more) fetch_query(after);
       __syncthreads();
       float score_factor[kNT][2], zero_factor[kNT][2][kNG];    // lane (g, t): heads 2 t and 2 t + 1 of a tile
 #pragma unroll
@@ -789,7 +827,7 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
             }
           }
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");    // page numbers, if this warp asked for any
+        asm volatile("cp.async.wait_all;" ::: "memory");    // page numbers or the next query, if this warp asked for any
         __syncwarp();
         if (lane == 0) mbar_arrive(empty(s));
       }
@@ -864,7 +902,7 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     if (threadIdx.x == 0) {
       int4 cut = make_int4(0, 0, 0, 0);
       if (last_cut) {
-        const long long row_end = walk.base + static_cast<long long>(walk.row + 1) * walk.tiles;
+        const long long row_end = walk.base + static_cast<long long>(walk.row + 1) * walk.units;
         cut = make_int4(walk.b, walk.row, kv4_block_of(start.total, start.runs, row_end - 1), 1);
       }
       p.cuts[block] = cut;
@@ -1026,7 +1064,7 @@ int launch_kv4_attend(const Kv4Attend& p, const CUtensorMap& map_k, const CUtens
   return check_launch("kv4_decode");
 }
 
-int kv4_blocks(int sm_count) { return kKv4PerSm * sm_count; }
+int kv4_blocks(int sm_count, int groups, int block_heads) { return kv4_per_sm(groups, block_heads / 8) * sm_count; }
 
 }  // namespace
 }  // namespace trinity_sm100
@@ -1090,7 +1128,7 @@ extern "C" size_t trinity_sm100_kv4_decode_workspace_bytes(int32_t heads, int32_
   int sm_count = 0;
   if (heads <= 0 || kv_heads <= 0 || head_dim <= 0 || heads % kv_heads || require_sm100(&sm_count)) return 0;
   const int group_heads = heads / kv_heads;
-  const size_t blocks = kv4_blocks(sm_count);
+  const size_t blocks = kv4_blocks(sm_count, 1, 8);      // the most that any grouping uses
   return blocks * 2 * (group_heads > 8 ? 16 : 8) * (size_t(head_dim) + 2) * 4 + blocks * sizeof(int4);
 }
 
@@ -1149,7 +1187,7 @@ extern "C" int trinity_sm100_kv4_decode(const trinity_sm100_kv4_cache* cache, co
   const uint32_t box_lines = p.box * (c.head_dim / 2) / 128;
   if (int rc = make_tensor_map_3d(&map_k, c.k_codes, 2, 64, lines, 1, 128, 128 * lines, 64, box_lines, 1, 128)) return rc;
   if (int rc = make_tensor_map_3d(&map_v, c.v_codes, 2, 64, lines, 1, 128, 128 * lines, 64, box_lines, 1, 128)) return rc;
-  const int blocks = kv4_blocks(sm_count);
+  const int blocks = kv4_blocks(sm_count, c.head_dim / c.group, block_heads);
   p.cuts = reinterpret_cast<int4*>(p.parts + static_cast<size_t>(blocks) * 2 * block_heads * (c.head_dim + 2));
   cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
   const int groups = c.head_dim / c.group;
