@@ -196,7 +196,7 @@ constexpr int kKv4Sub = kKv4Tile / (16 * kKv4Warps);   // groups of 16 positions
 constexpr int kKv4RowUnits = 2;
 // Resident blocks an SM: three (twelve warps of 168 registers), or two where sixteen heads with four
 // groups of scales each need more registers and shared memory.
-__host__ __device__ constexpr int kv4_per_sm(int groups, int head_tiles) { return groups * head_tiles > 4 ? 2 : 3; }
+__host__ __device__ constexpr int kv4_per_sm(int groups, int head_tiles) { return head_tiles > 1 ? 2 : 3; }
 constexpr uint32_t kKv4Lag = 2;
 constexpr int kKv4Threads = kKv4Warps * 32;
 
