@@ -34,121 +34,185 @@ struct Kv4Rows {
   const long long* slots;
   long long tokens, positions;     // positions = pages * page
   long long token_stride[2], head_stride[2];
-  int kv_heads, page, group, out_f32;
+  int kv_heads, page, out_f32;
+  int group_shift;                 // logarithm of the group
+  int heads_shift, page_shift;     // logarithms of kv_heads and page, -1 where they are no powers of two
 };
 
-// Row of the cache that holds head `head` of position `slot`.
-__device__ __forceinline__ long long kv4_row(const Kv4Rows& p, long long slot, int head) {
-  const long long page = slot / p.page;
-  return (page * p.kv_heads + head) * p.page + (slot - page * p.page);
+// Row of the cache that holds head `head` of position `slot` (the cache has fewer than 2^31 rows).
+__device__ __forceinline__ long long kv4_row(const Kv4Rows& p, uint32_t slot, uint32_t head) {
+  const uint32_t page = p.page_shift >= 0 ? slot >> p.page_shift : slot / uint32_t(p.page);
+  return static_cast<long long>((page * p.kv_heads + head) * p.page + (slot - page * p.page));
+}
+// The kBatch rows (token, head) of a group of kLanes lanes, a block's rows apart; the launcher keeps
+// all lanes of a launch below 2^31.  All loads of a step are issued before the first use.
+template <int kLanes, int kBatch>
+struct Kv4Batch {
+  uint32_t token[kBatch], head[kBatch];
+  long long slot[kBatch];     // -1: nothing to do
+  bool live[kBatch];
+  __device__ __forceinline__ Kv4Batch(const Kv4Rows& p) {
+    constexpr uint32_t kRows = 256 / kLanes;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const uint32_t index = (blockIdx.x * kBatch + i) * kRows + threadIdx.x / kLanes;
+      token[i] = p.heads_shift >= 0 ? index >> p.heads_shift : index / uint32_t(p.kv_heads);
+      head[i] = index - token[i] * p.kv_heads;
+      live[i] = token[i] < p.tokens;
+      slot[i] = live[i] ? p.slots[token[i]] : -1;
+    }
+  }
+  __device__ __forceinline__ long long offset(const Kv4Rows& p, int which, int i) const {
+    return static_cast<long long>(token[i]) * p.token_stride[which] + static_cast<long long>(head[i]) * p.head_stride[which];
+  }
+};
+
+// Larger of each pair of BF16 values; NaN if either is.
+__device__ __forceinline__ uint32_t nan_max2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ float reciprocal_approx(float x) {   // 2^-23 relative
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 
-template <int kD, bool kVector>
+// The divisions that hardly any group needs, out of line.
+__device__ __noinline__ uint32_t divided_code(float x, float scale) {
+  return static_cast<uint32_t>(fminf(rintf(x / scale), 15.0f));
+}
+__device__ __noinline__ float divided_spread(float spread) { return spread / 15.0f; }
+
+template <int kD, bool kVector, int kBatch>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4Rows p) {
   constexpr int kLanes = kD / 8;
   grid_dependents_may_launch();
   grid_dependency_wait();
-  const int which = blockIdx.y;
-  const long long index = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) / kLanes;
-  const int lane = threadIdx.x % kLanes;
-  const bool live = index < p.tokens * p.kv_heads;   // shuffles below need every lane of the warp
-  const long long token = live ? index / p.kv_heads : 0;
-  const int head = live ? int(index - token * p.kv_heads) : 0;
-  const long long slot = live ? p.slots[token] : -1;
-  bool write = live && slot >= 0;
-  if (write && slot >= p.positions) {
-    write = false;
-    report_timeout(kSiteKv4AppendSlot);
-  }
-  float v[8];
-  const __nv_bfloat16* src = p.in[which] + token * p.token_stride[which] + head * p.head_stride[which] + lane * 8;
-  if (!write) {
+  const int which = blockIdx.y, lane = threadIdx.x % kLanes;
+  const Kv4Batch<kLanes, kBatch> rows(p);
+  uint4 raw[kBatch];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-  } else if (kVector) {
-    const uint4 a = __ldcs(reinterpret_cast<const uint4*>(src));
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+  for (int i = 0; i < kBatch; ++i) {
+    const __nv_bfloat16* src = p.in[which] + rows.offset(p, which, i) + lane * 8;
+    raw[i] = make_uint4(0, 0, 0, 0);
+    if (!rows.live[i]) continue;
+    if (kVector) {
+      raw[i] = __ldcs(reinterpret_cast<const uint4*>(src));
+    } else {
+      const uint16_t* one = reinterpret_cast<const uint16_t*>(src);
+      raw[i] = make_uint4(one[0] | uint32_t(one[1]) << 16, one[2] | uint32_t(one[3]) << 16,
+                          one[4] | uint32_t(one[5]) << 16, one[6] | uint32_t(one[7]) << 16);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kBatch; ++i) {      // (the shuffles need every lane of the warp, rows or not)
+    const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+    // (max, -min) of the group as a BF16 pair; a NaN goes through, an infinity stays one
+    uint32_t extrema = nan_max2(nan_max2(w[0], w[1]), nan_max2(w[2], w[3]));
+    const uint32_t negated = nan_max2(nan_max2(w[0] ^ 0x80008000u, w[1] ^ 0x80008000u),
+                                      nan_max2(w[2] ^ 0x80008000u, w[3] ^ 0x80008000u));
+    extrema = nan_max2(__byte_perm(extrema, negated, 0x5410), __byte_perm(extrema, negated, 0x7632));
+    for (int step = 1; step < 1 << (p.group_shift - 3); step *= 2)     // the lanes of a group are neighbours
+      extrema = nan_max2(extrema, __shfl_xor_sync(0xffffffffu, extrema, step));
+    const float high = bf16_lo(extrema), low = -bf16_hi(extrema), spread = high - low;
+    // spread / 15, correctly rounded: a product with 1 / 15 and one Newton step (the remainder is exact
+    // unless it is subnormal)
+    float fifteenth = spread * (1.0f / 15.0f);
+    fifteenth = fmaf(fmaf(-15.0f, fifteenth, spread), 1.0f / 15.0f, fifteenth);
+    if (!(spread > 0x1p-90f)) fifteenth = divided_spread(spread);
+    const __nv_bfloat16 scale16 = __float2bfloat16(spread < INFINITY ? fifteenth : NAN);
+    const float scale = __bfloat162float(scale16);
+    float v[8];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      v[2 * e] = bf16_lo(w[e]);
-      v[2 * e + 1] = bf16_hi(w[e]);
+      v[2 * e] = bf16_lo(w[e]) - low;
+      v[2 * e + 1] = bf16_hi(w[e]) - low;
     }
-  } else {
+    // code = rint((x - zero) / scale), at most 15.06 before rounding as the scale is rounded by 2^-8 at
+    // most.  BF16 values and scales are so coarse that half of all warps meet a quotient of exactly k + 1/2,
+    // so the quotient must be the correctly rounded one: the product with the correctly rounded
+    // reciprocal, corrected once by its exact remainder (Markstein's division; an 8-bit divisor is
+    // none of its exceptions).
+    uint32_t codes = 0;
+    if (scale > 0x1p-100f) {
+      constexpr float kInteger = 12582912.0f;      // 1.5 * 2^23: adding it rounds to an integer, half to even
+      float inverse = reciprocal_approx(scale);
+      inverse = fmaf(inverse, fmaf(-scale, inverse, 1.0f), inverse);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = __bfloat162float(src[e]);
-  }
-  float low = v[0], high = v[0];
-  bool bad = false;
+      for (int e = 7; e >= 0; --e) {
+        float quotient = v[e] * inverse;
+        quotient = fmaf(fmaf(-quotient, scale, v[e]), inverse, quotient);
+        codes = codes * 16u + __float_as_uint(quotient + kInteger);   // the code in the last four bits
+      }
+      codes -= 0x3f400000u;                        // what the exponents of the eight sums have added up to
+    } else if (scale > 0.0f) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    low = fminf(low, v[e]);
-    high = fmaxf(high, v[e]);
-    bad |= !(fabsf(v[e]) < INFINITY);
-  }
-  for (int step = 1; step < p.group / 8; step *= 2) {   // the lanes of a group are neighbours
-    low = fminf(low, __shfl_xor_sync(0xffffffffu, low, step));
-    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, step));
-    bad |= __shfl_xor_sync(0xffffffffu, int(bad), step) != 0;
-  }
-  if (!write) return;
-  const float spread = high - low;
-  bad |= !(spread < INFINITY);
-  const __nv_bfloat16 scale16 = __float2bfloat16(bad ? NAN : spread / 15.0f);
-  const float scale = __bfloat162float(scale16);
-  uint32_t codes = 0;
-  if (scale > 0.0f) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float code = fminf(fmaxf(rintf((v[e] - low) / scale), 0.0f), 15.0f);
-      codes |= static_cast<uint32_t>(code) << (4 * e);
+      for (int e = 0; e < 8; ++e) codes |= divided_code(v[e], scale) << (4 * e);
     }
-  }
-  const long long row = kv4_row(p, slot, head);
-  reinterpret_cast<uint32_t*>(p.codes[which])[row * kLanes + lane] = codes;
-  if (lane % (p.group / 8) == 0) {
-    __nv_bfloat162 pair;
-    pair.x = scale16;
-    pair.y = __float2bfloat16(low);
-    p.scales[which][row * (kD / p.group) + lane * 8 / p.group] = pair;
+    if (rows.slot[i] < 0) continue;
+    if (rows.slot[i] >= p.positions) {
+      report_timeout(kSiteKv4AppendSlot);
+      continue;
+    }
+    const long long row = kv4_row(p, uint32_t(rows.slot[i]), rows.head[i]);
+    reinterpret_cast<uint32_t*>(p.codes[which])[row * kLanes + lane] = codes;
+    if ((lane & ((1 << (p.group_shift - 3)) - 1)) == 0) {
+      __nv_bfloat162 pair;
+      pair.x = scale16;
+      pair.y = __float2bfloat16(low);
+      p.scales[which][row * (kD >> p.group_shift) + (lane * 8 >> p.group_shift)] = pair;
+    }
   }
 }
 
 // The values that the codes at `slots` stand for, one rounding to the output type (the product
 // scale * code is exact in FP32).  A negative slot reads as zeros.
-template <int kD>
+template <int kD, int kBatch>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Rows p) {
   constexpr int kLanes = kD / 8;
   grid_dependents_may_launch();
   grid_dependency_wait();
-  const int which = blockIdx.y;
-  const long long index = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) / kLanes;
-  const int lane = threadIdx.x % kLanes;
-  if (index >= p.tokens * p.kv_heads) return;
-  const long long token = index / p.kv_heads;
-  const int head = int(index - token * p.kv_heads);
-  const long long slot = p.slots[token];
-  float v[8];
-  if (slot >= 0 && slot < p.positions) {
-    const long long row = kv4_row(p, slot, head);
-    const uint32_t codes = reinterpret_cast<const uint32_t*>(p.codes[which])[row * kLanes + lane];
-    const __nv_bfloat162 pair = p.scales[which][row * (kD / p.group) + lane * 8 / p.group];
-    const float scale = __bfloat162float(pair.x), zero = __bfloat162float(pair.y);
+  const int which = blockIdx.y, lane = threadIdx.x % kLanes;
+  const Kv4Batch<kLanes, kBatch> rows(p);
+  uint32_t codes[kBatch];
+  __nv_bfloat162 pair[kBatch];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = fmaf(static_cast<float>((codes >> (4 * e)) & 15u), scale, zero);
-  } else {
-    if (slot >= 0) report_timeout(kSiteKv4ReadSlot);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+  for (int i = 0; i < kBatch; ++i) {
+    codes[i] = 0;
+    pair[i] = __floats2bfloat162_rn(0.0f, 0.0f);
+    if (rows.slot[i] >= 0 && rows.slot[i] < p.positions) {
+      const long long row = kv4_row(p, uint32_t(rows.slot[i]), rows.head[i]);
+      codes[i] = reinterpret_cast<const uint32_t*>(p.codes[which])[row * kLanes + lane];
+      pair[i] = p.scales[which][row * (kD >> p.group_shift) + (lane * 8 >> p.group_shift)];
+    } else if (rows.slot[i] >= 0) {
+      report_timeout(kSiteKv4ReadSlot);
+    }
   }
-  const long long at = token * p.token_stride[which] + head * p.head_stride[which] + lane * 8;
-  if (p.out_f32) {
-    float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out[which]) + at);
-    __stcs(dst, make_float4(v[0], v[1], v[2], v[3]));
-    __stcs(dst + 1, make_float4(v[4], v[5], v[6], v[7]));
-  } else {
-    __stcs(reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out[which]) + at),
-           make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
-                      pack_bf16x2(v[6], v[7])));
+#pragma unroll
+  for (int i = 0; i < kBatch; ++i) {
+    if (!rows.live[i]) continue;
+    const float scale = __bfloat162float(pair[i].x), zero = __bfloat162float(pair[i].y);
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      // the code in the last mantissa bits of 2^23 (five of them reach without a shift)
+      constexpr float kInteger = 8388608.0f;
+      const int at = 4 * (e < 4 ? e : e - 4);
+      const uint32_t bits = ((e < 4 ? codes[i] : codes[i] >> 16) & (15u << at)) | __float_as_uint(kInteger);
+      v[e] = fmaf((__uint_as_float(bits) - kInteger) * (1.0f / (1 << at)), scale, zero);
+    }
+    const long long at = rows.offset(p, which, i) + lane * 8;
+    if (p.out_f32) {
+      float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out[which]) + at);
+      __stcs(dst, make_float4(v[0], v[1], v[2], v[3]));
+      __stcs(dst + 1, make_float4(v[4], v[5], v[6], v[7]));
+    } else {
+      __stcs(reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out[which]) + at),
+             make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                        pack_bf16x2(v[6], v[7])));
+    }
   }
 }
 
@@ -1029,9 +1093,24 @@ Kv4Rows kv4_rows(const trinity_sm100_kv4_cache& c, const trinity_sm100_kv4_rows&
   p.head_stride[1] = r.v_head_stride;
   p.kv_heads = c.kv_heads;
   p.page = c.page;
-  p.group = c.group;
+  p.group_shift = __builtin_ctz(c.group);
+  p.heads_shift = (c.kv_heads & (c.kv_heads - 1)) == 0 ? __builtin_ctz(c.kv_heads) : -1;
+  p.page_shift = (c.page & (c.page - 1)) == 0 ? __builtin_ctz(c.page) : -1;
   return p;
 }
+
+// Rows a thread takes: one while the GPU is not full of them (least latency), else four (four times the
+// bytes in flight).
+constexpr int kKv4Batch = 4;
+struct Kv4Grid {
+  int batch;
+  dim3 blocks;
+  Kv4Grid(long long tokens, const trinity_sm100_kv4_cache& c) {
+    const long long lanes = tokens * c.kv_heads * (c.head_dim / 8);
+    batch = lanes > 148 * 2048 ? kKv4Batch : 1;
+    blocks = dim3(unsigned((lanes + 256 * batch - 1) / (256 * batch)), 2);
+  }
+};
 
 int check_kv4_rows(const char* what, const trinity_sm100_kv4_cache& c, const trinity_sm100_kv4_rows& r) {
   if (int rc = check_kv4_cache(what, c)) return rc;
@@ -1085,15 +1164,18 @@ extern "C" int trinity_sm100_kv4_append(const trinity_sm100_kv4_cache* cache, co
   // 16-byte loads where every row starts on 16 bytes
   const bool vectors = aligned16(r.k) && aligned16(r.v) && r.k_token_stride % 8 == 0 && r.v_token_stride % 8 == 0 &&
                        r.k_head_stride % 8 == 0 && r.v_head_stride % 8 == 0;
-  const long long threads = r.tokens * cache->kv_heads * (cache->head_dim / 8);
-  KernelLaunch launch(dim3(unsigned((threads + 255) / 256), 2), dim3(256), 0, static_cast<cudaStream_t>(stream_handle));
+  const Kv4Grid grid(r.tokens, *cache);
+  KernelLaunch launch(grid.blocks, dim3(256), 0, static_cast<cudaStream_t>(stream_handle));
   cudaError_t e;
-  if (cache->head_dim == 128)
-    e = vectors ? cudaLaunchKernelEx(&launch.config, kv4_append_kernel<128, true>, p)
-                : cudaLaunchKernelEx(&launch.config, kv4_append_kernel<128, false>, p);
-  else
-    e = vectors ? cudaLaunchKernelEx(&launch.config, kv4_append_kernel<64, true>, p)
-                : cudaLaunchKernelEx(&launch.config, kv4_append_kernel<64, false>, p);
+#define TRINITY_KV4_APPEND(D, V) \
+  e = grid.batch == 1 ? cudaLaunchKernelEx(&launch.config, kv4_append_kernel<D, V, 1>, p) \
+                      : cudaLaunchKernelEx(&launch.config, kv4_append_kernel<D, V, kKv4Batch>, p);
+  if (cache->head_dim == 128) {
+    if (vectors) TRINITY_KV4_APPEND(128, true) else TRINITY_KV4_APPEND(128, false)
+  } else {
+    if (vectors) TRINITY_KV4_APPEND(64, true) else TRINITY_KV4_APPEND(64, false)
+  }
+#undef TRINITY_KV4_APPEND
   if (e != cudaSuccess) return fail(TRINITY_SM100_E_CUDA, "kv4_append launch: %s", cudaGetErrorString(e));
   count_launch();
   return check_launch("kv4_append");
@@ -1115,10 +1197,15 @@ extern "C" int trinity_sm100_kv4_read(const trinity_sm100_kv4_cache* cache, cons
   p.out[0] = r.k;
   p.out[1] = r.v;
   p.out_f32 = out_dtype == TRINITY_SM100_FP32;
-  const long long threads = r.tokens * cache->kv_heads * (cache->head_dim / 8);
-  KernelLaunch launch(dim3(unsigned((threads + 255) / 256), 2), dim3(256), 0, static_cast<cudaStream_t>(stream_handle));
-  cudaError_t e = cache->head_dim == 128 ? cudaLaunchKernelEx(&launch.config, kv4_read_kernel<128>, p)
-                                         : cudaLaunchKernelEx(&launch.config, kv4_read_kernel<64>, p);
+  const Kv4Grid grid(r.tokens, *cache);
+  KernelLaunch launch(grid.blocks, dim3(256), 0, static_cast<cudaStream_t>(stream_handle));
+  cudaError_t e;
+  if (cache->head_dim == 128)
+    e = grid.batch == 1 ? cudaLaunchKernelEx(&launch.config, kv4_read_kernel<128, 1>, p)
+                        : cudaLaunchKernelEx(&launch.config, kv4_read_kernel<128, kKv4Batch>, p);
+  else
+    e = grid.batch == 1 ? cudaLaunchKernelEx(&launch.config, kv4_read_kernel<64, 1>, p)
+                        : cudaLaunchKernelEx(&launch.config, kv4_read_kernel<64, kKv4Batch>, p);
   if (e != cudaSuccess) return fail(TRINITY_SM100_E_CUDA, "kv4_read launch: %s", cudaGetErrorString(e));
   count_launch();
   return check_launch("kv4_read");
