@@ -122,6 +122,38 @@ TRINITY_SM100_API int trinity_sm100_gemm_batched_bf16(const trinity_sm100_gemm* 
                                                       const trinity_sm100_gemm_batch* batch, void* stream);
 
 /*
+ * GEMM with low-rank adapters of many requests beside the weight that they share:
+ *   out[i,:] = act(a[i,:] @ b + bias + scales[z] * (a[i,:] @ down[z]) @ up[z]),   z = index[i]
+ * A negative index means no adapter; one of count or more too, and sets the device status word
+ * (0xA01).  Rows with the same adapter need not be neighbours (products are fewer if they are).
+ *
+ *   down    [count, k, rank]  bf16, row pitch ld_down, stride_down between adapters (elements)
+ *   up      [count, rank, n]  bf16, row pitch ld_up, stride_up between adapters
+ *   index   int32 [m]
+ *   scales  fp32 [count] or NULL (1)
+ *   workspace: trinity_sm100_gemm_adapters_workspace_bytes(m, n, rank) bytes, 16-byte aligned; nothing
+ *           in it needs clearing, calls that may overlap in time need one each
+ *
+ * gemm: bias mode none or column vector, any activation but the gated one; k and n multiples of 8, as are
+ * pitches and strides; rank a multiple of 8 up to 128.  Only the adapters that index names are read,
+ * and one that holds infinities or NaN reaches no rows but its own.  scales * (a @ down) and the
+ * adapter's contribution (with the bias) are rounded to BF16 once each; all sums are FP32.
+ */
+typedef struct trinity_sm100_adapters {
+  const void* down;
+  const void* up;
+  const void* index;
+  const void* scales;
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t ld_down, stride_down, ld_up, stride_up;
+  int32_t count, rank;
+} trinity_sm100_adapters;
+TRINITY_SM100_API size_t trinity_sm100_gemm_adapters_workspace_bytes(int64_t m, int64_t n, int32_t rank);
+TRINITY_SM100_API int trinity_sm100_gemm_adapters_bf16(const trinity_sm100_gemm* gemm,
+                                                       const trinity_sm100_adapters* adapters, void* stream);
+
+/*
  * RMSNorm over the last axis:
  *   y[r,c] = x[r,c] / sqrt(sum_c(x[r,c]^2) / cols + eps) * gain[c]      (FP32 math, BF16 I/O)
  * gain may be NULL (no gain) and eps may be 0, which keeps the reference's 0/0 -> NaN for an

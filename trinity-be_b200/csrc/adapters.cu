@@ -1,0 +1,430 @@
+// Low-rank adapters of many requests beside a projection that they share:
+//
+//   out[i] = act(x[i] W + bias + scale[a] (x[i] down[a]) up[a]),   a = index[i], none if negative
+//
+// Three launches of one stream:
+//   1. shrink   t[i] = scale[a] * (x[i] down[a])        [m, rank], rounded to BF16 once
+//   2. expand   delta[i] = t[i] up[a] + bias            [m, n], rounded to BF16 once
+//   3. the GEMM kernel with delta as its matrix side operand (added in FP32)
+// Both small kernels work on tiles of rows.  A tile's rows may have any adapters; the distinct ones are
+// taken in turn, each multiplied with all rows of the tile, and every row keeps only the result of
+// its own adapter (a selection, not a product with zero: an adapter that holds infinities or NaN
+// reaches its own rows only).  Sorted prompts have one or two adapters in a tile; decode batches of
+// sixteen rows sixteen at most, where the weights' bytes and not the products are what takes time.
+//
+// Rounding t and delta to BF16 costs 2^-8 of the adapter's own contribution each, as the
+// intermediates of the other chained products of this library do.
+#include "host_common.h"
+#include "sm100_ptx.cuh"
+
+namespace trinity_sm100 {
+namespace {
+
+constexpr uint32_t kSiteAdapterIndex = 0xA01;   // an index that names no adapter (the row gets none)
+constexpr int kAdapterThreads = 128;
+constexpr int kAdapterK = 128;                  // inner extent of a stage of the shrink kernel
+constexpr int kAdapterStages = 3;
+constexpr int kExpandRows = 64, kExpandCols = 128;
+
+struct AdapterParams {
+  const __nv_bfloat16* x;
+  const __nv_bfloat16* down;
+  const __nv_bfloat16* up;
+  const int* index;
+  const float* scales;         // null: 1
+  const __nv_bfloat16* bias;   // null: none
+  __nv_bfloat16* t;            // [m, padded rank]
+  __nv_bfloat16* delta;        // [m, n]
+  long long ldx, ld_down, stride_down, ld_up, stride_up;
+  int m, n, k, rank, count;
+};
+
+__device__ __forceinline__ void mma_bf16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// 16 bytes to shared memory, zeros where `valid` is false (the address is then not read).
+__device__ __forceinline__ void copy_or_zero(uint32_t dst, const void* src, bool valid) {
+  const int bytes = valid ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
+}
+
+// The adapters of a tile of kRows rows: `of_row` (-1: none) and, in `distinct`, the different ones in
+// order of their first row.  All threads of the block; returns how many there are.
+template <int kRows>
+__device__ __forceinline__ int tile_adapters(const AdapterParams& p, int row0, int* of_row, int* distinct, int* count) {
+  if (threadIdx.x == 0) *count = 0;
+  for (int i = threadIdx.x; i < kRows; i += kAdapterThreads) {
+    int a = row0 + i < p.m ? p.index[row0 + i] : -1;
+    if (a >= p.count) {
+      report_timeout(kSiteAdapterIndex);
+      a = -1;
+    }
+    of_row[i] = a < 0 ? -1 : a;
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {     // one warp: leaders are rows whose adapter no earlier row has
+    int found = 0;
+    for (int i0 = 0; i0 < kRows; i0 += 32) {
+      const int i = i0 + int(threadIdx.x);
+      bool leads = i < kRows && of_row[i < kRows ? i : 0] >= 0;
+      if (leads)
+        for (int j = 0; j < i && leads; ++j) leads = of_row[j] != of_row[i];
+      const uint32_t all = __ballot_sync(0xffffffffu, leads);
+      if (leads) distinct[found + __popc(all & ((1u << threadIdx.x) - 1))] = of_row[i];
+      found += __popc(all);
+    }
+    if (threadIdx.x == 0) *count = found;
+  }
+  __syncthreads();
+  return *count;
+}
+
+template <int kRows, int kRank>
+__host__ __device__ constexpr int shrink_stage_bytes() {
+  return (kRows * (kAdapterK + 8) + kAdapterK * (kRank + 8)) * 2;   // rows padded by 16 bytes: ldmatrix without conflicts
+}
+template <int kRows, int kRank>
+__host__ __device__ constexpr int shrink_smem_bytes() {
+  const int ring = kAdapterStages * shrink_stage_bytes<kRows, kRank>();
+  const int sums = (kRows == 16 ? kAdapterThreads / 32 : 1) * kRows * kRank * 4;
+  return (ring > sums ? ring : sums) + kRows * kRank * 4;
+}
+
+// t of kRows rows.  The inner axis is shared by the blocks of a cluster (blockIdx.x), whose sums meet in
+// distributed shared memory in a fixed order; blockIdx.y takes every gridDim.y-th adapter of the tile,
+// blockIdx.z the tile.  With 16 rows the warps share the inner axis, with 64 each has 16 rows.
+template <int kRows, int kRank>
+__global__ void __launch_bounds__(kAdapterThreads) adapter_shrink_kernel(const AdapterParams p) {
+  constexpr int kWarps = kAdapterThreads / 32;
+  constexpr int kPitchX = (kAdapterK + 8) * 2, kPitchD = (kRank + 8) * 2;
+  constexpr int kStage = shrink_stage_bytes<kRows, kRank>();
+  constexpr int kRing = shrink_smem_bytes<kRows, kRank>() - kRows * kRank * 4;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int of_row[kRows], distinct[kRows], found;
+  const uint32_t ring = smem_u32(smem);
+  float* part = reinterpret_cast<float*>(smem);               // after the products: the warps' sums
+  float* sums = reinterpret_cast<float*>(smem + kRing);       // this block's sum [kRows][kRank], read by the cluster
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row0 = blockIdx.z * kRows;
+  const uint32_t cluster = gridDim.x;
+  grid_dependency_wait();
+  grid_dependents_may_launch();
+  const int adapters = tile_adapters<kRows>(p, row0, of_row, distinct, &found);
+  const int blocks_k = (p.k + kAdapterK - 1) / kAdapterK;
+  const int begin = int(static_cast<long long>(blockIdx.x) * blocks_k / cluster);
+  const int end = int(static_cast<long long>(blockIdx.x + 1) * blocks_k / cluster);
+
+  for (int ordinal = blockIdx.y; ordinal < adapters; ordinal += gridDim.y) {
+    const int adapter = distinct[ordinal];
+    const __nv_bfloat16* down = p.down + adapter * p.stride_down;
+    auto fetch = [&](int kb) {
+      const uint32_t stage = ring + (kb - begin) % kAdapterStages * kStage;
+      const int k0 = kb * kAdapterK;
+      for (int i = threadIdx.x; i < kRows * (kAdapterK / 8); i += kAdapterThreads) {
+        const int r = i / (kAdapterK / 8), c = (i % (kAdapterK / 8)) * 8;
+        const bool valid = row0 + r < p.m && k0 + c < p.k;      // k is a multiple of 8
+        copy_or_zero(stage + r * kPitchX + c * 2, valid ? p.x + (row0 + r) * p.ldx + k0 + c : p.x, valid);
+      }
+      for (int i = threadIdx.x; i < kAdapterK * (kRank / 8); i += kAdapterThreads) {
+        const int r = i / (kRank / 8), c = (i % (kRank / 8)) * 8;
+        const bool valid = k0 + r < p.k && c < p.rank;
+        copy_or_zero(stage + kRows * kPitchX + r * kPitchD + c * 2, valid ? down + (k0 + r) * p.ld_down + c : p.down, valid);
+      }
+    };
+    float acc[kRank / 8][4];
+#pragma unroll
+    for (int j = 0; j < kRank / 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[j][e] = 0.0f;
+#pragma unroll
+    for (int s = 0; s < kAdapterStages - 1; ++s) {
+      if (begin + s < end) fetch(begin + s);
+      copies_commit();
+    }
+    for (int kb = begin; kb < end; ++kb) {
+      copies_wait<kAdapterStages - 2>();
+      __syncthreads();
+      if (kb + kAdapterStages - 1 < end) fetch(kb + kAdapterStages - 1);
+      copies_commit();
+      const uint32_t xs = ring + (kb - begin) % kAdapterStages * kStage, ds = xs + kRows * kPitchX;
+      const int first = kRows == 16 ? warp : 0, step = kRows == 16 ? kWarps : 1;
+      const int rows = kRows == 16 ? 0 : warp * 16;
+#pragma unroll
+      for (int s = 0; s < kAdapterK / 16 / (kRows == 16 ? kWarps : 1); ++s) {
+        const int k16 = (first + s * step) * 16;
+        uint32_t a[4];
+        load_matrices<false>(xs + (rows + (lane & 15)) * kPitchX + (k16 + (lane >> 4) * 8) * 2, a);
+#pragma unroll
+        for (int j = 0; j < kRank / 16; ++j) {
+          uint32_t b[4];
+          load_matrices<true>(ds + (k16 + (lane & 15)) * kPitchD + (j * 16 + (lane >> 4) * 8) * 2, b);
+          mma_bf16_16816(acc[2 * j], a, b[0], b[1]);
+          mma_bf16_16816(acc[2 * j + 1], a, b[2], b[3]);
+        }
+      }
+    }
+    copies_wait<0>();
+    __syncthreads();      // the ring is free: it holds the warps' sums now
+    {
+      float* mine = part + (kRows == 16 ? warp * 16 * kRank : warp * 16 * kRank);
+      const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+      for (int j = 0; j < kRank / 8; ++j) {
+        *reinterpret_cast<float2*>(mine + g * kRank + j * 8 + 2 * t) = make_float2(acc[j][0], acc[j][1]);
+        *reinterpret_cast<float2*>(mine + (g + 8) * kRank + j * 8 + 2 * t) = make_float2(acc[j][2], acc[j][3]);
+      }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < kRows * kRank; i += kAdapterThreads) {
+      float v = part[i];
+      if (kRows == 16)
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) v += part[w * 16 * kRank + i];
+      sums[i] = v;
+    }
+    if (cluster > 1) cluster_sync_all(); else __syncthreads();
+    const float scale = p.scales ? p.scales[adapter] : 1.0f;
+    for (int i = blockIdx.x * kAdapterThreads + threadIdx.x; i < kRows * kRank; i += cluster * kAdapterThreads) {
+      const int r = i / kRank;
+      if (of_row[r] != adapter) continue;
+      float v = 0.0f;
+      for (uint32_t c = 0; c < cluster; ++c) {
+        float other;
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(other) : "r"(map_to_peer(smem_u32(sums + i), c)));
+        v += other;
+      }
+      p.t[static_cast<long long>(row0 + r) * kRank + (i - r * kRank)] = __float2bfloat16(v * scale);
+    }
+    if (cluster > 1) cluster_sync_all(); else __syncthreads();   // sums may be written again (or the block may end)
+  }
+}
+
+template <int kRank>
+__host__ __device__ constexpr int expand_smem_bytes() {
+  return (kExpandRows * (kRank + 8) + 2 * kRank * (kExpandCols + 8)) * 2 + kExpandRows * (kExpandCols + 8) * 2;
+}
+
+// delta of 64 rows and 128 columns: warps take 32 columns each; the adapters' up weights are fetched one
+// ahead.
+template <int kRank>
+__global__ void __launch_bounds__(kAdapterThreads) adapter_expand_kernel(const AdapterParams p) {
+  constexpr int kPitchT = (kRank + 8) * 2, kPitchU = (kExpandCols + 8) * 2;
+  constexpr int kSlab = kRank * kPitchU;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int of_row[kExpandRows], distinct[kExpandRows], found;
+  const uint32_t ts = smem_u32(smem), us = ts + kExpandRows * kPitchT;
+  uint8_t* staging = smem + kExpandRows * kPitchT + 2 * kSlab;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int row0 = blockIdx.y * kExpandRows, col0 = blockIdx.x * kExpandCols;
+  const int rows = min(kExpandRows, p.m - row0);
+  grid_dependency_wait();
+  grid_dependents_may_launch();
+  const int adapters = tile_adapters<kExpandRows>(p, row0, of_row, distinct, &found);
+  auto fetch = [&](int ordinal) {
+    const __nv_bfloat16* up = p.up + distinct[ordinal] * p.stride_up;
+    const uint32_t slab = us + (ordinal & 1) * kSlab;
+    for (int i = threadIdx.x; i < kRank * (kExpandCols / 8); i += kAdapterThreads) {
+      const int r = i / (kExpandCols / 8), c = (i % (kExpandCols / 8)) * 8;
+      const bool valid = r < p.rank && col0 + c < p.n;      // n is a multiple of 8
+      copy_or_zero(slab + r * kPitchU + c * 2, valid ? up + r * p.ld_up + col0 + c : p.up, valid);
+    }
+  };
+  if (adapters) {
+    for (int i = threadIdx.x; i < kExpandRows * (kRank / 8); i += kAdapterThreads) {
+      const int r = i / (kRank / 8), c = (i % (kRank / 8)) * 8;
+      const bool valid = r < rows && of_row[r] >= 0;         // rows without an adapter have no t
+      copy_or_zero(ts + r * kPitchT + c * 2, valid ? p.t + static_cast<long long>(row0 + r) * kRank + c : p.t, valid);
+    }
+    fetch(0);
+  }
+  copies_commit();
+  float out[4][4][4];     // [16 rows][8 columns][fragment]
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) out[i][j][e] = 0.0f;
+  for (int ordinal = 0; ordinal < adapters; ++ordinal) {
+    if (ordinal + 1 < adapters) fetch(ordinal + 1);
+    copies_commit();
+    copies_wait<1>();
+    __syncthreads();
+    const uint32_t slab = us + (ordinal & 1) * kSlab;
+    const int adapter = distinct[ordinal];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i * 16 >= rows) break;
+      const bool low = of_row[i * 16 + g] == adapter, high = of_row[i * 16 + g + 8] == adapter;
+      if (!__any_sync(0xffffffffu, low || high)) continue;
+      float acc[4][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[j][e] = 0.0f;
+#pragma unroll
+      for (int k16 = 0; k16 < kRank; k16 += 16) {
+        uint32_t a[4];
+        load_matrices<false>(ts + (i * 16 + (lane & 15)) * kPitchT + (k16 + (lane >> 4) * 8) * 2, a);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          uint32_t b[4];
+          load_matrices<true>(slab + (k16 + (lane & 15)) * kPitchU + (warp * 32 + j * 16 + (lane >> 4) * 8) * 2, b);
+          mma_bf16_16816(acc[2 * j], a, b[0], b[1]);
+          mma_bf16_16816(acc[2 * j + 1], a, b[2], b[3]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (low) { out[i][j][0] = acc[j][0]; out[i][j][1] = acc[j][1]; }
+        if (high) { out[i][j][2] = acc[j][2]; out[i][j][3] = acc[j][3]; }
+      }
+    }
+    __syncthreads();      // the slab may be written again
+  }
+  copies_wait<0>();
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int col = warp * 32 + j * 8 + 2 * t;
+    float b0 = 0.0f, b1 = 0.0f;
+    if (p.bias) {
+      if (col0 + col < p.n) {
+        b0 = __bfloat162float(p.bias[col0 + col]);
+        b1 = __bfloat162float(p.bias[col0 + col + 1]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      *reinterpret_cast<uint32_t*>(staging + (i * 16 + g) * kPitchU + col * 2) = pack_bf16x2(out[i][j][0] + b0, out[i][j][1] + b1);
+      *reinterpret_cast<uint32_t*>(staging + (i * 16 + g + 8) * kPitchU + col * 2) = pack_bf16x2(out[i][j][2] + b0, out[i][j][3] + b1);
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows * (kExpandCols / 8); i += kAdapterThreads) {
+    const int r = i / (kExpandCols / 8), c = (i % (kExpandCols / 8)) * 8;
+    if (col0 + c < p.n)
+      *reinterpret_cast<uint4*>(p.delta + static_cast<long long>(row0 + r) * p.n + col0 + c) = *reinterpret_cast<const uint4*>(staging + r * kPitchU + c * 2);
+  }
+}
+
+int padded_rank(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
+size_t adapter_t_bytes(long long m, int rank) { return (size_t(m) * padded_rank(rank) * 2 + 255) / 256 * 256; }
+
+template <int kRows, int kRank>
+int launch_shrink(const AdapterParams& p, int sm_count, cudaStream_t stream) {
+  static unsigned long long opted = 0;
+  constexpr int kSmem = shrink_smem_bytes<kRows, kRank>();
+  static_assert(kSmem <= 232448 - 2048, "exceeds the 227 KB shared-memory limit");
+  auto kernel = adapter_shrink_kernel<kRows, kRank>;
+  if (int rc = opt_in_shared_memory(reinterpret_cast<const void*>(kernel), kSmem, &opted, "adapter_shrink")) return rc;
+  const int tiles = (p.m + kRows - 1) / kRows;
+  const int ordinals = min(p.count, min(kRows, 16));
+  // blocks that share the inner axis: while they find a place beside the tiles and keep two stages each
+  unsigned cluster = 1;
+  while (cluster < 8 && static_cast<long long>(tiles) * (kRows == 16 ? ordinals : 1) * cluster * 2 <= 2 * sm_count &&
+         p.k >= static_cast<long long>(cluster) * 2 * 2 * kAdapterK)
+    cluster *= 2;
+  KernelLaunch launch(dim3(cluster, ordinals, tiles), dim3(kAdapterThreads), kSmem, stream, cluster);
+  cudaError_t e = cudaLaunchKernelEx(&launch.config, kernel, p);
+  if (e != cudaSuccess) return fail(TRINITY_SM100_E_CUDA, "adapter_shrink launch: %s", cudaGetErrorString(e));
+  count_launch();
+  return check_launch("adapter_shrink");
+}
+
+template <int kRank>
+int launch_adapters(const AdapterParams& p, int sm_count, cudaStream_t stream) {
+  // tiles of 16 rows while there are few of them, of 64 rows once those fill half the SMs
+  if (int rc = p.m >= 64 * (sm_count / 2) ? launch_shrink<64, kRank>(p, sm_count, stream) : launch_shrink<16, kRank>(p, sm_count, stream))
+    return rc;
+  static unsigned long long opted = 0;
+  constexpr int kSmem = expand_smem_bytes<kRank>();
+  auto kernel = adapter_expand_kernel<kRank>;
+  if (int rc = opt_in_shared_memory(reinterpret_cast<const void*>(kernel), kSmem, &opted, "adapter_expand")) return rc;
+  KernelLaunch launch(dim3((p.n + kExpandCols - 1) / kExpandCols, (p.m + kExpandRows - 1) / kExpandRows), dim3(kAdapterThreads), kSmem, stream);
+  cudaError_t e = cudaLaunchKernelEx(&launch.config, kernel, p);
+  if (e != cudaSuccess) return fail(TRINITY_SM100_E_CUDA, "adapter_expand launch: %s", cudaGetErrorString(e));
+  count_launch();
+  return check_launch("adapter_expand");
+}
+
+}  // namespace
+}  // namespace trinity_sm100
+
+using namespace trinity_sm100;
+
+extern "C" size_t trinity_sm100_gemm_adapters_workspace_bytes(int64_t m, int64_t n, int32_t rank) {
+  if (m <= 0 || n <= 0 || rank <= 0 || rank > 128) return 0;
+  return adapter_t_bytes(m, rank) + size_t(m) * size_t(n) * 2;
+}
+
+extern "C" int trinity_sm100_gemm_adapters_bf16(const trinity_sm100_gemm* gemm, const trinity_sm100_adapters* adapters,
+                                                void* stream_handle) {
+  if (!gemm || !adapters) return fail(TRINITY_SM100_E_INVALID, "gemm_adapters: null argument block");
+  const trinity_sm100_gemm& g = *gemm;
+  const trinity_sm100_adapters& a = *adapters;
+  if (int rc = check_gemm_arguments(g)) return rc;
+  if (g.activation == TRINITY_SM100_ACT_SILU_GATE)
+    return fail(TRINITY_SM100_E_UNSUPPORTED, "gemm_adapters: the gated form takes no adapters");
+  if (g.bias_mode != TRINITY_SM100_BIAS_NONE && g.bias_mode != TRINITY_SM100_BIAS_COL_VECTOR)
+    return fail(TRINITY_SM100_E_UNSUPPORTED, "gemm_adapters: bias mode %d (a vector over the columns is supported)", g.bias_mode);
+  if (!a.down || !a.up || !a.index || !a.workspace) return fail(TRINITY_SM100_E_INVALID, "gemm_adapters: null operand");
+  if (a.count <= 0) return fail(TRINITY_SM100_E_INVALID, "gemm_adapters: no adapters");
+  if (a.rank <= 0 || a.rank % 8 || a.rank > 128)
+    return fail(TRINITY_SM100_E_UNSUPPORTED, "gemm_adapters: rank %d (multiples of 8 up to 128)", a.rank);
+  if (g.k % 8 || g.n % 8)
+    return fail(TRINITY_SM100_E_UNSUPPORTED, "gemm_adapters: k (%lld) and n (%lld) must be multiples of 8", (long long)g.k, (long long)g.n);
+  if (a.ld_down < a.rank || a.ld_up < g.n) return fail(TRINITY_SM100_E_INVALID, "gemm_adapters: leading dimension smaller than the row");
+  if (a.ld_down % 8 || a.ld_up % 8 || a.stride_down % 8 || a.stride_up % 8 || !aligned16(a.down) || !aligned16(a.up) ||
+      !aligned16(a.workspace))
+    return fail(TRINITY_SM100_E_INVALID, "gemm_adapters: adapter rows and the workspace must start on 16 bytes");
+  if (reinterpret_cast<uintptr_t>(a.index) % 4 || reinterpret_cast<uintptr_t>(a.scales) % 4)
+    return fail(TRINITY_SM100_E_INVALID, "gemm_adapters: a pointer is not aligned to its element type");
+  if (g.m > 65535ll * 16 || (g.n + kExpandCols - 1) / kExpandCols > INT32_MAX)
+    return fail(TRINITY_SM100_E_UNSUPPORTED, "gemm_adapters: too many rows (%lld)", (long long)g.m);
+  const size_t need = trinity_sm100_gemm_adapters_workspace_bytes(g.m, g.n, a.rank);
+  if (a.workspace_bytes < need)
+    return fail(TRINITY_SM100_E_INVALID, "gemm_adapters: workspace of %zu bytes, %zu needed", a.workspace_bytes, need);
+  int sm_count = 0;
+  if (int rc = require_sm100(&sm_count)) return rc;
+  AdapterParams p;
+  p.x = static_cast<const __nv_bfloat16*>(g.a);
+  p.down = static_cast<const __nv_bfloat16*>(a.down);
+  p.up = static_cast<const __nv_bfloat16*>(a.up);
+  p.index = static_cast<const int*>(a.index);
+  p.scales = static_cast<const float*>(a.scales);
+  p.bias = g.bias_mode == TRINITY_SM100_BIAS_COL_VECTOR ? static_cast<const __nv_bfloat16*>(g.bias) : nullptr;
+  p.t = static_cast<__nv_bfloat16*>(a.workspace);
+  p.delta = reinterpret_cast<__nv_bfloat16*>(static_cast<uint8_t*>(a.workspace) + adapter_t_bytes(g.m, a.rank));
+  p.ldx = g.lda;
+  p.ld_down = a.ld_down;
+  p.stride_down = a.stride_down;
+  p.ld_up = a.ld_up;
+  p.stride_up = a.stride_up;
+
+  p.m = int(g.m);
+  p.n = int(g.n);
+  p.k = int(g.k);
+  p.rank = a.rank;
+  p.count = a.count;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
+  int rc = 0;
+  switch (padded_rank(a.rank)) {
+    case 16: rc = launch_adapters<16>(p, sm_count, stream); break;
+    case 32: rc = launch_adapters<32>(p, sm_count, stream); break;
+    case 64: rc = launch_adapters<64>(p, sm_count, stream); break;
+    default: rc = launch_adapters<128>(p, sm_count, stream); break;
+  }
+  if (rc) return rc;
+  trinity_sm100_gemm with_delta = g;
+  with_delta.bias = p.delta;
+  with_delta.ld_bias = g.n;
+  with_delta.bias_mode = TRINITY_SM100_BIAS_MATRIX;
+  return trinity_sm100_gemm_bf16(&with_delta, stream_handle);
+}

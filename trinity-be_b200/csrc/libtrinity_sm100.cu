@@ -8,5 +8,6 @@
 #include "pointwise.cu"
 #include "mla_decode.cu"
 #include "kv4.cu"
+#include "adapters.cu"
 #include "allreduce.cu"
 #include "allgather.cu"

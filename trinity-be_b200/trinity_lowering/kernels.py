@@ -19,6 +19,8 @@ DT_BF16, DT_FP32 = 0, 1
 EXPORTS = (
     "trinity_sm100_gemm_bf16",
     "trinity_sm100_gemm_batched_bf16",
+    "trinity_sm100_gemm_adapters_workspace_bytes",
+    "trinity_sm100_gemm_adapters_bf16",
     "trinity_sm100_gemm_pair_capacity",
     "trinity_sm100_rmsnorm_bf16",
     "trinity_sm100_rmsnorm_residual",
@@ -78,6 +80,16 @@ class GemmArgs(ctypes.Structure):
 class GemmBatchArgs(ctypes.Structure):
     _fields_ = [("batch", ctypes.c_int64), ("stride_a", ctypes.c_int64), ("stride_b", ctypes.c_int64),
                 ("stride_out", ctypes.c_int64), ("stride_bias", ctypes.c_int64)]
+
+
+class AdaptersArgs(ctypes.Structure):
+    _fields_ = [
+        ("down", ctypes.c_void_p), ("up", ctypes.c_void_p), ("index", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+        ("ld_down", ctypes.c_int64), ("stride_down", ctypes.c_int64),
+        ("ld_up", ctypes.c_int64), ("stride_up", ctypes.c_int64),
+        ("count", ctypes.c_int32), ("rank", ctypes.c_int32),
+    ]
 
 
 class RmsnormResidualArgs(ctypes.Structure):
@@ -163,6 +175,11 @@ def library():
                     "(there is no fallback path)")
             lib = ctypes.CDLL(str(_LIB_PATH))
             lib.trinity_sm100_gemm_bf16.argtypes = [ctypes.POINTER(GemmArgs), ctypes.c_void_p]
+            lib.trinity_sm100_gemm_adapters_workspace_bytes.argtypes = [
+                ctypes.c_int64, ctypes.c_int64, ctypes.c_int32]
+            lib.trinity_sm100_gemm_adapters_workspace_bytes.restype = ctypes.c_size_t
+            lib.trinity_sm100_gemm_adapters_bf16.argtypes = [
+                ctypes.POINTER(GemmArgs), ctypes.POINTER(AdaptersArgs), ctypes.c_void_p]
             lib.trinity_sm100_rmsnorm_bf16.argtypes = [
                 ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
                 ctypes.c_float, ctypes.c_void_p]
@@ -374,6 +391,69 @@ def gemm_batched(a, b, *, bias=None, activation=ACT_NONE, out=None, out_dtype=to
     with torch.cuda.device(a.device):
         _check(library().trinity_sm100_gemm_batched_bf16(ctypes.byref(args), ctypes.byref(how), _stream(stream)))
     return out
+
+
+def gemm_adapters_workspace_bytes(m, n, rank):
+    """Bytes of workspace that ``gemm_adapters`` needs."""
+    return int(library().trinity_sm100_gemm_adapters_workspace_bytes(m, n, rank))
+
+
+def gemm_adapters(x, w, down, up, index, *, scales=None, bias=None, activation=ACT_NONE, out=None,
+                  out_dtype=torch.bfloat16, workspace=None, stream=None):
+    """out[i] = act(x[i] @ w + bias + scales[z] * (x[i] @ down[z]) @ up[z]) with z = index[i] (negative: no
+    adapter); see ``trinity_sm100_gemm_adapters_bf16``.
+
+    ``x`` [m, k] and ``w`` [k, n] as in ``gemm``; ``down`` [adapters, k, rank] and ``up``
+    [adapters, rank, n] BF16 with a unit inner stride, ``index`` int32 [m], ``scales`` FP32 [adapters],
+    ``bias`` BF16 [n].  ``workspace`` (uint8, ``gemm_adapters_workspace_bytes``) is allocated per call
+    unless given; calls that may overlap need one each."""
+    for name, t in (("x", x), ("w", w), ("down", down), ("up", up)):
+        _require(t, torch.bfloat16, name)
+    _require(index, torch.int32, "index")
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[0] or not _rows_ok(x) or not _rows_ok(w):
+        raise ValueError("gemm_adapters: x must be [m,k] and w [k,n], row-major with unit inner strides")
+    m, k = x.shape
+    n = w.shape[1]
+    if (down.dim() != 3 or up.dim() != 3 or down.shape[0] != up.shape[0] or down.shape[1] != k
+            or up.shape[2] != n or down.shape[2] != up.shape[1] or down.stride(2) != 1 or up.stride(2) != 1):
+        raise ValueError("gemm_adapters: down must be [adapters,k,rank] and up [adapters,rank,n], unit inner strides")
+    count, _, rank = down.shape
+    if tuple(index.shape) != (m,) or not index.is_contiguous():
+        raise ValueError("gemm_adapters: index must be [m]")
+    if scales is not None:
+        _require(scales, torch.float32, "scales")
+        if tuple(scales.shape) != (count,) or not scales.is_contiguous():
+            raise ValueError("gemm_adapters: scales must be [adapters]")
+    if bias is not None:
+        _require(bias, torch.bfloat16, "bias")
+        if tuple(bias.shape) != (n,) or not bias.is_contiguous():
+            raise ValueError("gemm_adapters: bias must be [n]")
+    if out is not None:
+        out_dtype = out.dtype
+        if tuple(out.shape) != (m, n) or not _rows_ok(out):
+            raise ValueError("gemm_adapters: out must be a row-major [m,n] tensor")
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("gemm_adapters: out dtype must be bf16 or fp32")
+    device = x.device
+    _same_device(device, w=w, down=down, up=up, index=index, scales=scales, bias=bias, out=out, workspace=workspace)
+
+    def launch(handle):
+        o = torch.empty((m, n), dtype=out_dtype, device=device) if out is None else out
+        room = workspace
+        if room is None:
+            room = torch.empty(gemm_adapters_workspace_bytes(m, n, rank), dtype=torch.uint8, device=device)
+        args = GemmArgs(x.data_ptr(), w.data_ptr(), None, bias.data_ptr() if bias is not None else None, o.data_ptr(),
+                        m, n, k, _pitch(x), _pitch(w), _pitch(o), 0,
+                        BIAS_NONE if bias is None else BIAS_COL_VECTOR, activation,
+                        DT_FP32 if out_dtype == torch.float32 else DT_BF16, 0)
+        adapters = AdaptersArgs(down.data_ptr(), up.data_ptr(), index.data_ptr(),
+                                scales.data_ptr() if scales is not None else None, room.data_ptr(),
+                                room.numel() * room.element_size(), down.stride(1), down.stride(0),
+                                up.stride(1), up.stride(0), count, rank)
+        _check(library().trinity_sm100_gemm_adapters_bf16(ctypes.byref(args), ctypes.byref(adapters), handle))
+        return o
+
+    return _submit(device, stream, (x, w, down, up, index, scales, bias, out, workspace), launch)
 
 
 def rmsnorm(x, gain=None, eps=0.0, out=None, stream=None):
