@@ -167,6 +167,8 @@ def library_path():
 def library():
     """Loads the kernel library once; raises if it has not been built."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is None:
             if not _LIB_PATH.exists():
@@ -245,8 +247,9 @@ def _submit(device, stream, operands, launch):
     results here, so neither is handed out again too early; ordering the two streams is left to
     the caller, as with every torch operation."""
     if stream is None:
-        if device.index == torch.cuda.current_device():
-            return launch(torch.cuda.current_stream().cuda_stream)
+        index = device.index
+        if index == torch._C._cuda_getDevice():     # the common case, a few hundred nanoseconds
+            return launch(torch._C._cuda_getCurrentRawStream(index))
         with torch.cuda.device(device):
             return launch(torch.cuda.current_stream().cuda_stream)
     if stream.device != device:
@@ -266,10 +269,10 @@ def _submit(device, stream, operands, launch):
         return result
 
 
-def _same_device(device, **operands):
-    for name, t in operands.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, the other operands on {device}")
+def _operand(t, dtype, index, name):
+    """Checks the type of an operand and that it lies on CUDA device ``index``."""
+    if t.dtype != dtype or t.get_device() != index or index < 0:
+        raise ValueError(f"{name}: expected a tensor of {dtype} on cuda:{max(index, 0)}, got {t.device} {t.dtype}")
 
 
 def _rows_ok(t):
@@ -282,10 +285,19 @@ def _pitch(t):
     return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
 
 
-def _dtype_code(t, name):
-    if not t.is_cuda or t.dtype not in (torch.bfloat16, torch.float32):
-        raise ValueError(f"{name}: expected a CUDA tensor of bf16 or fp32, got {t.device} {t.dtype}")
-    return DT_FP32 if t.dtype == torch.float32 else DT_BF16
+def _empty_rows(like, dtype):
+    """An uninitialised contiguous tensor of ``like``'s shape (empty_like is the cheaper call)."""
+    if like.dtype is dtype and like.is_contiguous():
+        return torch.empty_like(like)
+    return torch.empty(like.shape, dtype=dtype, device=like.device)
+
+
+def _real_operand(t, index, name):
+    """``_operand`` for either of BF16 and FP32; the type's code."""
+    dtype = t.dtype
+    if dtype is not torch.bfloat16 and dtype is not torch.float32 or t.get_device() != index or index < 0:
+        raise ValueError(f"{name}: expected a tensor of bf16 or fp32 on cuda:{max(index, 0)}, got {t.device} {dtype}")
+    return DT_FP32 if dtype is torch.float32 else DT_BF16
 
 
 def launch_count():
@@ -407,9 +419,11 @@ def gemm_adapters(x, w, down, up, index, *, scales=None, bias=None, activation=A
     [adapters, rank, n] BF16 with a unit inner stride, ``index`` int32 [m], ``scales`` FP32 [adapters],
     ``bias`` BF16 [n].  ``workspace`` (uint8, ``gemm_adapters_workspace_bytes``) is allocated per call
     unless given; calls that may overlap need one each."""
+    device = x.device
+    at = x.get_device()
     for name, t in (("x", x), ("w", w), ("down", down), ("up", up)):
-        _require(t, torch.bfloat16, name)
-    _require(index, torch.int32, "index")
+        _operand(t, torch.bfloat16, at, name)
+    _operand(index, torch.int32, at, "index")
     if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[0] or not _rows_ok(x) or not _rows_ok(w):
         raise ValueError("gemm_adapters: x must be [m,k] and w [k,n], row-major with unit inner strides")
     m, k = x.shape
@@ -421,21 +435,21 @@ def gemm_adapters(x, w, down, up, index, *, scales=None, bias=None, activation=A
     if tuple(index.shape) != (m,) or not index.is_contiguous():
         raise ValueError("gemm_adapters: index must be [m]")
     if scales is not None:
-        _require(scales, torch.float32, "scales")
+        _operand(scales, torch.float32, at, "scales")
         if tuple(scales.shape) != (count,) or not scales.is_contiguous():
             raise ValueError("gemm_adapters: scales must be [adapters]")
     if bias is not None:
-        _require(bias, torch.bfloat16, "bias")
+        _operand(bias, torch.bfloat16, at, "bias")
         if tuple(bias.shape) != (n,) or not bias.is_contiguous():
             raise ValueError("gemm_adapters: bias must be [n]")
     if out is not None:
         out_dtype = out.dtype
-        if tuple(out.shape) != (m, n) or not _rows_ok(out):
+        if tuple(out.shape) != (m, n) or not _rows_ok(out) or out.get_device() != at:
             raise ValueError("gemm_adapters: out must be a row-major [m,n] tensor")
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise ValueError("gemm_adapters: out dtype must be bf16 or fp32")
-    device = x.device
-    _same_device(device, w=w, down=down, up=up, index=index, scales=scales, bias=bias, out=out, workspace=workspace)
+    if workspace is not None and workspace.get_device() != at:
+        raise ValueError("gemm_adapters: the workspace is on another device")
 
     def launch(handle):
         o = torch.empty((m, n), dtype=out_dtype, device=device) if out is None else out
@@ -483,28 +497,31 @@ def rmsnorm_residual(x, residual, *, gain=None, post_gain=None, post_norm=None, 
     ``x`` and ``residual`` are [rows, cols], BF16 or FP32, with a unit inner stride; ``h`` has the
     residual's type, ``y`` is BF16.  ``gate`` is a BF16 tensor that broadcasts to [rows, cols]:
     [cols], [1, cols], [rows, 1] or [rows, cols].  ``residual_out=residual`` updates the stream in place."""
-    x_dtype = _dtype_code(x, "x")
-    residual_dtype = _dtype_code(residual, "residual")
-    if residual.shape != x.shape or not _rows_ok(x) or not _rows_ok(residual):
-        raise ValueError("rmsnorm_residual: x and residual must be [rows, cols] with a unit inner stride")
-    rows, cols = x.shape
     device = x.device
+    index = x.get_device()
+    x_dtype = _real_operand(x, index, "x")
+    residual_dtype = _real_operand(residual, index, "residual")
+    shape = x.shape
+    if residual.shape != shape or not _rows_ok(x) or not _rows_ok(residual):
+        raise ValueError("rmsnorm_residual: x and residual must be [rows, cols] with a unit inner stride")
+    rows, cols = shape
     for name, t in (("gain", gain), ("post_gain", post_gain)):
         if t is not None:
-            _require(t, torch.bfloat16, name)
-            if tuple(t.shape) != (cols,) or not t.is_contiguous():
+            _operand(t, torch.bfloat16, index, name)
+            if t.shape != (cols,) or not t.is_contiguous():
                 raise ValueError(f"rmsnorm_residual: {name} must be [cols]")
     if post_norm is None:
         post_norm = post_gain is not None
     elif not post_norm and post_gain is not None:
         raise ValueError("rmsnorm_residual: post_gain without the post norm")
-    args = RmsnormResidualArgs()
+    gate_pointer, row_stride, col_stride = None, 0, 0
     if gate is not None:
-        _require(gate, torch.bfloat16, "gate")
-        try:
-            gate = gate.expand(rows, cols)
-        except RuntimeError:
-            raise ValueError(f"rmsnorm_residual: gate {tuple(gate.shape)} does not broadcast to {(rows, cols)}") from None
+        _operand(gate, torch.bfloat16, index, "gate")
+        if gate.shape != shape:
+            try:
+                gate = gate.expand(rows, cols)
+            except RuntimeError:
+                raise ValueError(f"rmsnorm_residual: gate {tuple(gate.shape)} does not broadcast to {(rows, cols)}") from None
         row_stride, col_stride = gate.stride()
         if cols == 1:
             col_stride = 0
@@ -512,29 +529,21 @@ def rmsnorm_residual(x, residual, *, gain=None, post_gain=None, post_norm=None, 
             row_stride = 0
         if col_stride not in (0, 1):
             raise ValueError("rmsnorm_residual: gate must have an inner stride of 0 or 1")
-        args.gate, args.gate_row_stride, args.gate_col_stride = gate.data_ptr(), row_stride, col_stride
+        gate_pointer = gate.data_ptr()
     for name, t, dtype in (("residual_out", residual_out, residual.dtype), ("out", out, torch.bfloat16)):
         if t is not None:
-            _require(t, dtype, name)
-            if t.shape != x.shape or not _rows_ok(t):
+            _operand(t, dtype, index, name)
+            if t.shape != shape or not _rows_ok(t):
                 raise ValueError(f"rmsnorm_residual: {name} must be [rows, cols] with a unit inner stride")
-    _same_device(device, residual=residual, gain=gain, post_gain=post_gain, gate=gate, residual_out=residual_out,
-                 out=out)
-    args.x, args.residual = x.data_ptr(), residual.data_ptr()
-    args.gain = gain.data_ptr() if gain is not None else None
-    args.post_gain = post_gain.data_ptr() if post_gain is not None else None
-    args.rows, args.cols = rows, cols
-    args.ld_x, args.ld_residual = _pitch(x), _pitch(residual)
-    args.x_dtype, args.residual_dtype = x_dtype, residual_dtype
-    args.post_norm = int(post_norm)
-    args.eps, args.post_eps = eps, eps if post_eps is None else post_eps
-    args.residual_scale = residual_scale
 
     def launch(handle):
-        h = torch.empty((rows, cols), dtype=residual.dtype, device=device) if residual_out is None else residual_out
-        y = torch.empty((rows, cols), dtype=torch.bfloat16, device=device) if out is None else out
-        args.residual_out, args.out = h.data_ptr(), y.data_ptr()
-        args.ld_residual_out, args.ld_out = _pitch(h), _pitch(y)
+        h = _empty_rows(residual, residual.dtype) if residual_out is None else residual_out
+        y = _empty_rows(x, torch.bfloat16) if out is None else out
+        args = RmsnormResidualArgs(
+            x.data_ptr(), residual.data_ptr(), gate_pointer, None if gain is None else gain.data_ptr(),
+            None if post_gain is None else post_gain.data_ptr(), h.data_ptr(), y.data_ptr(), rows, cols,
+            _pitch(x), _pitch(residual), _pitch(h), _pitch(y), row_stride, col_stride, x_dtype, residual_dtype,
+            bool(post_norm), eps, eps if post_eps is None else post_eps, residual_scale)
         _check(library().trinity_sm100_rmsnorm_residual(ctypes.byref(args), handle))
         return h, y
 
@@ -636,15 +645,16 @@ class Kv4Cache:
         if (k_scales.shape[:3] != k_codes.shape[:3] or v_codes.shape != k_codes.shape
                 or v_scales.shape != k_scales.shape or groups == 0 or (2 * half) % groups):
             raise ValueError("Kv4Cache: codes and scales disagree")
+        index = k_codes.get_device()
         for name, t, dtype in (("k_codes", k_codes, torch.uint8), ("v_codes", v_codes, torch.uint8),
                                ("k_scales", k_scales, torch.bfloat16), ("v_scales", v_scales, torch.bfloat16)):
-            _require(t, dtype, name)
-            if not t.is_contiguous() or t.device != k_codes.device:
-                raise ValueError(f"Kv4Cache: {name} must be contiguous and on {k_codes.device}")
+            _operand(t, dtype, index, name)
+            if not t.is_contiguous():
+                raise ValueError(f"Kv4Cache: {name} must be contiguous")
         self.k_codes, self.k_scales, self.v_codes, self.v_scales = k_codes, k_scales, v_codes, v_scales
         self.pages, self.kv_heads, self.page = pages, kv_heads, page
         self.head_dim, self.group = 2 * half, 2 * half // groups
-        self.device = k_codes.device
+        self.device, self.index = k_codes.device, index
         self.args = Kv4CacheArgs(k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(),
                                  pages, kv_heads, page, self.head_dim, self.group, 0)
 
@@ -666,24 +676,24 @@ def kv4_cache(pages, kv_heads, page, head_dim, group=None, device="cuda"):
 
 
 def _kv4_rows(what, cache, k, v, slots):
-    expected = (slots.shape[0] if slots.dim() == 1 else -1, cache.kv_heads, cache.head_dim)
-    if tuple(k.shape) != expected or tuple(v.shape) != expected or k.stride(2) != 1 or v.stride(2) != 1:
+    tokens = slots.shape[0] if slots.dim() == 1 else -1
+    expected = (tokens, cache.kv_heads, cache.head_dim)
+    ks, vs = k.stride(), v.stride()
+    if k.shape != expected or v.shape != expected or ks[2] != 1 or vs[2] != 1:
         raise ValueError(f"{what}: k and v must be [tokens, {cache.kv_heads}, {cache.head_dim}] with a unit inner "
                          "stride and slots [tokens]")
-    _require(slots, torch.int64, "slots")
+    _operand(slots, torch.int64, cache.index, "slots")
     if not slots.is_contiguous():
         raise ValueError(f"{what}: slots must be contiguous")
-    _same_device(cache.device, k=k, v=v, slots=slots)
-    return Kv4RowsArgs(k.data_ptr(), v.data_ptr(), slots.data_ptr(), expected[0], k.stride(0), k.stride(1),
-                       v.stride(0), v.stride(1))
+    return Kv4RowsArgs(k.data_ptr(), v.data_ptr(), slots.data_ptr(), tokens, ks[0], ks[1], vs[0], vs[1])
 
 
 def kv4_append(cache, k, v, slots, stream=None):
     """Quantises the BF16 rows ``k`` and ``v`` [tokens, kv_heads, head_dim] (views with any token and
     head stride) into ``cache`` at positions ``slots`` (int64 [tokens]; distinct; negative: token not
     written); see ``trinity_sm100_kv4_append``."""
-    _require(k, torch.bfloat16, "k")
-    _require(v, torch.bfloat16, "v")
+    _operand(k, torch.bfloat16, cache.index, "k")
+    _operand(v, torch.bfloat16, cache.index, "v")
     args = _kv4_rows("kv4_append", cache, k, v, slots)
 
     def launch(handle):
@@ -699,8 +709,8 @@ def kv4_read(cache, slots, *, dtype=torch.bfloat16, k_out=None, v_out=None, stre
         raise ValueError("kv4_read: give both outputs or none")
     if k_out is not None:
         dtype = k_out.dtype
-        if v_out.dtype != dtype:
-            raise ValueError("kv4_read: the outputs differ in type")
+        _operand(k_out, dtype, cache.index, "k_out")
+        _operand(v_out, dtype, cache.index, "v_out")
     if dtype not in (torch.bfloat16, torch.float32):
         raise ValueError("kv4_read: dtype must be bf16 or fp32")
     code = DT_FP32 if dtype == torch.float32 else DT_BF16
@@ -710,7 +720,8 @@ def kv4_read(cache, slots, *, dtype=torch.bfloat16, k_out=None, v_out=None, stre
             shape = (slots.shape[0] if slots.dim() == 1 else -1, cache.kv_heads, cache.head_dim)
             if shape[0] < 0:
                 raise ValueError("kv4_read: slots must be [tokens]")
-            k, v = (torch.empty(shape, dtype=dtype, device=cache.device) for _ in range(2))
+            k = torch.empty(shape, dtype=dtype, device=cache.device)
+            v = torch.empty_like(k)
         else:
             k, v = k_out, v_out
         args = _kv4_rows("kv4_read", cache, k, v, slots)
@@ -734,28 +745,29 @@ def kv4_decode(q, cache, page_table, lengths, scale, *, out=None, lse=None, work
     ``lengths`` int32 [batch] on the device.  ``lse`` (FP32 [batch, heads]) receives the logarithm of
     the sum of exponentials.  ``workspace`` (uint8, ``kv4_decode_workspace_bytes``) is allocated per
     call unless given; calls that may overlap need one each."""
-    _require(q, torch.bfloat16, "q")
-    _require(page_table, torch.int32, "page_table")
-    _require(lengths, torch.int32, "lengths")
-    device = cache.device
+    device, index = cache.device, cache.index
+    _operand(q, torch.bfloat16, index, "q")
+    _operand(page_table, torch.int32, index, "page_table")
+    _operand(lengths, torch.int32, index, "lengths")
     if q.dim() != 3 or q.shape[2] != cache.head_dim or q.stride(2) != 1:
         raise ValueError(f"kv4_decode: q must be [batch, heads, {cache.head_dim}] with a unit inner stride")
     batch, heads, head_dim = q.shape
-    if (page_table.dim() != 2 or page_table.shape[0] != batch or page_table.stride(1) != 1 and page_table.shape[1] != 1
-            or tuple(lengths.shape) != (batch,) or not lengths.is_contiguous()):
+    if (not _rows_ok(page_table) or page_table.shape[0] != batch or lengths.shape != (batch,)
+            or not lengths.is_contiguous()):
         raise ValueError("kv4_decode: page_table must be [batch, max_pages] and lengths [batch]")
     if out is not None:
-        _require(out, torch.bfloat16, "out")
+        _operand(out, torch.bfloat16, index, "out")
         if out.shape != q.shape or not out.is_contiguous():
             raise ValueError("kv4_decode: out must be a contiguous [batch, heads, head_dim] tensor")
     if lse is not None:
-        _require(lse, torch.float32, "lse")
-        if tuple(lse.shape) != (batch, heads) or not lse.is_contiguous():
+        _operand(lse, torch.float32, index, "lse")
+        if lse.shape != (batch, heads) or not lse.is_contiguous():
             raise ValueError("kv4_decode: lse must be a contiguous [batch, heads] tensor")
-    _same_device(device, q=q, page_table=page_table, lengths=lengths, out=out, lse=lse, workspace=workspace)
+    if workspace is not None and workspace.get_device() != index:
+        raise ValueError("kv4_decode: the workspace is on another device")
 
     def launch(handle):
-        o = torch.empty((batch, heads, head_dim), dtype=torch.bfloat16, device=device) if out is None else out
+        o = _empty_rows(q, torch.bfloat16) if out is None else out
         room = workspace
         if room is None:
             room = torch.empty(kv4_decode_workspace_bytes(heads, cache.kv_heads, head_dim), dtype=torch.uint8,
