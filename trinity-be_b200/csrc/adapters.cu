@@ -23,7 +23,6 @@ namespace {
 constexpr uint32_t kSiteAdapterIndex = 0xA01;   // an index that names no adapter (the row gets none)
 constexpr int kAdapterThreads = 128;
 constexpr int kAdapterK = 128;                  // inner extent of a stage of the shrink kernel
-constexpr int kAdapterStages = 3;
 constexpr int kExpandRows = 64, kExpandCols = 128;
 
 struct AdapterParams {
@@ -44,41 +43,35 @@ __device__ __forceinline__ void mma_bf16_16816(float (&d)[4], const uint32_t (&a
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// 16 bytes to shared memory, zeros where `valid` is false (the address is then not read).
-__device__ __forceinline__ void copy_or_zero(uint32_t dst, const void* src, bool valid) {
-  const int bytes = valid ? 16 : 0;
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int kPending>
-__device__ __forceinline__ void copies_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
+// Byte offset `at` of a tile that TMA laid down with rows of `row_bytes` (32, 64 or 128) in the swizzle of
+// that width, from a base on 1024 bytes: 16-byte chunks move so that eight rows of one column of
+// chunks, which is what ldmatrix reads, lie in distinct banks.
+__device__ __forceinline__ uint32_t swizzled(uint32_t at, int row_bytes) {
+  return at ^ (((at >> 7) & uint32_t(row_bytes / 16 - 1)) << 4);
 }
 
 // The adapters of a tile of kRows rows: `of_row` (-1: none) and, in `distinct`, the different ones in
 // order of their first row.  All threads of the block; returns how many there are.
 template <int kRows>
 __device__ __forceinline__ int tile_adapters(const AdapterParams& p, int row0, int* of_row, int* distinct, int* count) {
-  if (threadIdx.x == 0) *count = 0;
-  for (int i = threadIdx.x; i < kRows; i += kAdapterThreads) {
-    int a = row0 + i < p.m ? p.index[row0 + i] : -1;
-    if (a >= p.count) {
-      report_timeout(kSiteAdapterIndex);
-      a = -1;
-    }
-    of_row[i] = a < 0 ? -1 : a;
-  }
-  __syncthreads();
-  if (threadIdx.x < 32) {     // one warp: leaders are rows whose adapter no earlier row has
+  if (threadIdx.x < 32) {
     int found = 0;
     for (int i0 = 0; i0 < kRows; i0 += 32) {
       const int i = i0 + int(threadIdx.x);
-      bool leads = i < kRows && of_row[i < kRows ? i : 0] >= 0;
-      if (leads)
-        for (int j = 0; j < i && leads; ++j) leads = of_row[j] != of_row[i];
+      int a = i < kRows && row0 + i < p.m ? p.index[row0 + i] : -1;
+      if (a >= p.count) {
+        report_timeout(kSiteAdapterIndex);
+        a = -1;
+      }
+      a = a < 0 ? -1 : a;
+      if (i < kRows) of_row[i] = a;
+      const uint32_t same = __match_any_sync(0xffffffffu, a);         // (every lane takes part)
+      bool leads = a >= 0 && (same & ((1u << threadIdx.x) - 1)) == 0;
+      for (int j = 0; j < found; ++j) leads &= distinct[j] != a;      // those of the 32 rows before
       const uint32_t all = __ballot_sync(0xffffffffu, leads);
-      if (leads) distinct[found + __popc(all & ((1u << threadIdx.x) - 1))] = of_row[i];
+      if (leads) distinct[found + __popc(all & ((1u << threadIdx.x) - 1))] = a;
       found += __popc(all);
+      __syncwarp();
     }
     if (threadIdx.x == 0) *count = found;
   }
@@ -88,92 +81,105 @@ __device__ __forceinline__ int tile_adapters(const AdapterParams& p, int row0, i
 
 template <int kRows, int kRank>
 __host__ __device__ constexpr int shrink_stage_bytes() {
-  return (kRows * (kAdapterK + 8) + kAdapterK * (kRank + 8)) * 2;   // rows padded by 16 bytes: ldmatrix without conflicts
+  return (kRows + kRank) * kAdapterK * 2;
+}
+template <int kRows, int kRank>
+__host__ __device__ constexpr int shrink_stages() {
+  const int fit = 96 * 1024 / shrink_stage_bytes<kRows, kRank>();
+  return fit > 8 ? 8 : fit < 3 ? 3 : fit;
 }
 template <int kRows, int kRank>
 __host__ __device__ constexpr int shrink_smem_bytes() {
-  const int ring = kAdapterStages * shrink_stage_bytes<kRows, kRank>();
+  const int ring = shrink_stages<kRows, kRank>() * shrink_stage_bytes<kRows, kRank>();
   const int sums = (kRows == 16 ? kAdapterThreads / 32 : 1) * kRows * kRank * 4;
-  return (ring > sums ? ring : sums) + kRows * kRank * 4;
+  return 1024 + (ring > sums ? ring : sums) + kRows * kRank * 4;
 }
 
 // t of kRows rows.  The inner axis is shared by the blocks of a cluster (blockIdx.x), whose sums meet in
 // distributed shared memory in a fixed order; blockIdx.y takes every gridDim.y-th adapter of the tile,
-// blockIdx.z the tile.  With 16 rows the warps share the inner axis, with 64 each has 16 rows.
+// blockIdx.z the tile.  With 16 rows the warps share the inner axis, with 64 each has 16 rows.  One
+// thread keeps a ring of TMA tiles filled (x in boxes of 64 columns, down in boxes of at most 64).
 template <int kRows, int kRank>
-__global__ void __launch_bounds__(kAdapterThreads) adapter_shrink_kernel(const AdapterParams p) {
+__global__ void __launch_bounds__(kAdapterThreads)
+adapter_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_down,
+                      const AdapterParams p) {
   constexpr int kWarps = kAdapterThreads / 32;
-  constexpr int kPitchX = (kAdapterK + 8) * 2, kPitchD = (kRank + 8) * 2;
+  constexpr int kStages = shrink_stages<kRows, kRank>();
   constexpr int kStage = shrink_stage_bytes<kRows, kRank>();
-  constexpr int kRing = shrink_smem_bytes<kRows, kRank>() - kRows * kRank * 4;
-  extern __shared__ __align__(128) uint8_t smem[];
+  constexpr int kRowD = kRank < 64 ? kRank * 2 : 128;         // bytes of a row of a box of down
+  constexpr int kRing = shrink_smem_bytes<kRows, kRank>() - 1024 - kRows * kRank * 4;
+  extern __shared__ uint8_t smem_raw[];
   __shared__ int of_row[kRows], distinct[kRows], found;
-  const uint32_t ring = smem_u32(smem);
+  __shared__ __align__(8) uint64_t full[kStages];
+  const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (ring - smem_u32(smem_raw));
   float* part = reinterpret_cast<float*>(smem);               // after the products: the warps' sums
   float* sums = reinterpret_cast<float*>(smem + kRing);       // this block's sum [kRows][kRank], read by the cluster
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int row0 = blockIdx.z * kRows;
   const uint32_t cluster = gridDim.x;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) mbar_init(smem_u32(full + s), 1);
+    mbar_fence_init();
+    tma_prefetch_desc(&map_x);
+    tma_prefetch_desc(&map_down);
+  }
   grid_dependency_wait();
   grid_dependents_may_launch();
   const int adapters = tile_adapters<kRows>(p, row0, of_row, distinct, &found);
   const int blocks_k = (p.k + kAdapterK - 1) / kAdapterK;
   const int begin = int(static_cast<long long>(blockIdx.x) * blocks_k / cluster);
   const int end = int(static_cast<long long>(blockIdx.x + 1) * blocks_k / cluster);
+  uint32_t issued = 0, taken = 0;      // tiles, over all adapters of this block
+  bool ok = true;
 
   for (int ordinal = blockIdx.y; ordinal < adapters; ordinal += gridDim.y) {
     const int adapter = distinct[ordinal];
-    const __nv_bfloat16* down = p.down + adapter * p.stride_down;
-    auto fetch = [&](int kb) {
-      const uint32_t stage = ring + (kb - begin) % kAdapterStages * kStage;
-      const int k0 = kb * kAdapterK;
-      for (int i = threadIdx.x; i < kRows * (kAdapterK / 8); i += kAdapterThreads) {
-        const int r = i / (kAdapterK / 8), c = (i % (kAdapterK / 8)) * 8;
-        const bool valid = row0 + r < p.m && k0 + c < p.k;      // k is a multiple of 8
-        copy_or_zero(stage + r * kPitchX + c * 2, valid ? p.x + (row0 + r) * p.ldx + k0 + c : p.x, valid);
-      }
-      for (int i = threadIdx.x; i < kAdapterK * (kRank / 8); i += kAdapterThreads) {
-        const int r = i / (kRank / 8), c = (i % (kRank / 8)) * 8;
-        const bool valid = k0 + r < p.k && c < p.rank;
-        copy_or_zero(stage + kRows * kPitchX + r * kPitchD + c * 2, valid ? down + (k0 + r) * p.ld_down + c : p.down, valid);
-      }
+    auto fetch = [&](int kb) {         // one thread
+      const uint32_t s = issued % kStages, bar = smem_u32(full + s), stage = ring + s * kStage;
+      mbar_arrive_expect_tx(bar, kStage);
+#pragma unroll
+      for (int c = 0; c < kAdapterK / 64; ++c)
+        tma_load_2d(stage + c * kRows * 128, &map_x, bar, kb * kAdapterK + c * 64, row0);
+#pragma unroll
+      for (int c = 0; c < (kRank + 63) / 64; ++c)
+        tma_load_3d(stage + kRows * kAdapterK * 2 + c * kAdapterK * 128, &map_down, bar, c * 64, kb * kAdapterK, adapter);
+      ++issued;
     };
     float acc[kRank / 8][4];
 #pragma unroll
     for (int j = 0; j < kRank / 8; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[j][e] = 0.0f;
-#pragma unroll
-    for (int s = 0; s < kAdapterStages - 1; ++s) {
-      if (begin + s < end) fetch(begin + s);
-      copies_commit();
-    }
-    for (int kb = begin; kb < end; ++kb) {
-      copies_wait<kAdapterStages - 2>();
-      __syncthreads();
-      if (kb + kAdapterStages - 1 < end) fetch(kb + kAdapterStages - 1);
-      copies_commit();
-      const uint32_t xs = ring + (kb - begin) % kAdapterStages * kStage, ds = xs + kRows * kPitchX;
+    if (threadIdx.x == 0)
+      for (int kb = begin; kb < end && kb < begin + kStages - 1; ++kb) fetch(kb);
+    for (int kb = begin; kb < end; ++kb, ++taken) {
+      const uint32_t s = taken % kStages;
+      if (ok) ok = mbar_wait(smem_u32(full + s), (taken / kStages) & 1u, 0xA11);
+      __syncthreads();                 // everyone is through with the tile before, whose stage is filled again
+      if (threadIdx.x == 0 && kb + kStages - 1 < end) fetch(kb + kStages - 1);
+      const uint32_t xs = ring + s * kStage, ds = xs + kRows * kAdapterK * 2;
       const int first = kRows == 16 ? warp : 0, step = kRows == 16 ? kWarps : 1;
       const int rows = kRows == 16 ? 0 : warp * 16;
 #pragma unroll
-      for (int s = 0; s < kAdapterK / 16 / (kRows == 16 ? kWarps : 1); ++s) {
-        const int k16 = (first + s * step) * 16;
+      for (int i = 0; i < kAdapterK / 16 / (kRows == 16 ? kWarps : 1); ++i) {
+        const int k16 = (first + i * step) * 16;
         uint32_t a[4];
-        load_matrices<false>(xs + (rows + (lane & 15)) * kPitchX + (k16 + (lane >> 4) * 8) * 2, a);
+        load_matrices<false>(xs + k16 / 64 * kRows * 128 +
+                             swizzled((rows + (lane & 15)) * 128 + (k16 % 64 + (lane >> 4) * 8) * 2, 128), a);
 #pragma unroll
         for (int j = 0; j < kRank / 16; ++j) {
           uint32_t b[4];
-          load_matrices<true>(ds + (k16 + (lane & 15)) * kPitchD + (j * 16 + (lane >> 4) * 8) * 2, b);
+          load_matrices<true>(ds + j / 4 * kAdapterK * 128 +
+                              swizzled((k16 + (lane & 15)) * kRowD + (j % 4) * 32 + (lane >> 4) * 16, kRowD), b);
           mma_bf16_16816(acc[2 * j], a, b[0], b[1]);
           mma_bf16_16816(acc[2 * j + 1], a, b[2], b[3]);
         }
       }
     }
-    copies_wait<0>();
     __syncthreads();      // the ring is free: it holds the warps' sums now
     {
-      float* mine = part + (kRows == 16 ? warp * 16 * kRank : warp * 16 * kRank);
+      float* mine = part + warp * 16 * kRank;
       const int g = lane >> 2, t = lane & 3;
 #pragma unroll
       for (int j = 0; j < kRank / 8; ++j) {
@@ -189,6 +195,7 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_shrink_kernel(const A
         for (int w = 1; w < kWarps; ++w) v += part[w * 16 * kRank + i];
       sums[i] = v;
     }
+    fence_async_smem();   // the next adapter's tiles are written over the sums by TMA
     if (cluster > 1) cluster_sync_all(); else __syncthreads();
     const float scale = p.scales ? p.scales[adapter] : 1.0f;
     for (int i = blockIdx.x * kAdapterThreads + threadIdx.x; i < kRows * kRank; i += cluster * kAdapterThreads) {
@@ -204,47 +211,69 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_shrink_kernel(const A
     }
     if (cluster > 1) cluster_sync_all(); else __syncthreads();   // sums may be written again (or the block may end)
   }
+  // after a wait that gave up, nothing may still be in flight into this block's shared memory
+  if (!ok && threadIdx.x == 0)
+    for (uint32_t back = min(issued, uint32_t(kStages)); back > 0; --back)
+      mbar_wait(smem_u32(full + (issued - back) % kStages), ((issued - back) / kStages) & 1u, 0xA12);
 }
 
+template <int kRank>
+__host__ __device__ constexpr int expand_slabs() {   // of up weights in flight
+  const int fit = 96 * 1024 / (kRank * kExpandCols * 2);
+  return fit > 8 ? 8 : fit;
+}
 template <int kRank>
 __host__ __device__ constexpr int expand_smem_bytes() {
-  return (kExpandRows * (kRank + 8) + 2 * kRank * (kExpandCols + 8)) * 2 + kExpandRows * (kExpandCols + 8) * 2;
+  return 1024 + kExpandRows * kRank * 2 + expand_slabs<kRank>() * kRank * kExpandCols * 2 + kExpandRows * (kExpandCols + 8) * 2;
 }
 
-// delta of 64 rows and 128 columns: warps take 32 columns each; the adapters' up weights are fetched one
-// ahead.
+// delta of 64 rows and 128 columns: warps take 32 columns each; one thread keeps a ring of the adapters' up
+// weights filled.  With few rows this is a stream of those weights.
 template <int kRank>
-__global__ void __launch_bounds__(kAdapterThreads) adapter_expand_kernel(const AdapterParams p) {
-  constexpr int kPitchT = (kRank + 8) * 2, kPitchU = (kExpandCols + 8) * 2;
-  constexpr int kSlab = kRank * kPitchU;
-  extern __shared__ __align__(128) uint8_t smem[];
+__global__ void __launch_bounds__(kAdapterThreads)
+adapter_expand_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant__ CUtensorMap map_up,
+                      const AdapterParams p) {
+  constexpr int kRowT = kRank < 64 ? kRank * 2 : 128;
+  constexpr int kTile = kExpandRows * kRank * 2, kSlab = kRank * kExpandCols * 2, kSlabs = expand_slabs<kRank>();
+  constexpr int kPitch = (kExpandCols + 8) * 2;
+  extern __shared__ uint8_t smem_raw[];
   __shared__ int of_row[kExpandRows], distinct[kExpandRows], found;
-  const uint32_t ts = smem_u32(smem), us = ts + kExpandRows * kPitchT;
-  uint8_t* staging = smem + kExpandRows * kPitchT + 2 * kSlab;
+  __shared__ __align__(8) uint64_t full[kSlabs], t_full;
+  const uint32_t ts = (smem_u32(smem_raw) + 1023u) & ~1023u, us = ts + kTile;
+  uint8_t* staging = smem_raw + (ts - smem_u32(smem_raw)) + kTile + kSlabs * kSlab;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int row0 = blockIdx.y * kExpandRows, col0 = blockIdx.x * kExpandCols;
   const int rows = min(kExpandRows, p.m - row0);
-  grid_dependency_wait();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kSlabs; ++s) mbar_init(smem_u32(full + s), 1);
+    mbar_init(smem_u32(&t_full), 1);
+    mbar_fence_init();
+    tma_prefetch_desc(&map_t);
+    tma_prefetch_desc(&map_up);
+  }
+  // The shrink kernel has waited for everything before it, so index and up may be read now, t may not.
   grid_dependents_may_launch();
   const int adapters = tile_adapters<kExpandRows>(p, row0, of_row, distinct, &found);
-  auto fetch = [&](int ordinal) {
-    const __nv_bfloat16* up = p.up + distinct[ordinal] * p.stride_up;
-    const uint32_t slab = us + (ordinal & 1) * kSlab;
-    for (int i = threadIdx.x; i < kRank * (kExpandCols / 8); i += kAdapterThreads) {
-      const int r = i / (kExpandCols / 8), c = (i % (kExpandCols / 8)) * 8;
-      const bool valid = r < p.rank && col0 + c < p.n;      // n is a multiple of 8
-      copy_or_zero(slab + r * kPitchU + c * 2, valid ? up + r * p.ld_up + col0 + c : p.up, valid);
-    }
+  auto fetch = [&](int ordinal) {      // one thread
+    const uint32_t s = ordinal % kSlabs, bar = smem_u32(full + s);
+    mbar_arrive_expect_tx(bar, kSlab);
+#pragma unroll
+    for (int c = 0; c < kExpandCols / 64; ++c)
+      tma_load_3d(us + s * kSlab + c * kRank * 128, &map_up, bar, col0 + c * 64, 0, distinct[ordinal]);
   };
+  if (threadIdx.x == 0)
+    for (int ordinal = 0; ordinal < adapters && ordinal < kSlabs - 1; ++ordinal) fetch(ordinal);
+  grid_dependency_wait();
+  bool ok = true;
   if (adapters) {
-    for (int i = threadIdx.x; i < kExpandRows * (kRank / 8); i += kAdapterThreads) {
-      const int r = i / (kRank / 8), c = (i % (kRank / 8)) * 8;
-      const bool valid = r < rows && of_row[r] >= 0;         // rows without an adapter have no t
-      copy_or_zero(ts + r * kPitchT + c * 2, valid ? p.t + static_cast<long long>(row0 + r) * kRank + c : p.t, valid);
+    if (threadIdx.x == 0) {
+      mbar_arrive_expect_tx(smem_u32(&t_full), kTile);
+#pragma unroll
+      for (int c = 0; c < (kRank + 63) / 64; ++c)
+        tma_load_3d(ts + c * kExpandRows * 128, &map_t, smem_u32(&t_full), c * 64, row0, 0);
     }
-    fetch(0);
+    ok = mbar_wait(smem_u32(&t_full), 0, 0xA21);
   }
-  copies_commit();
   float out[4][4][4];     // [16 rows][8 columns][fragment]
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -253,11 +282,11 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_expand_kernel(const A
 #pragma unroll
       for (int e = 0; e < 4; ++e) out[i][j][e] = 0.0f;
   for (int ordinal = 0; ordinal < adapters; ++ordinal) {
-    if (ordinal + 1 < adapters) fetch(ordinal + 1);
-    copies_commit();
-    copies_wait<1>();
-    __syncthreads();
-    const uint32_t slab = us + (ordinal & 1) * kSlab;
+    const uint32_t s = ordinal % kSlabs;
+    if (ok) ok = mbar_wait(smem_u32(full + s), (ordinal / kSlabs) & 1u, 0xA22);
+    __syncthreads();                   // everyone is through with the slab before, which is filled again
+    if (threadIdx.x == 0 && ordinal + kSlabs - 1 < adapters) fetch(ordinal + kSlabs - 1);
+    const uint32_t slab = us + s * kSlab + warp / 2 * kRank * 128;      // the half with this warp's columns
     const int adapter = distinct[ordinal];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -272,11 +301,12 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_expand_kernel(const A
 #pragma unroll
       for (int k16 = 0; k16 < kRank; k16 += 16) {
         uint32_t a[4];
-        load_matrices<false>(ts + (i * 16 + (lane & 15)) * kPitchT + (k16 + (lane >> 4) * 8) * 2, a);
+        load_matrices<false>(ts + k16 / 64 * kExpandRows * 128 +
+                             swizzled((i * 16 + (lane & 15)) * kRowT + (k16 % 64 + (lane >> 4) * 8) * 2, kRowT), a);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           uint32_t b[4];
-          load_matrices<true>(slab + (k16 + (lane & 15)) * kPitchU + (warp * 32 + j * 16 + (lane >> 4) * 8) * 2, b);
+          load_matrices<true>(slab + swizzled((k16 + (lane & 15)) * 128 + (warp % 2) * 64 + j * 32 + (lane >> 4) * 16, 128), b);
           mma_bf16_16816(acc[2 * j], a, b[0], b[1]);
           mma_bf16_16816(acc[2 * j + 1], a, b[2], b[3]);
         }
@@ -287,9 +317,7 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_expand_kernel(const A
         if (high) { out[i][j][2] = acc[j][2]; out[i][j][3] = acc[j][3]; }
       }
     }
-    __syncthreads();      // the slab may be written again
   }
-  copies_wait<0>();
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int col = warp * 32 + j * 8 + 2 * t;
@@ -302,15 +330,20 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_expand_kernel(const A
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      *reinterpret_cast<uint32_t*>(staging + (i * 16 + g) * kPitchU + col * 2) = pack_bf16x2(out[i][j][0] + b0, out[i][j][1] + b1);
-      *reinterpret_cast<uint32_t*>(staging + (i * 16 + g + 8) * kPitchU + col * 2) = pack_bf16x2(out[i][j][2] + b0, out[i][j][3] + b1);
+      *reinterpret_cast<uint32_t*>(staging + (i * 16 + g) * kPitch + col * 2) = pack_bf16x2(out[i][j][0] + b0, out[i][j][1] + b1);
+      *reinterpret_cast<uint32_t*>(staging + (i * 16 + g + 8) * kPitch + col * 2) = pack_bf16x2(out[i][j][2] + b0, out[i][j][3] + b1);
     }
   }
   __syncthreads();
   for (int i = threadIdx.x; i < rows * (kExpandCols / 8); i += kAdapterThreads) {
     const int r = i / (kExpandCols / 8), c = (i % (kExpandCols / 8)) * 8;
     if (col0 + c < p.n)
-      *reinterpret_cast<uint4*>(p.delta + static_cast<long long>(row0 + r) * p.n + col0 + c) = *reinterpret_cast<const uint4*>(staging + r * kPitchU + c * 2);
+      *reinterpret_cast<uint4*>(p.delta + static_cast<long long>(row0 + r) * p.n + col0 + c) = *reinterpret_cast<const uint4*>(staging + r * kPitch + c * 2);
+  }
+  if (!ok && threadIdx.x == 0) {       // as in the kernel above
+    if (adapters) mbar_wait(smem_u32(&t_full), 0, 0xA23);
+    for (int ordinal = max(0, adapters - kSlabs); ordinal < adapters; ++ordinal)
+      mbar_wait(smem_u32(full + ordinal % kSlabs), (ordinal / kSlabs) & 1u, 0xA23);
   }
 }
 
@@ -325,14 +358,21 @@ int launch_shrink(const AdapterParams& p, int sm_count, cudaStream_t stream) {
   auto kernel = adapter_shrink_kernel<kRows, kRank>;
   if (int rc = opt_in_shared_memory(reinterpret_cast<const void*>(kernel), kSmem, &opted, "adapter_shrink")) return rc;
   const int tiles = (p.m + kRows - 1) / kRows;
-  const int ordinals = min(p.count, min(kRows, 16));
+  // Tiles of 16 rows spread their adapters over blocks; those of 64 rows are there for prompts, whose rows
+  // come in runs of one adapter, and take what a tile has one after the other.
+  const int ordinals = kRows == 16 ? min(p.count, 16) : 1;
+  CUtensorMap map_x, map_down;
+  if (int rc = make_tensor_map_2d(&map_x, p.x, 2, p.k, p.m, p.ldx * 2, 64, kRows, true)) return rc;
+  constexpr int kBox = kRank < 64 ? kRank : 64;
+  if (int rc = make_tensor_map_3d(&map_down, p.down, 2, p.rank, p.k, p.count, p.ld_down * 2, p.stride_down * 2, kBox, kAdapterK, 1, kBox * 2))
+    return rc;
   // blocks that share the inner axis: while they find a place beside the tiles and keep two stages each
   unsigned cluster = 1;
-  while (cluster < 8 && static_cast<long long>(tiles) * (kRows == 16 ? ordinals : 1) * cluster * 2 <= 2 * sm_count &&
+  while (cluster < 8 && static_cast<long long>(tiles) * ordinals * cluster * 2 <= 2 * sm_count &&
          p.k >= static_cast<long long>(cluster) * 2 * 2 * kAdapterK)
     cluster *= 2;
   KernelLaunch launch(dim3(cluster, ordinals, tiles), dim3(kAdapterThreads), kSmem, stream, cluster);
-  cudaError_t e = cudaLaunchKernelEx(&launch.config, kernel, p);
+  cudaError_t e = cudaLaunchKernelEx(&launch.config, kernel, map_x, map_down, p);
   if (e != cudaSuccess) return fail(TRINITY_SM100_E_CUDA, "adapter_shrink launch: %s", cudaGetErrorString(e));
   count_launch();
   return check_launch("adapter_shrink");
@@ -347,8 +387,12 @@ int launch_adapters(const AdapterParams& p, int sm_count, cudaStream_t stream) {
   constexpr int kSmem = expand_smem_bytes<kRank>();
   auto kernel = adapter_expand_kernel<kRank>;
   if (int rc = opt_in_shared_memory(reinterpret_cast<const void*>(kernel), kSmem, &opted, "adapter_expand")) return rc;
+  CUtensorMap map_t, map_up;
+  constexpr int kBox = kRank < 64 ? kRank : 64;
+  if (int rc = make_tensor_map_3d(&map_t, p.t, 2, kRank, p.m, 1, kRank * 2, kRank * 2ull * p.m, kBox, kExpandRows, 1, kBox * 2)) return rc;
+  if (int rc = make_tensor_map_3d(&map_up, p.up, 2, p.n, p.rank, p.count, p.ld_up * 2, p.stride_up * 2, 64, kRank, 1, 128)) return rc;
   KernelLaunch launch(dim3((p.n + kExpandCols - 1) / kExpandCols, (p.m + kExpandRows - 1) / kExpandRows), dim3(kAdapterThreads), kSmem, stream);
-  cudaError_t e = cudaLaunchKernelEx(&launch.config, kernel, p);
+  cudaError_t e = cudaLaunchKernelEx(&launch.config, kernel, map_t, map_up, p);
   if (e != cudaSuccess) return fail(TRINITY_SM100_E_CUDA, "adapter_expand launch: %s", cudaGetErrorString(e));
   count_launch();
   return check_launch("adapter_expand");
@@ -381,6 +425,8 @@ extern "C" int trinity_sm100_gemm_adapters_bf16(const trinity_sm100_gemm* gemm, 
   if (g.k % 8 || g.n % 8)
     return fail(TRINITY_SM100_E_UNSUPPORTED, "gemm_adapters: k (%lld) and n (%lld) must be multiples of 8", (long long)g.k, (long long)g.n);
   if (a.ld_down < a.rank || a.ld_up < g.n) return fail(TRINITY_SM100_E_INVALID, "gemm_adapters: leading dimension smaller than the row");
+  if (a.count > 1 && (a.stride_down <= 0 || a.stride_up <= 0))
+    return fail(TRINITY_SM100_E_INVALID, "gemm_adapters: strides between adapters must be positive");
   if (a.ld_down % 8 || a.ld_up % 8 || a.stride_down % 8 || a.stride_up % 8 || !aligned16(a.down) || !aligned16(a.up) ||
       !aligned16(a.workspace))
     return fail(TRINITY_SM100_E_INVALID, "gemm_adapters: adapter rows and the workspace must start on 16 bytes");
@@ -404,9 +450,9 @@ extern "C" int trinity_sm100_gemm_adapters_bf16(const trinity_sm100_gemm* gemm, 
   p.delta = reinterpret_cast<__nv_bfloat16*>(static_cast<uint8_t*>(a.workspace) + adapter_t_bytes(g.m, a.rank));
   p.ldx = g.lda;
   p.ld_down = a.ld_down;
-  p.stride_down = a.stride_down;
+  p.stride_down = a.count > 1 ? a.stride_down : a.ld_down * g.k;
   p.ld_up = a.ld_up;
-  p.stride_up = a.stride_up;
+  p.stride_up = a.count > 1 ? a.stride_up : a.ld_up * a.rank;
 
   p.m = int(g.m);
   p.n = int(g.n);
