@@ -23,7 +23,7 @@ namespace {
 constexpr uint32_t kSiteAdapterIndex = 0xA01;   // an index that names no adapter (the row gets none)
 constexpr int kAdapterThreads = 128;
 constexpr int kAdapterK = 128;                  // inner extent of a stage of the shrink kernel
-constexpr int kExpandRows = 64, kExpandCols = 128;
+constexpr int kExpandRows = 64;
 
 struct AdapterParams {
   const __nv_bfloat16* x;
@@ -128,15 +128,17 @@ adapter_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
   grid_dependents_may_launch();
   const int adapters = tile_adapters<kRows>(p, row0, of_row, distinct, &found);
   const int blocks_k = (p.k + kAdapterK - 1) / kAdapterK;
-  const int begin = int(static_cast<long long>(blockIdx.x) * blocks_k / cluster);
-  const int end = int(static_cast<long long>(blockIdx.x + 1) * blocks_k / cluster);
+  // Block c of a cluster takes every cluster-th chunk of the inner axis: at any time the blocks read
+  // neighbouring pieces of the rows.
+  const int chunks = (blocks_k - int(blockIdx.x) + int(cluster) - 1) / int(cluster);
   uint32_t issued = 0, taken = 0;      // tiles, over all adapters of this block
   bool ok = true;
 
   for (int ordinal = blockIdx.y; ordinal < adapters; ordinal += gridDim.y) {
     const int adapter = distinct[ordinal];
-    auto fetch = [&](int kb) {         // one thread
+    auto fetch = [&](int chunk) {      // one thread
       const uint32_t s = issued % kStages, bar = smem_u32(full + s), stage = ring + s * kStage;
+      const int kb = int(blockIdx.x) + chunk * int(cluster);
       mbar_arrive_expect_tx(bar, kStage);
 #pragma unroll
       for (int c = 0; c < kAdapterK / 64; ++c)
@@ -152,12 +154,12 @@ adapter_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[j][e] = 0.0f;
     if (threadIdx.x == 0)
-      for (int kb = begin; kb < end && kb < begin + kStages - 1; ++kb) fetch(kb);
-    for (int kb = begin; kb < end; ++kb, ++taken) {
+      for (int chunk = 0; chunk < chunks && chunk < kStages - 1; ++chunk) fetch(chunk);
+    for (int chunk = 0; chunk < chunks; ++chunk, ++taken) {
       const uint32_t s = taken % kStages;
       if (ok) ok = mbar_wait(smem_u32(full + s), (taken / kStages) & 1u, 0xA11);
       __syncthreads();                 // everyone is through with the tile before, whose stage is filled again
-      if (threadIdx.x == 0 && kb + kStages - 1 < end) fetch(kb + kStages - 1);
+      if (threadIdx.x == 0 && chunk + kStages - 1 < chunks) fetch(chunk + kStages - 1);
       const uint32_t xs = ring + s * kStage, ds = xs + kRows * kAdapterK * 2;
       const int first = kRows == 16 ? warp : 0, step = kRows == 16 ? kWarps : 1;
       const int rows = kRows == 16 ? 0 : warp * 16;
@@ -217,32 +219,37 @@ adapter_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
       mbar_wait(smem_u32(full + (issued - back) % kStages), ((issued - back) / kStages) & 1u, 0xA12);
 }
 
-template <int kRank>
-__host__ __device__ constexpr int expand_slabs() {   // of up weights in flight
-  const int fit = 96 * 1024 / (kRank * kExpandCols * 2);
-  return fit > 8 ? 8 : fit;
+// Prompts (kCols 128): rows come in runs of one adapter, a tile has one or two, two slabs of up weights do
+// and many small blocks fit an SM.  Few rows (kCols 256): a stream of up weights, as wide as the rows
+// of a slab get (narrow pieces of far-apart rows are slow to fetch) and several in flight.
+template <int kRank, int kCols>
+__host__ __device__ constexpr int expand_slabs() {
+  const int fit = 96 * 1024 / (kRank * kCols * 2);
+  return kCols == 128 ? 2 : fit > 8 ? 8 : fit < 2 ? 2 : fit;
 }
-template <int kRank>
+template <int kRank, int kCols>
 __host__ __device__ constexpr int expand_smem_bytes() {
-  return 1024 + kExpandRows * kRank * 2 + expand_slabs<kRank>() * kRank * kExpandCols * 2 + kExpandRows * (kExpandCols + 8) * 2;
+  return 1024 + kExpandRows * kRank * 2 + expand_slabs<kRank, kCols>() * kRank * kCols * 2 + kExpandRows * (kCols + 8) * 2;
 }
 
-// delta of 64 rows and 128 columns: warps take 32 columns each; one thread keeps a ring of the adapters' up
-// weights filled.  With few rows this is a stream of those weights.
-template <int kRank>
-__global__ void __launch_bounds__(kAdapterThreads)
+// delta of 64 rows and kCols columns: warps take 32 columns each; one thread keeps a ring of the adapters' up
+// weights filled.  Block blockIdx.z of gridDim.z takes every gridDim.z-th adapter of the tile and writes
+// the rows of those (the first one those without an adapter too): no two blocks write the same row.
+template <int kRank, int kCols>
+__global__ void __launch_bounds__(kCols)
 adapter_expand_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant__ CUtensorMap map_up,
                       const AdapterParams p) {
   constexpr int kRowT = kRank < 64 ? kRank * 2 : 128;
-  constexpr int kTile = kExpandRows * kRank * 2, kSlab = kRank * kExpandCols * 2, kSlabs = expand_slabs<kRank>();
-  constexpr int kPitch = (kExpandCols + 8) * 2;
+  constexpr int kTile = kExpandRows * kRank * 2, kSlab = kRank * kCols * 2, kSlabs = expand_slabs<kRank, kCols>();
+  constexpr int kPitch = (kCols + 8) * 2;
   extern __shared__ uint8_t smem_raw[];
   __shared__ int of_row[kExpandRows], distinct[kExpandRows], found;
+  __shared__ bool mine[kExpandRows];       // rows that this block writes
   __shared__ __align__(8) uint64_t full[kSlabs], t_full;
   const uint32_t ts = (smem_u32(smem_raw) + 1023u) & ~1023u, us = ts + kTile;
   uint8_t* staging = smem_raw + (ts - smem_u32(smem_raw)) + kTile + kSlabs * kSlab;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int row0 = blockIdx.y * kExpandRows, col0 = blockIdx.x * kExpandCols;
+  const int row0 = blockIdx.y * kExpandRows, col0 = blockIdx.x * kCols;
   const int rows = min(kExpandRows, p.m - row0);
   if (threadIdx.x == 0) {
     for (int s = 0; s < kSlabs; ++s) mbar_init(smem_u32(full + s), 1);
@@ -253,14 +260,22 @@ adapter_expand_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_co
   }
   // The shrink kernel has waited for everything before it, so index and up may be read now, t may not.
   grid_dependents_may_launch();
-  const int adapters = tile_adapters<kExpandRows>(p, row0, of_row, distinct, &found);
+  const int in_tile = tile_adapters<kExpandRows>(p, row0, of_row, distinct, &found);
+  const int share = gridDim.z, part = blockIdx.z;
+  const int adapters = (in_tile - part + share - 1) / share;      // of this block (at least 0: part < share)
+  auto adapter_of = [&](int ordinal) { return distinct[part + ordinal * share]; };
   auto fetch = [&](int ordinal) {      // one thread
     const uint32_t s = ordinal % kSlabs, bar = smem_u32(full + s);
     mbar_arrive_expect_tx(bar, kSlab);
 #pragma unroll
-    for (int c = 0; c < kExpandCols / 64; ++c)
-      tma_load_3d(us + s * kSlab + c * kRank * 128, &map_up, bar, col0 + c * 64, 0, distinct[ordinal]);
+    for (int c = 0; c < kCols / 64; ++c)
+      tma_load_3d(us + s * kSlab + c * kRank * 128, &map_up, bar, col0 + c * 64, 0, adapter_of(ordinal));
   };
+  for (int i = threadIdx.x; i < kExpandRows; i += kCols) {
+    bool write = part == 0 && of_row[i] < 0;
+    for (int ordinal = 0; ordinal < adapters && !write; ++ordinal) write = of_row[i] == adapter_of(ordinal);
+    mine[i] = write;
+  }
   if (threadIdx.x == 0)
     for (int ordinal = 0; ordinal < adapters && ordinal < kSlabs - 1; ++ordinal) fetch(ordinal);
   grid_dependency_wait();
@@ -287,7 +302,7 @@ adapter_expand_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_co
     __syncthreads();                   // everyone is through with the slab before, which is filled again
     if (threadIdx.x == 0 && ordinal + kSlabs - 1 < adapters) fetch(ordinal + kSlabs - 1);
     const uint32_t slab = us + s * kSlab + warp / 2 * kRank * 128;      // the half with this warp's columns
-    const int adapter = distinct[ordinal];
+    const int adapter = adapter_of(ordinal);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (i * 16 >= rows) break;
@@ -335,9 +350,9 @@ adapter_expand_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_co
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < rows * (kExpandCols / 8); i += kAdapterThreads) {
-    const int r = i / (kExpandCols / 8), c = (i % (kExpandCols / 8)) * 8;
-    if (col0 + c < p.n)
+  for (int i = threadIdx.x; i < rows * (kCols / 8); i += kCols) {
+    const int r = i / (kCols / 8), c = (i % (kCols / 8)) * 8;
+    if (col0 + c < p.n && mine[r])
       *reinterpret_cast<uint4*>(p.delta + static_cast<long long>(row0 + r) * p.n + col0 + c) = *reinterpret_cast<const uint4*>(staging + r * kPitch + c * 2);
   }
   if (!ok && threadIdx.x == 0) {       // as in the kernel above
@@ -378,24 +393,36 @@ int launch_shrink(const AdapterParams& p, int sm_count, cudaStream_t stream) {
   return check_launch("adapter_shrink");
 }
 
-template <int kRank>
-int launch_adapters(const AdapterParams& p, int sm_count, cudaStream_t stream) {
-  // tiles of 16 rows while there are few of them, of 64 rows once those fill half the SMs
-  if (int rc = p.m >= 64 * (sm_count / 2) ? launch_shrink<64, kRank>(p, sm_count, stream) : launch_shrink<16, kRank>(p, sm_count, stream))
-    return rc;
+template <int kRank, int kCols>
+int launch_expand(const AdapterParams& p, int sm_count, cudaStream_t stream) {
   static unsigned long long opted = 0;
-  constexpr int kSmem = expand_smem_bytes<kRank>();
-  auto kernel = adapter_expand_kernel<kRank>;
+  constexpr int kSmem = expand_smem_bytes<kRank, kCols>();
+  static_assert(kSmem <= 232448 - 2048, "exceeds the 227 KB shared-memory limit");
+  auto kernel = adapter_expand_kernel<kRank, kCols>;
   if (int rc = opt_in_shared_memory(reinterpret_cast<const void*>(kernel), kSmem, &opted, "adapter_expand")) return rc;
   CUtensorMap map_t, map_up;
   constexpr int kBox = kRank < 64 ? kRank : 64;
   if (int rc = make_tensor_map_3d(&map_t, p.t, 2, kRank, p.m, 1, kRank * 2, kRank * 2ull * p.m, kBox, kExpandRows, 1, kBox * 2)) return rc;
   if (int rc = make_tensor_map_3d(&map_up, p.up, 2, p.n, p.rank, p.count, p.ld_up * 2, p.stride_up * 2, 64, kRank, 1, 128)) return rc;
-  KernelLaunch launch(dim3((p.n + kExpandCols - 1) / kExpandCols, (p.m + kExpandRows - 1) / kExpandRows), dim3(kAdapterThreads), kSmem, stream);
+  const dim3 tiles((p.n + kCols - 1) / kCols, (p.m + kExpandRows - 1) / kExpandRows);
+  // blocks that share a tile's adapters, while there are SMs without one
+  unsigned share = 1;
+  if (kCols == 256)
+    while (share < 8 && share * 2 <= unsigned(min(p.count, kExpandRows)) && tiles.x * tiles.y * share * 2 <= unsigned(2 * sm_count)) share *= 2;
+  KernelLaunch launch(dim3(tiles.x, tiles.y, share), dim3(kCols), kSmem, stream);
   cudaError_t e = cudaLaunchKernelEx(&launch.config, kernel, map_t, map_up, p);
   if (e != cudaSuccess) return fail(TRINITY_SM100_E_CUDA, "adapter_expand launch: %s", cudaGetErrorString(e));
   count_launch();
   return check_launch("adapter_expand");
+}
+
+template <int kRank>
+int launch_adapters(const AdapterParams& p, int sm_count, cudaStream_t stream) {
+  // tiles of 16 rows while there are few of them, of 64 rows once those fill half the SMs
+  if (int rc = p.m >= 64 * (sm_count / 2) ? launch_shrink<64, kRank>(p, sm_count, stream) : launch_shrink<16, kRank>(p, sm_count, stream))
+    return rc;
+  // wide tiles for up to four tiles of rows (decode batches), narrow ones beyond
+  return p.m <= 4 * kExpandRows ? launch_expand<kRank, 256>(p, sm_count, stream) : launch_expand<kRank, 128>(p, sm_count, stream);
 }
 
 }  // namespace
@@ -432,7 +459,7 @@ extern "C" int trinity_sm100_gemm_adapters_bf16(const trinity_sm100_gemm* gemm, 
     return fail(TRINITY_SM100_E_INVALID, "gemm_adapters: adapter rows and the workspace must start on 16 bytes");
   if (reinterpret_cast<uintptr_t>(a.index) % 4 || reinterpret_cast<uintptr_t>(a.scales) % 4)
     return fail(TRINITY_SM100_E_INVALID, "gemm_adapters: a pointer is not aligned to its element type");
-  if (g.m > 65535ll * 16 || (g.n + kExpandCols - 1) / kExpandCols > INT32_MAX)
+  if (g.m > 65535ll * 16 || g.n > INT32_MAX - 256)
     return fail(TRINITY_SM100_E_UNSUPPORTED, "gemm_adapters: too many rows (%lld)", (long long)g.m);
   const size_t need = trinity_sm100_gemm_adapters_workspace_bytes(g.m, g.n, a.rank);
   if (a.workspace_bytes < need)

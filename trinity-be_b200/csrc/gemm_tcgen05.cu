@@ -282,6 +282,12 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a,
   // (other CTAs) is the first CTA's word that its stage ring is free to receive them
   const uint32_t partial_bar = stored_count + 8u;
   const uint32_t go_bar = stored_count + 16u;
+  // A matrix side operand of BF16 outputs comes by TMA into the staging buffers, where the result then
+  // takes its place (thread-wise loads of its own row by each thread cost the 8192^3 GEMM up to a tenth
+  // of its time).  Its tensor map travels in the place of the second right operand's.
+  constexpr bool kCanStageBias = !kOutF32 && !kGated && !kFused && !kBatched && !kSplit;
+  const bool staged_bias = kCanStageBias && p.bias_mode == TRINITY_SM100_BIAS_MATRIX;
+  auto bias_bar = [&](int quad, uint32_t buffer) { return stored_count + 24u + 8u * (quad * 2 + buffer); };
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -308,6 +314,8 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a,
       mbar_init(tmem_full_bar(a), 1);
       mbar_init(tmem_empty_bar(a), kPair ? 8 : 4);
     }
+    if (kCanStageBias)
+      for (int i = 0; i < 8; ++i) mbar_init(bias_bar(i >> 1, i & 1), 1);
     asm volatile("st.shared::cta.u32 [%0], %1;" ::"r"(stored_count), "r"(0u) : "memory");
     if (kSplit) {
       mbar_init(partial_bar, 1);
@@ -450,6 +458,17 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a,
     uint32_t store_buf = 0;
     bool ok = true;
     const int etid = threadIdx.x - 64;      // 0..127 within the epilogue group
+    // staged side operand: chunk `chunk` of this warp (kColsPerStore columns of its 32 rows) lies in buffer
+    // chunk & 1; the one after it is fetched while it is worked on, across tiles
+    uint32_t chunk = 0;
+    auto fetch_bias = [&](int unit, int c0, uint32_t buffer) {
+      int m_blk, n_blk, tile;
+      locate_tile<kPair>(p, unit, rank, m_blk, n_blk, tile);
+      mbar_arrive_expect_tx(bias_bar(quad, buffer), kStoreBufBytes);
+      tma_load_2d(my_staging_u32 + buffer * kStoreBufBytes, &map_b2, bias_bar(quad, buffer), n_blk * kOutN + c0,
+                  m_blk * kBM + quad * 32);
+    };
+    if (staged_bias && lane == 0 && first_unit < num_units) fetch_bias(first_unit, 0, 0);
     for (int unit = first_unit; unit < num_units && ok; unit += unit_stride, ++local_tile) {
       int m_blk, n_blk, tile;
       const int z = kBatched ? unit / p.tiles_per_batch : 0;
@@ -632,8 +651,17 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a,
         continue;
       }
 
-      for (int c0 = 0; c0 < kOutN; c0 += kColsPerStore) {
-        if (lane == 0) tma_store_wait_read<1>();
+      for (int c0 = 0; c0 < kOutN; c0 += kColsPerStore, ++chunk) {
+        if (staged_bias) {
+          if (lane == 0) {
+            tma_store_wait_read<0>();     // the other buffer's last store, a chunk ago
+            const int next_unit = c0 + kColsPerStore < kOutN ? unit : unit + unit_stride;
+            if (next_unit < num_units) fetch_bias(next_unit, next_unit == unit ? c0 + kColsPerStore : 0, store_buf ^ 1u);
+          }
+          if (!__all_sync(0xffffffffu, mbar_wait(bias_bar(quad, store_buf), (chunk >> 1) & 1u, 0x304))) ok = false;
+        } else if (lane == 0) {
+          tma_store_wait_read<1>();
+        }
         __syncwarp();
         uint8_t* buf = my_staging + store_buf * kStoreBufBytes;
 #pragma unroll
@@ -681,6 +709,18 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a,
           } else if (p.bias_mode == TRINITY_SM100_BIAS_ROW_VECTOR) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) x[j] += row_bias;
+          } else if (staged_bias) {
+            const uint8_t* brow = buf + lane * 128;      // laid out as the result below
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              const uint4 b = *reinterpret_cast<const uint4*>(brow + (((sub * 4 + u) ^ (lane & 7)) << 4));
+              const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                x[u * 8 + e * 2] += bf16_lo(w[e]);
+                x[u * 8 + e * 2 + 1] += bf16_hi(w[e]);
+              }
+            }
           } else if (p.bias_mode == TRINITY_SM100_BIAS_MATRIX) {
             if (row < p.m) {
               const __nv_bfloat16* brow = bias_base + static_cast<long long>(row) * p.ld_bias + gcol;
@@ -764,6 +804,8 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a,
         if (blockIdx.x == 0 && etid == 0) g_fused_stamps[2] = global_ns();
       }
     }
+    // after a wait that gave up, the chunk of the side operand that was already asked for must still land
+    if (staged_bias && !ok && lane == 0) mbar_wait(bias_bar(quad, chunk & 1u), (chunk >> 1) & 1u, 0x305);
     if (lane == 0) tma_store_wait_all();
   }
   if (kFused && warp == 10) {
@@ -932,9 +974,11 @@ int launch_gemm(const trinity_sm100_gemm& g, int sm_count, cudaStream_t stream, 
     if ((rc = make_tensor_map_2d(&map_a, g.a, 2, g.k, g.m, g.lda * 2, kBK, kSplit ? (g.m <= 32 ? 32 : 64) : kBM, true)))
       return rc;
     if ((rc = make_tensor_map_2d(&map_b, g.b, 2, g.n, g.k, g.ldb * 2, 64, kBK, true))) return rc;
-    if ((rc = make_tensor_map_2d(&map_b2, kGated ? g.b2 : g.b, 2, g.n, g.k, g.ldb * 2, 64, kBK,
-                                 true)))
-      return rc;
+    if (!kOutF32 && !kGated && !kFused && !kSplit && g.bias_mode == TRINITY_SM100_BIAS_MATRIX)
+      rc = make_tensor_map_2d(&map_b2, g.bias, 2, g.n, g.m, g.ld_bias * 2, 64, 32, true);   // the staged side operand
+    else
+      rc = make_tensor_map_2d(&map_b2, kGated ? g.b2 : g.b, 2, g.n, g.k, g.ldb * 2, 64, kBK, true);
+    if (rc) return rc;
     if ((rc = make_tensor_map_2d(&map_out, g.out, out_bytes, g.n, g.m, g.ldo * out_bytes,
                                  128 / out_bytes, 32, true)))
       return rc;
