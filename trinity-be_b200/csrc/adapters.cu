@@ -21,7 +21,7 @@ namespace trinity_sm100 {
 namespace {
 
 constexpr uint32_t kSiteAdapterIndex = 0xA01;   // an index that names no adapter (the row gets none)
-constexpr int kAdapterThreads = 128;
+constexpr int kAdapterThreads = 256;            // of the shrink kernel
 constexpr int kAdapterK = 128;                  // inner extent of a stage of the shrink kernel
 constexpr int kExpandRows = 64;
 
@@ -91,19 +91,19 @@ __host__ __device__ constexpr int shrink_stages() {
 template <int kRows, int kRank>
 __host__ __device__ constexpr int shrink_smem_bytes() {
   const int ring = shrink_stages<kRows, kRank>() * shrink_stage_bytes<kRows, kRank>();
-  const int sums = (kRows == 16 ? kAdapterThreads / 32 : 1) * kRows * kRank * 4;
+  const int sums = kAdapterThreads / 32 * 16 * kRank * 4;
   return 1024 + (ring > sums ? ring : sums) + kRows * kRank * 4;
 }
 
 // t of kRows rows.  The inner axis is shared by the blocks of a cluster (blockIdx.x), whose sums meet in
 // distributed shared memory in a fixed order; blockIdx.y takes every gridDim.y-th adapter of the tile,
-// blockIdx.z the tile.  With 16 rows the warps share the inner axis, with 64 each has 16 rows.  One
+// blockIdx.z the tile.  A warp takes 16 rows and every kShares-th 16 of the inner axis.  One
 // thread keeps a ring of TMA tiles filled (x in boxes of 64 columns, down in boxes of at most 64).
 template <int kRows, int kRank>
 __global__ void __launch_bounds__(kAdapterThreads)
 adapter_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_down,
                       const AdapterParams p) {
-  constexpr int kWarps = kAdapterThreads / 32;
+  constexpr int kShares = kAdapterThreads / 32 / (kRows / 16);     // warps that share 16 rows
   constexpr int kStages = shrink_stages<kRows, kRank>();
   constexpr int kStage = shrink_stage_bytes<kRows, kRank>();
   constexpr int kRowD = kRank < 64 ? kRank * 2 : 128;         // bytes of a row of a box of down
@@ -161,11 +161,10 @@ adapter_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
       __syncthreads();                 // everyone is through with the tile before, whose stage is filled again
       if (threadIdx.x == 0 && chunk + kStages - 1 < chunks) fetch(chunk + kStages - 1);
       const uint32_t xs = ring + s * kStage, ds = xs + kRows * kAdapterK * 2;
-      const int first = kRows == 16 ? warp : 0, step = kRows == 16 ? kWarps : 1;
-      const int rows = kRows == 16 ? 0 : warp * 16;
+      const int rows = warp / kShares * 16;
 #pragma unroll
-      for (int i = 0; i < kAdapterK / 16 / (kRows == 16 ? kWarps : 1); ++i) {
-        const int k16 = (first + i * step) * 16;
+      for (int i = 0; i < kAdapterK / 16 / kShares; ++i) {
+        const int k16 = (warp % kShares + i * kShares) * 16;
         uint32_t a[4];
         load_matrices<false>(xs + k16 / 64 * kRows * 128 +
                              swizzled((rows + (lane & 15)) * 128 + (k16 % 64 + (lane >> 4) * 8) * 2, 128), a);
@@ -191,10 +190,10 @@ adapter_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
     }
     __syncthreads();
     for (int i = threadIdx.x; i < kRows * kRank; i += kAdapterThreads) {
-      float v = part[i];
-      if (kRows == 16)
+      const float* first = part + i / (16 * kRank) * kShares * 16 * kRank + i % (16 * kRank);
+      float v = first[0];
 #pragma unroll
-        for (int w = 1; w < kWarps; ++w) v += part[w * 16 * kRank + i];
+      for (int w = 1; w < kShares; ++w) v += first[w * 16 * kRank];
       sums[i] = v;
     }
     fence_async_smem();   // the next adapter's tiles are written over the sums by TMA
@@ -219,22 +218,24 @@ adapter_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
       mbar_wait(smem_u32(full + (issued - back) % kStages), ((issued - back) / kStages) & 1u, 0xA12);
 }
 
-// Prompts (kCols 128): rows come in runs of one adapter, a tile has one or two, two slabs of up weights do
-// and many small blocks fit an SM.  Few rows (kCols 256): a stream of up weights, as wide as the rows
-// of a slab get (narrow pieces of far-apart rows are slow to fetch) and several in flight.
+// Prompts (kCols 128): rows come in runs of one adapter, a slab of up weights is small and several small
+// blocks share an SM.  Few rows (kCols 256): a stream of up weights, as wide as the rows of a slab get
+// (narrow pieces of far-apart rows are slow to fetch).
 template <int kRank, int kCols>
 __host__ __device__ constexpr int expand_slabs() {
-  const int fit = 96 * 1024 / (kRank * kCols * 2);
-  return kCols == 128 ? 2 : fit > 8 ? 8 : fit < 2 ? 2 : fit;
+  const int fit = (kCols == 128 ? 32 : kRank < 64 ? 64 : 160) * 1024 / (kRank * kCols * 2);
+  return fit > 8 ? 8 : fit < 2 ? 2 : fit;
 }
 template <int kRank, int kCols>
 __host__ __device__ constexpr int expand_smem_bytes() {
   return 1024 + kExpandRows * kRank * 2 + expand_slabs<kRank, kCols>() * kRank * kCols * 2 + kExpandRows * (kCols + 8) * 2;
 }
 
-// delta of 64 rows and kCols columns: warps take 32 columns each; one thread keeps a ring of the adapters' up
-// weights filled.  Block blockIdx.z of gridDim.z takes every gridDim.z-th adapter of the tile and writes
-// the rows of those (the first one those without an adapter too): no two blocks write the same row.
+// delta of 64 rows.  The work on a tile of rows is a sequence of slabs, (kCols columns, adapter) with the
+// adapters innermost; the gridDim.x blocks of a tile take equal runs of it, with one thread keeping a ring
+// of slabs filled across the columns.  Warps take 32 columns each.  A block writes, of the columns of a
+// slab, the rows of the adapters that its run covered (rows without one go with the first adapter): every
+// element is written once.
 template <int kRank, int kCols>
 __global__ void __launch_bounds__(kCols)
 adapter_expand_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant__ CUtensorMap map_up,
@@ -243,13 +244,12 @@ adapter_expand_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_co
   constexpr int kTile = kExpandRows * kRank * 2, kSlab = kRank * kCols * 2, kSlabs = expand_slabs<kRank, kCols>();
   constexpr int kPitch = (kCols + 8) * 2;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ int of_row[kExpandRows], distinct[kExpandRows], found;
-  __shared__ bool mine[kExpandRows];       // rows that this block writes
+  __shared__ int of_row[kExpandRows], distinct[kExpandRows], place[kExpandRows], found;   // place of a row's adapter in distinct
   __shared__ __align__(8) uint64_t full[kSlabs], t_full;
   const uint32_t ts = (smem_u32(smem_raw) + 1023u) & ~1023u, us = ts + kTile;
   uint8_t* staging = smem_raw + (ts - smem_u32(smem_raw)) + kTile + kSlabs * kSlab;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int row0 = blockIdx.y * kExpandRows, col0 = blockIdx.x * kCols;
+  const int row0 = blockIdx.y * kExpandRows;
   const int rows = min(kExpandRows, p.m - row0);
   if (threadIdx.x == 0) {
     for (int s = 0; s < kSlabs; ++s) mbar_init(smem_u32(full + s), 1);
@@ -260,27 +260,29 @@ adapter_expand_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_co
   }
   // The shrink kernel has waited for everything before it, so index and up may be read now, t may not.
   grid_dependents_may_launch();
-  const int in_tile = tile_adapters<kExpandRows>(p, row0, of_row, distinct, &found);
-  const int share = gridDim.z, part = blockIdx.z;
-  const int adapters = (in_tile - part + share - 1) / share;      // of this block (at least 0: part < share)
-  auto adapter_of = [&](int ordinal) { return distinct[part + ordinal * share]; };
-  auto fetch = [&](int ordinal) {      // one thread
-    const uint32_t s = ordinal % kSlabs, bar = smem_u32(full + s);
+  const int adapters = tile_adapters<kExpandRows>(p, row0, of_row, distinct, &found);
+  const int steps = max(adapters, 1);
+  const long long total = static_cast<long long>((p.n + kCols - 1) / kCols) * steps;
+  const int begin = int(total * blockIdx.x / gridDim.x), end = int(total * (blockIdx.x + 1) / gridDim.x);
+  auto fetch = [&](int q) {            // one thread
+    const int s = (q - begin) % kSlabs;
+    const uint32_t bar = smem_u32(full + s);
     mbar_arrive_expect_tx(bar, kSlab);
 #pragma unroll
     for (int c = 0; c < kCols / 64; ++c)
-      tma_load_3d(us + s * kSlab + c * kRank * 128, &map_up, bar, col0 + c * 64, 0, adapter_of(ordinal));
+      tma_load_3d(us + s * kSlab + c * kRank * 128, &map_up, bar, q / steps * kCols + c * 64, 0, distinct[q % steps]);
   };
+  if (threadIdx.x == 0 && adapters)
+    for (int q = begin; q < end && q < begin + kSlabs - 1; ++q) fetch(q);
   for (int i = threadIdx.x; i < kExpandRows; i += kCols) {
-    bool write = part == 0 && of_row[i] < 0;
-    for (int ordinal = 0; ordinal < adapters && !write; ++ordinal) write = of_row[i] == adapter_of(ordinal);
-    mine[i] = write;
+    int at = 0;
+    for (int o = 1; o < adapters; ++o)
+      if (of_row[i] == distinct[o]) at = o;
+    place[i] = at;
   }
-  if (threadIdx.x == 0)
-    for (int ordinal = 0; ordinal < adapters && ordinal < kSlabs - 1; ++ordinal) fetch(ordinal);
   grid_dependency_wait();
   bool ok = true;
-  if (adapters) {
+  if (adapters && begin < end) {
     if (threadIdx.x == 0) {
       mbar_arrive_expect_tx(smem_u32(&t_full), kTile);
 #pragma unroll
@@ -296,69 +298,79 @@ adapter_expand_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_co
     for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) out[i][j][e] = 0.0f;
-  for (int ordinal = 0; ordinal < adapters; ++ordinal) {
-    const uint32_t s = ordinal % kSlabs;
-    if (ok) ok = mbar_wait(smem_u32(full + s), (ordinal / kSlabs) & 1u, 0xA22);
+  int from = begin % steps;            // first adapter of the run on the present columns
+  for (int q = begin; q < end; ++q) {
+    const int s = (q - begin) % kSlabs, ordinal = q % steps;
+    if (adapters && ok) ok = mbar_wait(smem_u32(full + s), ((q - begin) / kSlabs) & 1u, 0xA22);
     __syncthreads();                   // everyone is through with the slab before, which is filled again
-    if (threadIdx.x == 0 && ordinal + kSlabs - 1 < adapters) fetch(ordinal + kSlabs - 1);
-    const uint32_t slab = us + s * kSlab + warp / 2 * kRank * 128;      // the half with this warp's columns
-    const int adapter = adapter_of(ordinal);
+    if (threadIdx.x == 0 && adapters && q + kSlabs - 1 < end) fetch(q + kSlabs - 1);
+    if (adapters) {
+      const uint32_t slab = us + s * kSlab + warp / 2 * kRank * 128;      // the half with this warp's columns
+      const int adapter = distinct[ordinal];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (i * 16 >= rows) break;
-      const bool low = of_row[i * 16 + g] == adapter, high = of_row[i * 16 + g + 8] == adapter;
-      if (!__any_sync(0xffffffffu, low || high)) continue;
-      float acc[4][4];
+      for (int i = 0; i < 4; ++i) {
+        if (i * 16 >= rows) break;
+        const bool low = of_row[i * 16 + g] == adapter, high = of_row[i * 16 + g + 8] == adapter;
+        if (!__any_sync(0xffffffffu, low || high)) continue;
+        float acc[4][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[j][e] = 0.0f;
+          for (int e = 0; e < 4; ++e) acc[j][e] = 0.0f;
 #pragma unroll
-      for (int k16 = 0; k16 < kRank; k16 += 16) {
-        uint32_t a[4];
-        load_matrices<false>(ts + k16 / 64 * kExpandRows * 128 +
-                             swizzled((i * 16 + (lane & 15)) * kRowT + (k16 % 64 + (lane >> 4) * 8) * 2, kRowT), a);
+        for (int k16 = 0; k16 < kRank; k16 += 16) {
+          uint32_t a[4];
+          load_matrices<false>(ts + k16 / 64 * kExpandRows * 128 +
+                               swizzled((i * 16 + (lane & 15)) * kRowT + (k16 % 64 + (lane >> 4) * 8) * 2, kRowT), a);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          uint32_t b[4];
-          load_matrices<true>(slab + swizzled((k16 + (lane & 15)) * 128 + (warp % 2) * 64 + j * 32 + (lane >> 4) * 16, 128), b);
-          mma_bf16_16816(acc[2 * j], a, b[0], b[1]);
-          mma_bf16_16816(acc[2 * j + 1], a, b[2], b[3]);
+          for (int j = 0; j < 2; ++j) {
+            uint32_t b[4];
+            load_matrices<true>(slab + swizzled((k16 + (lane & 15)) * 128 + (warp % 2) * 64 + j * 32 + (lane >> 4) * 16, 128), b);
+            mma_bf16_16816(acc[2 * j], a, b[0], b[1]);
+            mma_bf16_16816(acc[2 * j + 1], a, b[2], b[3]);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (low) { out[i][j][0] = acc[j][0]; out[i][j][1] = acc[j][1]; }
+          if (high) { out[i][j][2] = acc[j][2]; out[i][j][3] = acc[j][3]; }
         }
       }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (low) { out[i][j][0] = acc[j][0]; out[i][j][1] = acc[j][1]; }
-        if (high) { out[i][j][2] = acc[j][2]; out[i][j][3] = acc[j][3]; }
-      }
     }
-  }
+    if (ordinal + 1 < steps && q + 1 < end) continue;
+    // the run leaves these columns: each warp turns its 32 columns through shared memory and writes them
+    const int col0 = q / steps * kCols;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int col = warp * 32 + j * 8 + 2 * t;
-    float b0 = 0.0f, b1 = 0.0f;
-    if (p.bias) {
-      if (col0 + col < p.n) {
+    for (int j = 0; j < 4; ++j) {
+      const int col = warp * 32 + j * 8 + 2 * t;
+      float b0 = 0.0f, b1 = 0.0f;
+      if (p.bias && col0 + col < p.n) {
         b0 = __bfloat162float(p.bias[col0 + col]);
         b1 = __bfloat162float(p.bias[col0 + col + 1]);
       }
-    }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      *reinterpret_cast<uint32_t*>(staging + (i * 16 + g) * kPitch + col * 2) = pack_bf16x2(out[i][j][0] + b0, out[i][j][1] + b1);
-      *reinterpret_cast<uint32_t*>(staging + (i * 16 + g + 8) * kPitch + col * 2) = pack_bf16x2(out[i][j][2] + b0, out[i][j][3] + b1);
+      for (int i = 0; i < 4; ++i) {
+        *reinterpret_cast<uint32_t*>(staging + (i * 16 + g) * kPitch + col * 2) = pack_bf16x2(out[i][j][0] + b0, out[i][j][1] + b1);
+        *reinterpret_cast<uint32_t*>(staging + (i * 16 + g + 8) * kPitch + col * 2) = pack_bf16x2(out[i][j][2] + b0, out[i][j][3] + b1);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[i][j][e] = 0.0f;
+      }
     }
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < rows * (kCols / 8); i += kCols) {
-    const int r = i / (kCols / 8), c = (i % (kCols / 8)) * 8;
-    if (col0 + c < p.n && mine[r])
-      *reinterpret_cast<uint4*>(p.delta + static_cast<long long>(row0 + r) * p.n + col0 + c) = *reinterpret_cast<const uint4*>(staging + r * kPitch + c * 2);
+    __syncwarp();
+    const int c = warp * 32 + (lane & 3) * 8;
+    if (col0 + c < p.n)
+#pragma unroll
+      for (int r = lane >> 2; r < kExpandRows; r += 8)
+        if (r < rows && place[r] >= from && place[r] <= ordinal)
+          *reinterpret_cast<uint4*>(p.delta + static_cast<long long>(row0 + r) * p.n + col0 + c) =
+              *reinterpret_cast<const uint4*>(staging + r * kPitch + c * 2);
+    __syncwarp();
+    from = 0;
   }
   if (!ok && threadIdx.x == 0) {       // as in the kernel above
-    if (adapters) mbar_wait(smem_u32(&t_full), 0, 0xA23);
-    for (int ordinal = max(0, adapters - kSlabs); ordinal < adapters; ++ordinal)
-      mbar_wait(smem_u32(full + ordinal % kSlabs), (ordinal / kSlabs) & 1u, 0xA23);
+    mbar_wait(smem_u32(&t_full), 0, 0xA23);
+    for (int q = max(begin, end - kSlabs); q < end; ++q)
+      mbar_wait(smem_u32(full + (q - begin) % kSlabs), ((q - begin) / kSlabs) & 1u, 0xA23);
   }
 }
 
@@ -404,12 +416,12 @@ int launch_expand(const AdapterParams& p, int sm_count, cudaStream_t stream) {
   constexpr int kBox = kRank < 64 ? kRank : 64;
   if (int rc = make_tensor_map_3d(&map_t, p.t, 2, kRank, p.m, 1, kRank * 2, kRank * 2ull * p.m, kBox, kExpandRows, 1, kBox * 2)) return rc;
   if (int rc = make_tensor_map_3d(&map_up, p.up, 2, p.n, p.rank, p.count, p.ld_up * 2, p.stride_up * 2, 64, kRank, 1, 128)) return rc;
-  const dim3 tiles((p.n + kCols - 1) / kCols, (p.m + kExpandRows - 1) / kExpandRows);
-  // blocks that share a tile's adapters, while there are SMs without one
-  unsigned share = 1;
-  if (kCols == 256)
-    while (share < 8 && share * 2 <= unsigned(min(p.count, kExpandRows)) && tiles.x * tiles.y * share * 2 <= unsigned(2 * sm_count)) share *= 2;
-  KernelLaunch launch(dim3(tiles.x, tiles.y, share), dim3(kCols), kSmem, stream);
+  // as many blocks as are resident together, an equal number for every tile of rows
+  const int tiles = (p.m + kExpandRows - 1) / kExpandRows, columns = (p.n + kCols - 1) / kCols;
+  const int resident = sm_count * min(kCols == 128 ? 4 : 2, 227 * 1024 / (kSmem + 2048));
+  const long long slabs = static_cast<long long>(columns) * min(p.count, min(kExpandRows, p.m));
+  const int blocks = int(max(1ll, min(slabs, static_cast<long long>(resident / tiles))));
+  KernelLaunch launch(dim3(blocks, tiles), dim3(kCols), kSmem, stream);
   cudaError_t e = cudaLaunchKernelEx(&launch.config, kernel, map_t, map_up, p);
   if (e != cudaSuccess) return fail(TRINITY_SM100_E_CUDA, "adapter_expand launch: %s", cudaGetErrorString(e));
   count_launch();
