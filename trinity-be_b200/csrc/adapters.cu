@@ -237,7 +237,7 @@ __host__ __device__ constexpr int expand_smem_bytes() {
 // slab, the rows of the adapters that its run covered (rows without one go with the first adapter): every
 // element is written once.
 template <int kRank, int kCols>
-__global__ void __launch_bounds__(kCols)
+__global__ void __launch_bounds__(kCols, kCols == 128 ? 4 : 2)
 adapter_expand_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant__ CUtensorMap map_up,
                       const AdapterParams p) {
   constexpr int kRowT = kRank < 64 ? kRank * 2 : 128;
@@ -299,9 +299,14 @@ adapter_expand_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_co
 #pragma unroll
       for (int e = 0; e < 4; ++e) out[i][j][e] = 0.0f;
   int from = begin % steps;            // first adapter of the run on the present columns
-  for (int q = begin; q < end; ++q) {
-    const int s = (q - begin) % kSlabs, ordinal = q % steps;
-    if (adapters && ok) ok = mbar_wait(smem_u32(full + s), ((q - begin) / kSlabs) & 1u, 0xA22);
+  int columns = begin / steps, ordinal = from, s = 0;      // of slab q: its columns, adapter and stage
+  uint32_t parity = 0;
+  for (int q = begin; q < end; ++q, s = s + 1 == kSlabs ? 0 : s + 1, parity ^= s == 0 ? 1u : 0u) {
+    if (q != begin && ++ordinal == steps) {
+      ordinal = 0;
+      ++columns;
+    }
+    if (adapters && ok) ok = mbar_wait(smem_u32(full + s), parity, 0xA22);
     __syncthreads();                   // everyone is through with the slab before, which is filled again
     if (threadIdx.x == 0 && adapters && q + kSlabs - 1 < end) fetch(q + kSlabs - 1);
     if (adapters) {
@@ -312,6 +317,22 @@ adapter_expand_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_co
         if (i * 16 >= rows) break;
         const bool low = of_row[i * 16 + g] == adapter, high = of_row[i * 16 + g + 8] == adapter;
         if (!__any_sync(0xffffffffu, low || high)) continue;
+        if (__all_sync(0xffffffffu, low && high)) {      // sixteen rows of one adapter: no selection
+#pragma unroll
+          for (int k16 = 0; k16 < kRank; k16 += 16) {
+            uint32_t a[4];
+            load_matrices<false>(ts + k16 / 64 * kExpandRows * 128 +
+                                 swizzled((i * 16 + (lane & 15)) * kRowT + (k16 % 64 + (lane >> 4) * 8) * 2, kRowT), a);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              uint32_t b[4];
+              load_matrices<true>(slab + swizzled((k16 + (lane & 15)) * 128 + (warp % 2) * 64 + j * 32 + (lane >> 4) * 16, 128), b);
+              mma_bf16_16816(out[i][2 * j], a, b[0], b[1]);
+              mma_bf16_16816(out[i][2 * j + 1], a, b[2], b[3]);
+            }
+          }
+          continue;
+        }
         float acc[4][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -339,7 +360,7 @@ adapter_expand_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_co
     }
     if (ordinal + 1 < steps && q + 1 < end) continue;
     // the run leaves these columns: each warp turns its 32 columns through shared memory and writes them
-    const int col0 = q / steps * kCols;
+    const int col0 = columns * kCols;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int col = warp * 32 + j * 8 + 2 * t;
