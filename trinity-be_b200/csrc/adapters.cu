@@ -532,5 +532,11 @@ extern "C" int trinity_sm100_gemm_adapters_bf16(const trinity_sm100_gemm* gemm, 
   with_delta.bias = p.delta;
   with_delta.ld_bias = g.n;
   with_delta.bias_mode = TRINITY_SM100_BIAS_MATRIX;
-  return trinity_sm100_gemm_bf16(&with_delta, stream_handle);
+  // The expand kernel lets its successor start before it has waited itself, and it was started by the
+  // shrink kernel after everything before that one had completed: x and the weight may be read at
+  // once, so the GEMM begins beside the small kernels where an SM is free, and waits in its epilogue.
+  g_late_wait_for_next_launch = true;
+  const int launched = trinity_sm100_gemm_bf16(&with_delta, stream_handle);
+  g_late_wait_for_next_launch = false;
+  return launched;
 }

@@ -96,6 +96,9 @@ struct GemmParams {
   long long stride_bias;   // elements between the side operands of consecutive batch entries
   int split_rows;          // split form: accumulator rows a CTA hands to its cluster's first CTA (16, 32 or 64)
   int split_a_rows;        // split form: rows of A loaded per K block (32 or 64)
+  // The previous kernel of the stream produces the side operand only, and everything before that one had
+  // completed when it let this one start: the operands are read at once, only the epilogue waits.
+  int late_wait;
   void* out;               // split form: the output, which its epilogue stores without a tensor map
   long long ldo;           // ... and its row pitch in elements
 };
@@ -234,6 +237,9 @@ __device__ __forceinline__ bool reduce_owned_tile(const GemmParams& p, const Gem
   return true;
 }
 
+// Set by the adapters entry point around its call of the GEMM entry point (same thread).
+thread_local bool g_late_wait_for_next_launch = false;
+
 // (the split form leaves the epilogue loop of the other forms unreachable in its instantiations)
 #pragma nv_diag_suppress 128
 template <int kBN, int kStages, bool kGated, bool kOutF32, bool kFused = false, bool kBatched = false,
@@ -348,7 +354,7 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a,
     // and this one goes on once the previous kernel's results are visible.  (The form with the
     // cross-GPU sum is always launched the ordinary way.)
     grid_dependents_may_launch();
-    grid_dependency_wait();
+    if (!p.late_wait || warp >= 2) grid_dependency_wait();
   }
 
   if (warp == 0) {
@@ -1003,6 +1009,7 @@ int launch_gemm(const trinity_sm100_gemm& g, int sm_count, cudaStream_t stream, 
   p.flag_tiles = (p.tiles_m + 1) / 2 * 2 * p.tiles_n;
   p.split_rows = g.m <= 16 ? 16 : g.m <= 32 ? 32 : 64;
   p.split_a_rows = g.m <= 32 ? 32 : 64;
+  p.late_wait = g_late_wait_for_next_launch ? 1 : 0;
   p.out = g.out;
   p.ldo = g.ldo;
   GemmPeers peers = {};
