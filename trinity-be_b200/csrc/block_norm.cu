@@ -30,12 +30,13 @@ struct SeamParams {
   float eps, post_eps, residual_scale;
 };
 
-// kW consecutive elements as FP32 (one 16-byte load for eight BF16 values, two for FP32).
-// Rows are read once and leave the caches first; gain vectors (kStream false) serve every row.
+// kW consecutive elements as FP32 (one 16-byte load for eight BF16 values, two for FP32), `at` elements
+// behind the lane's first one.  Rows are read once and leave the caches first; gain vectors
+// (kStream false) serve every row.
 template <int kW, bool kF32, bool kStream = true>
-__device__ __forceinline__ void load_elements(const void* base, long long offset, float (&v)[kW]) {
+__device__ __forceinline__ void load_elements(const void* base, int at, float (&v)[kW]) {
   if (kF32) {
-    const float* p = static_cast<const float*>(base) + offset;
+    const float* p = static_cast<const float*>(base) + at;
     if (kW == 8) {
       const float4 a = __ldcs(reinterpret_cast<const float4*>(p));
       const float4 b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
@@ -45,7 +46,7 @@ __device__ __forceinline__ void load_elements(const void* base, long long offset
       v[0] = __ldcs(p);
     }
   } else {
-    const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(base) + offset;
+    const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(base) + at;
     if (kW == 8) {
       const uint4 a = kStream ? __ldcs(reinterpret_cast<const uint4*>(p)) : *reinterpret_cast<const uint4*>(p);
       const uint32_t w[4] = {a.x, a.y, a.z, a.w};
@@ -61,9 +62,9 @@ __device__ __forceinline__ void load_elements(const void* base, long long offset
 }
 
 template <int kW, bool kF32>
-__device__ __forceinline__ void store_elements(void* base, long long offset, const float (&v)[kW]) {
+__device__ __forceinline__ void store_elements(void* base, int at, const float (&v)[kW]) {
   if (kF32) {
-    float* p = static_cast<float*>(base) + offset;
+    float* p = static_cast<float*>(base) + at;
     if (kW == 8) {
       reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1 % kW], v[2 % kW], v[3 % kW]);
       reinterpret_cast<float4*>(p)[1] = make_float4(v[4 % kW], v[5 % kW], v[6 % kW], v[7 % kW]);
@@ -71,13 +72,19 @@ __device__ __forceinline__ void store_elements(void* base, long long offset, con
       p[0] = v[0];
     }
   } else {
-    __nv_bfloat16* p = static_cast<__nv_bfloat16*>(base) + offset;
+    __nv_bfloat16* p = static_cast<__nv_bfloat16*>(base) + at;
     if (kW == 8)
       *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1 % kW]), pack_bf16x2(v[2 % kW], v[3 % kW]),
                                                 pack_bf16x2(v[4 % kW], v[5 % kW]), pack_bf16x2(v[6 % kW], v[7 % kW]));
     else
       p[0] = __float2bfloat16(v[0]);
   }
+}
+
+template <bool kF32>
+__device__ __forceinline__ const void* element_of(const void* base, long long offset) {
+  return kF32 ? static_cast<const void*>(static_cast<const float*>(base) + offset)
+              : static_cast<const void*>(static_cast<const __nv_bfloat16*>(base) + offset);
 }
 
 // kW = 8: 16-byte accesses (every row of every operand starts on 16 bytes); kW = 1: any layout.
@@ -87,22 +94,26 @@ rmsnorm_residual_kernel(const SeamParams p) {
   constexpr int kBlock = kThreads > kRowBlock ? kThreads : kRowBlock;
   constexpr int kRowsPerCta = kBlock / kThreads;
   constexpr int kN = kSeamElements / kW;
+  constexpr int kStep = kThreads * kW;     // columns between a lane's pieces
   __shared__ float scratch[kBlock / 32];
   grid_dependents_may_launch();
   grid_dependency_wait();   // the previous kernel of the stream may have produced any operand
-  const int lane = threadIdx.x % kThreads;
+  const int col = threadIdx.x % kThreads * kW;       // of the lane's first piece
   const long long row = static_cast<long long>(blockIdx.x) * kRowsPerCta + threadIdx.x / kThreads;
-  const bool live_row = row < p.rows;
+  // columns from the lane's first on; a lane without a row has none
+  const int left = row < p.rows ? p.cols - col : 0;
+  const long long at_row = row < p.rows ? row : 0;
+  const void* x = element_of<kXF32>(p.x, at_row * p.ld_x + col);
+  const void* residual = element_of<kResF32>(p.residual, at_row * p.ld_residual + col);
   float h[kN][kW], r[kN][kW];
 #pragma unroll
   for (int i = 0; i < kN; ++i) {
-    const int col = (i * kThreads + lane) * kW;
-    if (live_row && col < p.cols) {
-      load_elements<kW, kXF32>(p.x, row * p.ld_x + col, h[i]);
-      load_elements<kW, kResF32>(p.residual, row * p.ld_residual + col, r[i]);
-    } else {
 #pragma unroll
-      for (int e = 0; e < kW; ++e) h[i][e] = r[i][e] = 0.0f;
+    for (int e = 0; e < kW; ++e) h[i][e] = r[i][e] = 0.0f;
+    if (i * kStep >= p.cols) continue;       // (for all lanes: pieces behind the row cost nothing)
+    if (i * kStep < left) {
+      load_elements<kW, kXF32>(x, i * kStep, h[i]);
+      load_elements<kW, kResF32>(residual, i * kStep, r[i]);
     }
   }
   if (p.post_norm) {
@@ -113,55 +124,53 @@ rmsnorm_residual_kernel(const SeamParams p) {
       for (int e = 0; e < kW; ++e) ss = fmaf(h[i][e], h[i][e], ss);
     ss = row_reduce<kThreads, false>(ss, scratch);
     const float inv = 1.0f / sqrtf(ss / static_cast<float>(p.cols) + p.post_eps);
+    const __nv_bfloat16* gain = p.post_gain + col;
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
-      const int col = (i * kThreads + lane) * kW;
+      if (i * kStep >= p.cols) continue;
       float g[kW];
 #pragma unroll
       for (int e = 0; e < kW; ++e) g[e] = 1.0f;
-      if (p.post_gain && live_row && col < p.cols) load_elements<kW, false, false>(p.post_gain, col, g);
+      if (p.post_gain && i * kStep < left) load_elements<kW, false, false>(gain, i * kStep, g);
 #pragma unroll
       for (int e = 0; e < kW; ++e) h[i][e] = h[i][e] * inv * g[e];
     }
   }
   float ss = 0.0f;
+  const __nv_bfloat16* gate = p.gate + at_row * p.gate_row + col * p.gate_col;
+  const float row_gate = p.gate && !p.gate_col ? __bfloat162float(*gate) : 1.0f;
+  void* residual_out = const_cast<void*>(element_of<kResF32>(p.residual_out, at_row * p.ld_residual_out + col));
 #pragma unroll
   for (int i = 0; i < kN; ++i) {
-    const int col = (i * kThreads + lane) * kW;
-    if (live_row && col < p.cols) {
-      if (p.gate) {
-        float g[kW];
-        if (p.gate_col) {
-          load_elements<kW, false, false>(p.gate, row * p.gate_row + col * p.gate_col, g);
-        } else {
-          const float one = __bfloat162float(p.gate[row * p.gate_row]);
+    if (i * kStep >= p.cols) continue;
+    if (i * kStep < left) {
+      float g[kW];
 #pragma unroll
-          for (int e = 0; e < kW; ++e) g[e] = one;
-        }
-#pragma unroll
-        for (int e = 0; e < kW; ++e) h[i][e] *= g[e];
-      }
+      for (int e = 0; e < kW; ++e) g[e] = row_gate;
+      if (p.gate && p.gate_col) load_elements<kW, false, false>(gate, i * kStep, g);
 #pragma unroll
       for (int e = 0; e < kW; ++e) {
-        h[i][e] = fmaf(p.residual_scale, r[i][e], h[i][e]);
+        h[i][e] = fmaf(p.residual_scale, r[i][e], h[i][e] * g[e]);
         ss = fmaf(h[i][e], h[i][e], ss);
       }
-      store_elements<kW, kResF32>(p.residual_out, row * p.ld_residual_out + col, h[i]);
+      store_elements<kW, kResF32>(residual_out, i * kStep, h[i]);
     }
   }
   ss = row_reduce<kThreads, false>(ss, scratch);
   const float inv = 1.0f / sqrtf(ss / static_cast<float>(p.cols) + p.eps);
+  const __nv_bfloat16* gain = p.gain + col;
+  __nv_bfloat16* out = p.out + at_row * p.ld_out + col;
 #pragma unroll
   for (int i = 0; i < kN; ++i) {
-    const int col = (i * kThreads + lane) * kW;
-    if (live_row && col < p.cols) {
+    if (i * kStep >= p.cols) continue;
+    if (i * kStep < left) {
       float g[kW];
 #pragma unroll
       for (int e = 0; e < kW; ++e) g[e] = 1.0f;
-      if (p.gain) load_elements<kW, false, false>(p.gain, col, g);
+      if (p.gain) load_elements<kW, false, false>(gain, i * kStep, g);
 #pragma unroll
       for (int e = 0; e < kW; ++e) g[e] *= h[i][e] * inv;
-      store_elements<kW, false>(p.out, row * p.ld_out + col, g);
+      store_elements<kW, false>(out, i * kStep, g);
     }
   }
 }
