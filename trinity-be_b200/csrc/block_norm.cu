@@ -5,17 +5,19 @@
 //   y = h / sqrt(mean(h^2) + eps) * gain            -> out
 //
 // Bound by memory: x, the residual and a full gate are read once, residual_out and out written
-// once.  A row is spread over kThreads lanes (32..1024) of 16 elements each; the lane keeps its
-// part of the row in registers through both sums, so nothing is read twice.  All arithmetic is
-// FP32; the two roundings are those of the two outputs (out is computed from the unrounded h).
+// once.  A row is spread over kThreads lanes (32..1024) of 16 elements each (8 where the layout
+// allows only one at a time); the lane keeps its part of the row in registers through both sums, so
+// nothing is read twice.  Warps in flight decide: with 16-byte accesses 48 warps an SM (40 registers
+// a thread) take 169 us for 32768 x 4096 BF16 (1074 MB, 0.97 of the measured copy rate), 36 warps
+// 184 us and 56 warps (spilling) 205 us.  All arithmetic is FP32; the two roundings are those of the
+// two outputs (out is computed from the unrounded h).
 #include "host_common.h"
 #include "sm100_ptx.cuh"
 
 namespace trinity_sm100 {
 namespace {
 
-constexpr int kSeamElements = 16;   // per lane
-constexpr int kSeamMaxCols = 1024 * kSeamElements;
+constexpr int kSeamMaxCols = 1024 * 16;
 
 struct SeamParams {
   const void* x;
@@ -88,12 +90,16 @@ __device__ __forceinline__ const void* element_of(const void* base, long long of
 }
 
 // kW = 8: 16-byte accesses (every row of every operand starts on 16 bytes); kW = 1: any layout.
-template <int kThreads, int kW, bool kXF32, bool kResF32>
-__global__ void __launch_bounds__(kThreads > kRowBlock ? kThreads : kRowBlock)
+// kElements a lane.
+// Threads an SM is to hold, which bounds the registers of each (see above; FP32 operands need more).
+template <int kW, bool kF32>
+constexpr int seam_resident() { return kW == 1 ? 2048 : kF32 ? 1024 : 1536; }
+template <int kThreads, int kW, int kElements, bool kXF32, bool kResF32>
+__global__ void __launch_bounds__(kThreads > kRowBlock ? kThreads : kRowBlock, (kElements > 8 && kW == 1 ? 1 : seam_resident<kW, kXF32 || kResF32>() / (kThreads > kRowBlock ? kThreads : kRowBlock)))
 rmsnorm_residual_kernel(const SeamParams p) {
   constexpr int kBlock = kThreads > kRowBlock ? kThreads : kRowBlock;
   constexpr int kRowsPerCta = kBlock / kThreads;
-  constexpr int kN = kSeamElements / kW;
+  constexpr int kN = kElements / kW;
   constexpr int kStep = kThreads * kW;     // columns between a lane's pieces
   __shared__ float scratch[kBlock / 32];
   grid_dependents_may_launch();
@@ -175,26 +181,26 @@ rmsnorm_residual_kernel(const SeamParams p) {
   }
 }
 
-template <int kThreads, int kW>
+template <int kThreads, int kW, int kElements>
 cudaError_t launch_seam(const SeamParams& p, bool x_f32, bool res_f32, cudaStream_t stream) {
   constexpr int block = kThreads > kRowBlock ? kThreads : kRowBlock;
   const unsigned grid = unsigned((p.rows + block / kThreads - 1) / (block / kThreads));
   KernelLaunch launch(dim3(grid), dim3(block), 0, stream);
   if (x_f32)
-    return res_f32 ? cudaLaunchKernelEx(&launch.config, rmsnorm_residual_kernel<kThreads, kW, true, true>, p)
-                   : cudaLaunchKernelEx(&launch.config, rmsnorm_residual_kernel<kThreads, kW, true, false>, p);
-  return res_f32 ? cudaLaunchKernelEx(&launch.config, rmsnorm_residual_kernel<kThreads, kW, false, true>, p)
-                 : cudaLaunchKernelEx(&launch.config, rmsnorm_residual_kernel<kThreads, kW, false, false>, p);
+    return res_f32 ? cudaLaunchKernelEx(&launch.config, rmsnorm_residual_kernel<kThreads, kW, kElements, true, true>, p)
+                   : cudaLaunchKernelEx(&launch.config, rmsnorm_residual_kernel<kThreads, kW, kElements, true, false>, p);
+  return res_f32 ? cudaLaunchKernelEx(&launch.config, rmsnorm_residual_kernel<kThreads, kW, kElements, false, true>, p)
+                 : cudaLaunchKernelEx(&launch.config, rmsnorm_residual_kernel<kThreads, kW, kElements, false, false>, p);
 }
 
-template <int kW>
+template <int kW, int kElements>
 cudaError_t launch_seam_width(const SeamParams& p, bool x_f32, bool res_f32, cudaStream_t stream) {
-  if (p.cols <= 32 * kSeamElements) return launch_seam<32, kW>(p, x_f32, res_f32, stream);
-  if (p.cols <= 64 * kSeamElements) return launch_seam<64, kW>(p, x_f32, res_f32, stream);
-  if (p.cols <= 128 * kSeamElements) return launch_seam<128, kW>(p, x_f32, res_f32, stream);
-  if (p.cols <= 256 * kSeamElements) return launch_seam<256, kW>(p, x_f32, res_f32, stream);
-  if (p.cols <= 512 * kSeamElements) return launch_seam<512, kW>(p, x_f32, res_f32, stream);
-  return launch_seam<1024, kW>(p, x_f32, res_f32, stream);
+  if (p.cols <= 32 * kElements) return launch_seam<32, kW, kElements>(p, x_f32, res_f32, stream);
+  if (p.cols <= 64 * kElements) return launch_seam<64, kW, kElements>(p, x_f32, res_f32, stream);
+  if (p.cols <= 128 * kElements) return launch_seam<128, kW, kElements>(p, x_f32, res_f32, stream);
+  if (p.cols <= 256 * kElements) return launch_seam<256, kW, kElements>(p, x_f32, res_f32, stream);
+  if (p.cols <= 512 * kElements) return launch_seam<512, kW, kElements>(p, x_f32, res_f32, stream);
+  return launch_seam<1024, kW, kElements>(p, x_f32, res_f32, stream);
 }
 
 }  // namespace
@@ -262,8 +268,9 @@ extern "C" int trinity_sm100_rmsnorm_residual(const trinity_sm100_rmsnorm_residu
                        (a.ld_residual_out * res_size) % 16 == 0 && a.ld_out % 8 == 0 &&
                        (a.gate_col_stride == 0 || !a.gate || (aligned16(a.gate) && a.gate_row_stride % 8 == 0));
   cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
-  const cudaError_t e = vectors ? launch_seam_width<8>(p, x_f32, res_f32, stream)
-                                : launch_seam_width<1>(p, x_f32, res_f32, stream);
+  const cudaError_t e = vectors             ? launch_seam_width<8, 16>(p, x_f32, res_f32, stream)
+                        : a.cols <= 8 * 1024 ? launch_seam_width<1, 8>(p, x_f32, res_f32, stream)
+                                             : launch_seam<1024, 1, 16>(p, x_f32, res_f32, stream);
   if (e != cudaSuccess) return fail(TRINITY_SM100_E_CUDA, "rmsnorm_residual launch: %s", cudaGetErrorString(e));
   count_launch();
   return check_launch("rmsnorm_residual");
