@@ -146,6 +146,20 @@ def test_batches(kernels, batch_lengths, heads, kv_heads):
     run_attend(kernels, batch_lengths, heads, kv_heads, 64, 64, 64, seed=3)
 
 
+def test_long_averages(kernels):
+    """Weights so even that the values average to almost nothing: what is left must not drown in sums that
+    cancel.  The output's rounding is at most half a step of 2^-7, uniformly spread: 2^-8 / sqrt(3) =
+    0.0023 in the mean square.  The rounding of weight times scale, 2^-11 / sqrt(3), reaches a
+    position's code minus 8, at most 8 steps of about 0.35 where its value is about 1: 0.0008.  Together 0.0024."""
+    table, pages, _ = ref.scattered_table([200000], 128, 1, 8)
+    cache = ref.filled_cache(kernels, pages, 1, 128, 128, 64, 8)
+    q = torch.randn((1, 8, 128), generator=torch.Generator(device=DEV).manual_seed(2), device=DEV).to(BF16)
+    lengths = torch.tensor([200000], dtype=torch.int32, device=DEV)
+    out = kernels.kv4_decode(q, cache, table, lengths, 0.01).double()
+    want, _, _ = ref.attend(q, cache, table, [200000], 0.01)
+    assert want.abs().mean() < 0.02 and (out - want).norm() <= 0.0024 * want.norm()
+
+
 @pytest.mark.parametrize("scale,spread", [(0.0, 1.0), (-0.1, 1.0), (3.0, 4.0), (0.088, 2.0 ** -60), (2.0 ** -40, 2.0 ** 40)])
 def test_scales(kernels, scale, spread):
     """Equal weights, a negative scale, weights concentrated on few positions, tiny and large caches."""

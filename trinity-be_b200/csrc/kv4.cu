@@ -250,8 +250,11 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Rows p) {
 // zeros are applied outside the products:
 // * keys: s = scale_k * (q . codes) + zero_k * (sum of q), per group, in FP32.  The query enters as
 //   FP16 times a power of two per head, exactly down to 2^-22 of its largest element.
-// * values: out = sum_t (p_t scale_v[t]) codes[t] + sum_t p_t zero_v[t], per group; the second sum is
-//   FP32.  p_t scale_v[t] enters as FP16 (2^-12, far below the output's rounding): p_t is at most 2^15
+// * values: out = sum_t (p_t scale_v[t]) (codes[t] - 8) + sum_t p_t (zero_v[t] + 8 scale_v[t]), per group;
+//   the second sum is FP32.  (Without the 8 both sums would be some 3 where the values average to 0: over
+//   262144 positions that cancellation cost 2.5 times the output's own rounding.  One product of the
+//   weights with a constant operand gives what the 8 takes off every channel; it is added to the
+//   accumulators every fourth tile.)  p_t scale_v[t] enters as FP16 (2^-12, far below the output's rounding): p_t is at most 2^15
 //   (see the maximum below) and scale_v is divided by a power of two, a running bound of the
 //   scales seen, which the accumulators follow like they follow the maximum.
 constexpr int kKv4Tile = 128;          // positions in a stage
@@ -599,6 +602,8 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     constexpr uint32_t kSubBytes = kKv4Warps * 16 * kRow;       // a multiple of 1024: the swizzle repeats
     const uint32_t matrix_offset = matrix_row ^ (((matrix_row >> 7) & 7) << 4);
     const int position0 = warp * 16 + g;                        // first row of the lane's scores
+    // -8 in the form of the codes, for even and odd channels
+    const uint32_t minus_eight[4] = {0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u};
     uint32_t it = 0;
     bool ok = true, last_cut = false;
     // The query rows of a piece are copied to shared memory while the piece before it is worked on.
@@ -701,6 +706,13 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           for (int i = 0; i < kNG; ++i) zeros[n][c][i] = 0.0f;
         }
       }
+      float shift[kNT][kNG][4];      // the -8's part of the accumulators, which takes it in every few tiles
+#pragma unroll
+      for (int n = 0; n < kNT; ++n)
+#pragma unroll
+        for (int i = 0; i < kNG; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) shift[n][i][e] = 0.0f;
       for (int tile = walk.first; tile < walk.first + walk.count; ++tile, ++it) {
         const int s = it % kStages;
         if (ok && it >= kKv4Lag && warp == int(it % kKv4Warps)) {
@@ -841,6 +853,11 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
                 for (int i = 0; i < kNG; ++i) zeros[n][c][i] *= f;
                 f *= rescale;
 #pragma unroll
+                for (int i = 0; i < kNG; ++i) {
+                  shift[n][i][c] *= f;
+                  shift[n][i][2 + c] *= f;
+                }
+#pragma unroll
                 for (int i = 0; i < kMT; ++i) {
                   acc[n][i][c] *= f;
                   acc[n][i][2 + c] *= f;
@@ -862,7 +879,8 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
             for (int i = 0; i < kNG; ++i)
 #pragma unroll
               for (int r = 0; r < 2; ++r) {
-                const float scale = bf16_lo(value_pair[u][r][i]) * inverse_limit, zero = bf16_hi(value_pair[u][r][i]);
+                const float scale = bf16_lo(value_pair[u][r][i]) * inverse_limit;
+              const float zero = fmaf(8.0f, bf16_lo(value_pair[u][r][i]), bf16_hi(value_pair[u][r][i]));
 #pragma unroll
                 for (int n = 0; n < kNT; ++n) {
                   const __half2 h = __floats2half2_rn(weight[n][2 * r] * scale, weight[n][2 * r + 1] * scale);
@@ -871,6 +889,10 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
                   for (int c = 0; c < 2; ++c) zeros[n][c][i] = fmaf(weight[n][2 * r + c], zero, zeros[n][c][i]);
                 }
               }
+#pragma unroll
+            for (int n = 0; n < kNT; ++n)
+#pragma unroll
+              for (int i = 0; i < kNG; ++i) mma_f16(shift[n][i], minus_eight, pf[n][i][0], pf[n][i][1]);
             // A chunk of 32 channels: lane (g, t) holds channels 4 g .. 4 g + 3 of positions 2 t, 2 t + 1 (and + 8);
             // two tiles of 16 channels, row g the even and row g + 8 the odd channel (16 times too large).
 #pragma unroll
@@ -890,6 +912,17 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
               }
             }
           }
+        }
+        if ((tile & 3) == 3 || tile + 1 == walk.first + walk.count) {
+#pragma unroll
+          for (int n = 0; n < kNT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+#pragma unroll
+              for (int i = 0; i < kMT; ++i) acc[n][i][e] += shift[n][i * kNG / kMT][e];
+#pragma unroll
+              for (int i = 0; i < kNG; ++i) shift[n][i][e] = 0.0f;
+            }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");    // page numbers or the next query, if this warp asked for any
         __syncwarp();
