@@ -389,7 +389,8 @@ typedef struct trinity_sm100_kv4_rows {
 /*
  * Writes BF16 rows into the cache at their slots.  A negative slot marks a token of a padded batch
  * that is not written; a slot behind the last page is not written either and sets the device status
- * word (0x901).  Slots of one call are distinct (of equal ones any may win, row by row).
+ * word (0x901).  Slots of one call must be distinct: a place that is named twice ends up with a
+ * mixture of both rows.
  */
 TRINITY_SM100_API int trinity_sm100_kv4_append(const trinity_sm100_kv4_cache* cache,
                                                const trinity_sm100_kv4_rows* rows, void* stream);
@@ -553,8 +554,9 @@ TRINITY_SM100_API int trinity_sm100_gemm_allreduce_workspace_bf16(const trinity_
 TRINITY_SM100_API int trinity_sm100_gemm_allreduce_stamps(uint64_t* stamps);
 
 /*
- * Device status word: 0 while every bounded in-kernel wait has completed; otherwise the code
- * of the first wait that gave up (site id in the low 16 bits).  Reading synchronises the
+ * Device status word: 0 while every bounded in-kernel wait has completed and every slot, page number
+ * and adapter index read on the device was valid; otherwise the code of the first wait that gave up,
+ * or of the first invalid one (site id in the low 16 bits: 0x901 to 0x903, 0xA01).  Reading synchronises the
  * device.  `clear` != 0 resets it afterwards.
  * Counterpart of the generated trinity_status() (src/emit/native/cuda/templates/host.cu.j2:78-83).
  */

@@ -64,7 +64,8 @@ def test_rows(changes, code):
     ({"q": None}, -1, "null"), ({"workspace": None}, -1, "null"), ({"batch": 0}, -1, "empty"), ({"max_pages": 0}, -1, "empty"),
     ({"heads": 7}, -1, "divide"), ({"table_stride": 3}, -1, "table"), ({"q": 5 * BASE + 2}, -1, "16 bytes"),
     ({"q_head_stride": 130}, -1, "16 bytes"), ({"out": 8 * BASE + 8}, -1, "aligned"), ({"lengths": 7 * BASE + 2}, -1, "aligned"),
-    ({"max_pages": 1 << 27, "table_stride": 1 << 27}, -2, "2^31")])
+    ({"max_pages": 1 << 27, "table_stride": 1 << 27}, -2, "2^31"),
+    ({"max_pages": 1 << 25, "table_stride": 1 << 25, "heads": 1 << 14}, -2, "too long")])
 def test_decode(changes, code, text):
     lib = k.library()
     assert lib.trinity_sm100_kv4_decode(ctypes.byref(cache()), ctypes.byref(decode(**changes)), None) == code

@@ -1271,6 +1271,11 @@ extern "C" int trinity_sm100_kv4_decode(const trinity_sm100_kv4_cache* cache, co
     return fail(TRINITY_SM100_E_INVALID, "kv4_decode: a pointer is not aligned to its element type");
   if (static_cast<long long>(a.max_pages) * c.page > INT32_MAX - kKv4Tile)
     return fail(TRINITY_SM100_E_UNSUPPORTED, "kv4_decode: a table row covers 2^31 positions or more");
+  const int group_heads = a.heads / c.kv_heads;
+  const int block_heads = group_heads > 8 ? 16 : 8, head_blocks = (group_heads + block_heads - 1) / block_heads;
+  if (((static_cast<long long>(a.max_pages) * c.page + kKv4Tile - 1) / kKv4Tile + kKv4RowUnits) * c.kv_heads * head_blocks > INT32_MAX)
+    return fail(TRINITY_SM100_E_UNSUPPORTED, "kv4_decode: a sequence of up to %lld positions is too long for %d heads",
+                static_cast<long long>(a.max_pages) * c.page, a.heads);
   int sm_count = 0;
   if (int rc = require_sm100(&sm_count)) return rc;
   const size_t need = trinity_sm100_kv4_decode_workspace_bytes(a.heads, c.kv_heads, c.head_dim);
@@ -1291,9 +1296,8 @@ extern "C" int trinity_sm100_kv4_decode(const trinity_sm100_kv4_cache* cache, co
   p.batch = a.batch;
   p.heads = a.heads;
   p.kv_heads = c.kv_heads;
-  p.group_heads = a.heads / c.kv_heads;
-  const int block_heads = p.group_heads > 8 ? 16 : 8;
-  p.head_blocks = (p.group_heads + block_heads - 1) / block_heads;
+  p.group_heads = group_heads;
+  p.head_blocks = head_blocks;
   p.pages = c.pages;
   p.page = c.page;
   p.max_pages = a.max_pages;
