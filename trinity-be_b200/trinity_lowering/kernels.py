@@ -637,20 +637,23 @@ class Kv4Cache:
     head_dim / group, 2] with (scale, zero) pairs.  ``kv4_cache`` makes an empty one."""
 
     def __init__(self, k_codes, k_scales, v_codes, v_scales):
-        if k_codes.dim() != 4 or k_scales.dim() != 5 or k_scales.shape[4] != 2:
+        codes, scales = k_codes.shape, k_scales.shape
+        if len(codes) != 4 or len(scales) != 5 or scales[4] != 2:
             raise ValueError("Kv4Cache: codes are [pages, kv_heads, page, head_dim / 2], "
                              "scales [pages, kv_heads, page, head_dim / group, 2]")
-        pages, kv_heads, page, half = k_codes.shape
-        groups = k_scales.shape[3]
-        if (k_scales.shape[:3] != k_codes.shape[:3] or v_codes.shape != k_codes.shape
-                or v_scales.shape != k_scales.shape or groups == 0 or (2 * half) % groups):
+        pages, kv_heads, page, half = codes
+        groups = scales[3]
+        if (scales[:3] != codes[:3] or v_codes.shape != codes or v_scales.shape != scales
+                or groups == 0 or (2 * half) % groups):
             raise ValueError("Kv4Cache: codes and scales disagree")
         index = k_codes.get_device()
-        for name, t, dtype in (("k_codes", k_codes, torch.uint8), ("v_codes", v_codes, torch.uint8),
-                               ("k_scales", k_scales, torch.bfloat16), ("v_scales", v_scales, torch.bfloat16)):
-            _operand(t, dtype, index, name)
-            if not t.is_contiguous():
-                raise ValueError(f"Kv4Cache: {name} must be contiguous")
+        _operand(k_codes, torch.uint8, index, "k_codes")
+        _operand(v_codes, torch.uint8, index, "v_codes")
+        _operand(k_scales, torch.bfloat16, index, "k_scales")
+        _operand(v_scales, torch.bfloat16, index, "v_scales")
+        if not (k_codes.is_contiguous() and v_codes.is_contiguous() and k_scales.is_contiguous()
+                and v_scales.is_contiguous()):
+            raise ValueError("Kv4Cache: the tensors must be contiguous")
         self.k_codes, self.k_scales, self.v_codes, self.v_scales = k_codes, k_scales, v_codes, v_scales
         self.pages, self.kv_heads, self.page = pages, kv_heads, page
         self.head_dim, self.group = 2 * half, 2 * half // groups
@@ -731,9 +734,16 @@ def kv4_read(cache, slots, *, dtype=torch.bfloat16, k_out=None, v_out=None, stre
     return _submit(cache.device, stream, (slots, k_out, v_out, *cache.tensors), launch)
 
 
+_kv4_workspaces = {}
+
+
 def kv4_decode_workspace_bytes(heads, kv_heads, head_dim):
     """Bytes of workspace that ``kv4_decode`` needs on the current device."""
-    return int(library().trinity_sm100_kv4_decode_workspace_bytes(heads, kv_heads, head_dim))
+    key = (torch._C._cuda_getDevice(), heads, kv_heads, head_dim)
+    size = _kv4_workspaces.get(key)
+    if size is None:
+        size = _kv4_workspaces[key] = int(library().trinity_sm100_kv4_decode_workspace_bytes(heads, kv_heads, head_dim))
+    return size
 
 
 def kv4_decode(q, cache, page_table, lengths, scale, *, out=None, lse=None, workspace=None, stream=None):
