@@ -312,27 +312,37 @@ adapter_expand_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_co
     if (adapters) {
       const uint32_t slab = us + s * kSlab + warp / 2 * kRank * 128;      // the half with this warp's columns
       const int adapter = distinct[ordinal];
+      uint32_t whole = 0;              // tiles of sixteen rows that are all this adapter's: no selection
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (i * 16 >= rows) break;
-        const bool low = of_row[i * 16 + g] == adapter, high = of_row[i * 16 + g + 8] == adapter;
-        if (!__any_sync(0xffffffffu, low || high)) continue;
-        if (__all_sync(0xffffffffu, low && high)) {      // sixteen rows of one adapter: no selection
+      for (int i = 0; i < 4; ++i)
+        if (__all_sync(0xffffffffu, of_row[i * 16 + g] == adapter && of_row[i * 16 + g + 8] == adapter)) whole |= 1u << i;
+      if (whole) {
 #pragma unroll
-          for (int k16 = 0; k16 < kRank; k16 += 16) {
+        for (int k16 = 0; k16 < kRank; k16 += 16) {
+          uint32_t b[2][4];
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            load_matrices<true>(slab + swizzled((k16 + (lane & 15)) * 128 + (warp % 2) * 64 + j * 32 + (lane >> 4) * 16, 128), b[j]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (!(whole >> i & 1u)) continue;
             uint32_t a[4];
             load_matrices<false>(ts + k16 / 64 * kExpandRows * 128 +
                                  swizzled((i * 16 + (lane & 15)) * kRowT + (k16 % 64 + (lane >> 4) * 8) * 2, kRowT), a);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              uint32_t b[4];
-              load_matrices<true>(slab + swizzled((k16 + (lane & 15)) * 128 + (warp % 2) * 64 + j * 32 + (lane >> 4) * 16, 128), b);
-              mma_bf16_16816(out[i][2 * j], a, b[0], b[1]);
-              mma_bf16_16816(out[i][2 * j + 1], a, b[2], b[3]);
+              mma_bf16_16816(out[i][2 * j], a, b[j][0], b[j][1]);
+              mma_bf16_16816(out[i][2 * j + 1], a, b[j][2], b[j][3]);
             }
           }
-          continue;
         }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i * 16 >= rows) break;
+        if (whole >> i & 1u) continue;
+        const bool low = of_row[i * 16 + g] == adapter, high = of_row[i * 16 + g + 8] == adapter;
+        if (!__any_sync(0xffffffffu, low || high)) continue;
         float acc[4][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
