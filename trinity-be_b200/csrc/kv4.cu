@@ -511,8 +511,6 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   auto full = [&](int s) { return bars + 8u * s; };
   auto empty = [&](int s) { return bars + 8u * (kStages + s); };
   __shared__ long long locate_scratch[kKv4Threads / 32 + 2];
-  __shared__ Kv4Walk ahead_state[kKv4Lag];
-  __shared__ int ahead_pages[kKv4Lag][kKv4Tile / 16];
   __shared__ uint32_t fetched[kStages];                    // tiles fetched into a stage so far
   static_assert(kStages > int(kKv4Lag), "a tile must be on its way before it is waited for");
 
@@ -535,12 +533,14 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 
   // ---------------------------------------------------------- refilling the ring
   // At tile i one warp, number i modulo the warps, fetches tile i - kKv4Lag + kStages once all warps are
-  // through with tile i - kKv4Lag.  What it needs for that (where the tile lies, its page numbers) lies in
-  // slot i modulo kKv4Lag of shared memory, written by the warp that fetched at tile i - kKv4Lag before
-  // it said that it was through with that tile: the wait that frees the stage also orders the slot.
-  // It then leaves in the slot the tile kKv4Lag further on and starts the copy of its page numbers,
-  // which has landed before it says that it is through with tile i.
-  auto issue = [&](const Kv4Walk& at, int s, const int* pages) {     // one warp: a tile's copies into stage s
+  // through with tile i - kKv4Lag.  Every warp walks its own every-fourth tile ahead and has loaded its
+  // page numbers (each lane that of its copy) since its last turn.
+  auto load_page = [&](const Kv4Walk& at) {       // page of this lane's piece of the tile, if it has one
+    const int piece = lane >> 2;
+    const int live = (min(kKv4Tile, at.length - at.tile * kKv4Tile) + p.box - 1) >> p.box_shift;
+    return piece < live ? p.table[at.b * p.table_stride + kv4_page_of(p, at.tile * kKv4Tile + (piece << p.box_shift))] : 0;
+  };
+  auto issue = [&](const Kv4Walk& at, int s, int page) {             // one warp: a tile's copies into stage s
     const int live = (min(kKv4Tile, at.length - at.tile * kKv4Tile) + p.box - 1) >> p.box_shift;
     if (lane == 0) {
       mbar_arrive_expect_tx(full(s), uint32_t(live << p.box_shift) * (2 * kRow + 8 * kNG));
@@ -548,49 +548,36 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     }
     __syncwarp();
     const uint32_t stage = base + s * kStage;
-    if (lane < live * 4) {
-      const int piece = lane >> 2, kind = lane & 3;
-      const int position = at.tile * kKv4Tile + (piece << p.box_shift), entry = kv4_page_of(p, position);
-      int page = pages ? pages[piece] : p.table[at.b * p.table_stride + entry];
+    const int piece = lane >> 2, kind = lane & 3;
+    if (piece < live) {
       if (page < 0 || page >= p.pages) {   // nothing outside the cache is read
         report_timeout(kSiteKv4Page);
         page = 0;
       }
-      const long long row = (static_cast<long long>(page) * p.kv_heads + at.kv) * p.page + (position - entry * p.page);
+      const int position = at.tile * kKv4Tile + (piece << p.box_shift);
+      // (the cache has fewer than 2^31 rows)
+      const int row = (page * p.kv_heads + at.kv) * p.page + (position - kv4_page_of(p, position) * p.page);
       if (kind < 2)
-        tma_load_3d(stage + kind * kCodes + piece * p.box * kRow, kind ? &map_v : &map_k, full(s), 0, int(row * kRow / 128), 0);
+        tma_load_3d(stage + kind * kCodes + piece * p.box * kRow, kind ? &map_v : &map_k, full(s), 0, row / (128 / kRow), 0);
       else
         bulk_load(stage + 2 * kCodes + (kind - 2) * kScales + piece * p.box * kNG * 4,
-                  (kind == 2 ? p.k_scales : p.v_scales) + row * kNG, uint32_t(p.box) * kNG * 4, full(s));
+                  (kind == 2 ? p.k_scales : p.v_scales) + static_cast<long long>(row) * kNG, uint32_t(p.box) * kNG * 4, full(s));
     }
   };
-  auto look_ahead = [&](const Kv4Walk& at, int slot) {     // one warp: leaves `at` in the slot as the tile to fetch next
-    __syncwarp();
-    if (lane == 0) ahead_state[slot] = at;
-    if (at.count > 0) {
-      const int live = (min(kKv4Tile, at.length - at.tile * kKv4Tile) + p.box - 1) >> p.box_shift;
-      if (lane < live)
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(&ahead_pages[slot][lane])),
-                     "l"(p.table + at.b * p.table_stride + kv4_page_of(p, at.tile * kKv4Tile + (lane << p.box_shift)))
-                     : "memory");
-    }
-  };
+  Kv4Walk ahead = walk;
+  bool ahead_some = ahead.step(p);
+  int ahead_page = 0;
   {
-    // the first tiles: every warp finds and fetches its own
-    Kv4Walk at = walk;
     int behind = 0;
-    bool some = at.step(p);
-    for (int s = warp; s < kStages && some; s += kKv4Warps) {
-      for (; behind < s && some; ++behind) some = at.next_tile(p);
-      if (some) issue(at, s, nullptr);
+    auto advance = [&](int tile) {
+      for (; behind < tile && ahead_some; ++behind) ahead_some = ahead.next_tile(p);
+    };
+    for (int s = warp; s < kStages; s += kKv4Warps) {        // the first tiles
+      advance(s);
+      if (ahead_some) issue(ahead, s, load_page(ahead));
     }
-    if (warp == 0) {
-      for (; behind < kStages && some; ++behind) some = at.next_tile(p);
-      for (int slot = 0; slot < int(kKv4Lag); ++slot) {
-        look_ahead(at, slot);
-        if (some) some = at.next_tile(p);
-      }
-    }
+    advance((warp >= int(kKv4Lag) ? warp : warp + kKv4Warps) - int(kKv4Lag) + kStages);
+    if (ahead_some) ahead_page = load_page(ahead);
   }
   {
     // ---------------------------------------------------------- attention
@@ -612,7 +599,7 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     const int position0 = warp * 16 + g;                        // first row of the lane's scores
     // -8 in the form of the codes, for even and odd channels
     const uint32_t minus_eight[4] = {0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u};
-    uint32_t it = 0;
+    uint32_t it = 0, stage = 0, parity = 0;     // of the next tile: its number, stage and round
     bool ok = true, last_cut = false;
     // The query rows of a piece are copied to shared memory while the piece before it is worked on.
     auto fetch_query = [&](const Kv4Walk& at) {
@@ -681,7 +668,7 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           query[warp][j][lane] = make_uint4(w[0], w[1], w[2], w[3]);
         }
         if (t == 0) {
-          factors[warp * 8 + g][0] = exp2f(static_cast<float>(-exponent)) * p.scale_log2;
+          factors[warp * 8 + g][0] = ldexpf(p.scale_log2, 24 - exponent);     // 2^24: the codes' unit
 #pragma unroll
           for (int i = 0; i < kNG; ++i) factors[warp * 8 + g][1 + i] = sums[i] * p.scale_log2;
         }
@@ -722,21 +709,23 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 #pragma unroll
           for (int e = 0; e < 4; ++e) shift[n][i][e] = 0.0f;
       for (int tile = walk.first; tile < walk.first + walk.count; ++tile, ++it) {
-        const int s = it % kStages;
         if (ok && it >= kKv4Lag && warp == int(it % kKv4Warps)) {
-          const uint32_t old = it - kKv4Lag;
-          ok = __all_sync(0xffffffffu, mbar_wait(empty(old % kStages), (old / kStages) & 1u, 0x911));
-          if (ok) {
-            Kv4Walk at = ahead_state[it % kKv4Lag];
-            if (at.count > 0) {
-              issue(at, old % kStages, ahead_pages[it % kKv4Lag]);
-              bool some = true;
-              for (uint32_t i = 0; i < kKv4Lag && some; ++i) some = at.next_tile(p);
-              look_ahead(at, it % kKv4Lag);
-            }
+          // the stage of tile it - kKv4Lag, in the round before this one's if it lies behind this one's stage
+          const bool wrapped = stage < kKv4Lag;
+          const uint32_t free = wrapped ? stage + kStages - kKv4Lag : stage - kKv4Lag;
+          ok = __all_sync(0xffffffffu, mbar_wait(empty(free), wrapped ? parity ^ 1u : parity, 0x911));
+          if (ok && ahead_some) {
+            issue(ahead, int(free), ahead_page);
+            for (int i = 0; i < kKv4Warps && ahead_some; ++i) ahead_some = ahead.next_tile(p);
+            if (ahead_some) ahead_page = load_page(ahead);
           }
         }
-        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(full(s), (it / kStages) & 1u, 0x912));
+        const uint32_t s = stage;
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(full(s), parity, 0x912));
+        if (++stage == kStages) {
+          stage = 0;
+          parity ^= 1u;
+        }
         const int live = walk.length - tile * kKv4Tile;     // positions of the tile that exist
         if (ok && warp * 16 < live) {
           const uint32_t keys = base + s * kStage, values = keys + kCodes;
@@ -793,7 +782,7 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
                     x = fmaf(dot[u][n][i][2 * r + c], bf16_lo(pair[i]), x);
                     z = fmaf(bf16_hi(pair[i]), zero_factor[n][c][i], z);
                   }
-                  score[u][n][2 * r + c] = fmaf(x * 0x1p24f, score_factor[n][c], z);
+                  score[u][n][2 * r + c] = fmaf(x, score_factor[n][c], z);
                 }
             }
           if (live < kKv4Tile) {
@@ -932,7 +921,7 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
               for (int i = 0; i < kNG; ++i) shift[n][i][e] = 0.0f;
             }
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");    // page numbers or the next query, if this warp asked for any
+        asm volatile("cp.async.wait_all;" ::: "memory");    // the next query, if this warp asked for it
         __syncwarp();
         if (lane == 0) mbar_arrive(empty(s));
       }
