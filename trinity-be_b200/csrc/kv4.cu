@@ -285,7 +285,11 @@ struct Kv4Attend {
   float* lse;
   // Workspace: of each block two parts (sums, then maximum and total), and the row it leaves unfinished.
   float* parts;          // [blocks][2][8 kNT heads][D], behind them [blocks][2][8 kNT heads][2]
-  int4* cuts;            // [blocks] {sequence, row in it, last block that holds a part, 1} or {.., 0}
+  // Rows whose parts are to be joined: {sequence, row in it, last block that holds a part, 1 + first block}, or
+  // {.., 0}: of every row while there are at most as many rows as blocks, else of the last row that
+  // each block begins.
+  int4* cuts;
+  int cuts_by_row;
   long long q_batch, q_head, table_stride;
   int batch, heads, kv_heads, group_heads, head_blocks, pages, page, max_pages, box, box_shift, page_shift;
   float scale_log2;
@@ -589,6 +593,9 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       if (p.lse)
         for (int i = threadIdx.x; i < p.heads; i += kKv4Threads)
           p.lse[static_cast<long long>(b) * p.heads + i] = -INFINITY;
+      if (p.cuts_by_row)
+        for (int i = threadIdx.x; i < p.kv_heads * p.head_blocks; i += kKv4Threads)
+          p.cuts[b * p.kv_heads * p.head_blocks + i] = make_int4(0, 0, 0, 0);
     }
     const int g = lane >> 2, t = lane & 3;
     // ldmatrix: lane l gives the address of row l & 7 of matrix l >> 3, which are (positions 0-7, 8-15) x
@@ -600,7 +607,8 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     // -8 in the form of the codes, for even and odd channels
     const uint32_t minus_eight[4] = {0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u};
     uint32_t it = 0, stage = 0, parity = 0;     // of the next tile: its number, stage and round
-    bool ok = true, last_cut = false;
+    bool ok = true;
+    int4 cut = make_int4(0, 0, 0, 0);
     // The query rows of a piece are copied to shared memory while the piece before it is worked on.
     auto fetch_query = [&](const Kv4Walk& at) {
       if (warp >= kNT) return;
@@ -927,7 +935,14 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       }
       // ---- the warps' parts of this piece meet, four heads (those of one accumulator column) at a time
       const bool whole = walk.count == walk.tiles;
-      last_cut = walk.first == 0 && !whole;
+      if (walk.first == 0) {
+        cut = make_int4(0, 0, 0, 0);
+        if (!whole) {
+          const long long row_end = walk.base + static_cast<long long>(walk.row + 1) * walk.units;
+          cut = make_int4(walk.b, walk.row, kv4_block_of(start.total, start.runs, row_end - 1), 1 + block);
+        }
+        if (threadIdx.x == 0 && p.cuts_by_row) p.cuts[walk.b * p.kv_heads * p.head_blocks + walk.row] = cut;
+      }
       const int slot = walk.first == 0 ? 1 : 0;   // part 0: the row began in an earlier block
 #pragma unroll
       for (int n = 0; n < kNT; ++n)
@@ -992,15 +1007,8 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         }
       // (the next piece writes the join area behind the barrier that follows its query)
     }
-    // The row that this run began and did not end, for the joining kernel.
-    if (threadIdx.x == 0) {
-      int4 cut = make_int4(0, 0, 0, 0);
-      if (last_cut) {
-        const long long row_end = walk.base + static_cast<long long>(walk.row + 1) * walk.units;
-        cut = make_int4(walk.b, walk.row, kv4_block_of(start.total, start.runs, row_end - 1), 1);
-      }
-      p.cuts[block] = cut;
-    }
+    // (a block that begins no row, or ends the last one that it begins, leaves nothing to join)
+    if (threadIdx.x == 0 && !p.cuts_by_row) p.cuts[block] = cut;
     // After a wait that gave up, nothing may still be in flight into this block's shared memory.
     if (__syncthreads_or(!ok))
       for (int s = 0; s < kStages; ++s)
@@ -1008,18 +1016,17 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   }
 }
 
-// Joins the parts of the row that block blockIdx.x began and did not end.  A warp takes one head and
+// Joins the parts of a row that was cut; one block an entry of `cuts`.  A warp takes one head and
 // every kGroups-th part, lanes the channels; the groups meet in shared memory, all in a fixed order.
-constexpr int kKv4JoinThreads = 1024;
-template <int kD, int kHeads>
-__global__ void __launch_bounds__(kKv4JoinThreads) kv4_join_kernel(const Kv4Attend p, int blocks) {
-  constexpr int kGroups = kKv4JoinThreads / 32 / kHeads, kPerLane = kD / 32;
+template <int kD, int kHeads, int kGroups>
+__global__ void __launch_bounds__(32 * kHeads * kGroups) kv4_join_kernel(const Kv4Attend p, int blocks) {
+  constexpr int kPerLane = kD / 32, kJoinThreads = 32 * kHeads * kGroups;
   __shared__ float sums[kGroups][kHeads][kD], ml_shared[kGroups][kHeads][2];
   grid_dependents_may_launch();
   grid_dependency_wait();
   const int4 cut = p.cuts[blockIdx.x];
   if (!cut.w) return;
-  const int first = blockIdx.x, last = cut.z;
+  const int first = cut.w - 1, last = cut.z;
   const int head = (threadIdx.x >> 5) % kHeads, group = (threadIdx.x >> 5) / kHeads, lane = threadIdx.x & 31;
   const float* parts_ml = p.parts + static_cast<long long>(blocks) * 2 * kHeads * kD;
   float m = -INFINITY, total = 0.0f, o[kPerLane];
@@ -1074,7 +1081,7 @@ __global__ void __launch_bounds__(kKv4JoinThreads) kv4_join_kernel(const Kv4Atte
   __syncthreads();
   const int kv = cut.y / p.head_blocks, hb = cut.y - kv * p.head_blocks;
   const int head0 = kv * p.group_heads + hb * kHeads;
-  for (int i = threadIdx.x; i < kHeads * kD; i += kKv4JoinThreads) {
+  for (int i = threadIdx.x; i < kHeads * kD; i += kJoinThreads) {
     const int h = i / kD, channel = i - h * kD;
     if (hb * kHeads + h >= p.group_heads) break;
     float top = -INFINITY, all = 0.0f, sum = 0.0f;
@@ -1165,8 +1172,14 @@ int launch_kv4_attend(const Kv4Attend& p, const CUtensorMap& map_k, const CUtens
     count_launch();
   }
   if (blocks > 1) {
-    KernelLaunch launch(dim3(blocks), dim3(kKv4JoinThreads), 0, stream);
-    cudaError_t e = cudaLaunchKernelEx(&launch.config, kv4_join_kernel<kD, 8 * kNT>, p, blocks);
+    // Few rows for many blocks: a row may have many parts, which four (or two) groups of warps share.  Else
+    // it has ten at most, and small blocks leave sooner.
+    const long long rows = static_cast<long long>(p.batch) * p.kv_heads * p.head_blocks;
+    constexpr int kManyGroups = kNT == 1 ? 4 : 2;
+    const bool many = rows * 8 < blocks;
+    KernelLaunch launch(dim3(p.cuts_by_row ? unsigned(rows) : unsigned(blocks)), dim3(32 * 8 * kNT * (many ? kManyGroups : 1)), 0, stream);
+    cudaError_t e = many ? cudaLaunchKernelEx(&launch.config, kv4_join_kernel<kD, 8 * kNT, kManyGroups>, p, blocks)
+                         : cudaLaunchKernelEx(&launch.config, kv4_join_kernel<kD, 8 * kNT, 1>, p, blocks);
     if (e != cudaSuccess) return fail(TRINITY_SM100_E_CUDA, "kv4_join launch: %s", cudaGetErrorString(e));
     count_launch();
   }
@@ -1309,6 +1322,7 @@ extern "C" int trinity_sm100_kv4_decode(const trinity_sm100_kv4_cache* cache, co
   if (int rc = make_tensor_map_3d(&map_k, c.k_codes, 2, 64, lines, 1, 128, 128 * lines, 64, box_lines, 1, 128)) return rc;
   if (int rc = make_tensor_map_3d(&map_v, c.v_codes, 2, 64, lines, 1, 128, 128 * lines, 64, box_lines, 1, 128)) return rc;
   const int blocks = kv4_blocks(sm_count, c.head_dim / c.group, block_heads);
+  p.cuts_by_row = static_cast<long long>(a.batch) * c.kv_heads * head_blocks <= blocks ? 1 : 0;
   p.cuts = reinterpret_cast<int4*>(p.parts + static_cast<size_t>(blocks) * 2 * block_heads * (c.head_dim + 2));
   cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
   const int groups = c.head_dim / c.group;
