@@ -260,11 +260,12 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Rows p) {
 //   (see the maximum below) and scale_v is divided by a power of two, a running bound of the
 //   scales seen, which the accumulators follow like they follow the maximum.
 //
-// Measured: 64 sequences x 4096 positions x 8 cached heads (287 MB) 77 us, 2 x 262144 with sixteen query
-// heads to a cached one (604 MB) 193 us, 200 sequences of 0 to 8191 positions 28 us, one of 1023 10 us.
-// Without the arithmetic the first takes 60, without the copies 64: what bounds it is the latency of a
-// warp's chain of products, exponentials and products at the twelve (eight) warps that the registers
-// allow.  Tiles of 64 positions (85 to 90 us) and four blocks an SM with two stages (84) were slower.
+// Measured: 64 sequences x 4096 positions x 8 cached heads (287 MB) 70 us, 2 x 262144 with sixteen query
+// heads to a cached one (604 MB) 189 us, 200 sequences of 0 to 8191 positions 27 us, one of 1023 9.8 us.
+// When the first took 77, it took 60 without the arithmetic and 64 without the copies: what bounds it is
+// the latency of a warp's chain of products, exponentials and products at the twelve (eight) warps that
+// the registers allow.  Tiles of 64 positions (85 to 90 us) and four blocks an SM with two stages (84)
+// were slower then.
 constexpr int kKv4Tile = 128;          // positions in a stage
 constexpr int kKv4Warps = 4;
 constexpr int kKv4Sub = kKv4Tile / (16 * kKv4Warps);   // groups of 16 positions a warp takes of each tile
