@@ -482,7 +482,7 @@ __host__ __device__ constexpr int kv4_query_bytes() {
 template <int kD, int kNG, int kNT>
 __host__ __device__ constexpr int kv4_stages() {
   // what a block's share of an SM's 228 KB leaves beside the system's 1 KB a block, static variables and alignment
-  return (228 * 1024 / kv4_per_sm(kNG, kNT) - 3072 - kv4_join_bytes<kD>() - kv4_query_bytes<kD, kNT>()) / kv4_stage_bytes<kD, kNG>();
+  return (228 * 1024 / kv4_per_sm(kNG, kNT) - 3 * 1024 - kv4_join_bytes<kD>() - kv4_query_bytes<kD, kNT>()) / kv4_stage_bytes<kD, kNG>();
 }
 template <int kD, int kNG, int kNT>
 __host__ __device__ constexpr int kv4_smem_bytes() {
