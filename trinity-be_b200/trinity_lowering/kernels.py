@@ -282,7 +282,9 @@ def _rows_ok(t):
 
 def _pitch(t):
     """Row pitch of a [rows, cols] tensor in elements (of no meaning when there is one row)."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    rows, cols = t.shape
+    pitch = t.stride(0)
+    return pitch if rows > 1 or pitch > cols else cols
 
 
 def _empty_rows(like, dtype):
@@ -421,17 +423,20 @@ def gemm_adapters(x, w, down, up, index, *, scales=None, bias=None, activation=A
     unless given; calls that may overlap need one each."""
     device = x.device
     at = x.get_device()
-    for name, t in (("x", x), ("w", w), ("down", down), ("up", up)):
-        _operand(t, torch.bfloat16, at, name)
+    _operand(x, torch.bfloat16, at, "x")
+    _operand(w, torch.bfloat16, at, "w")
+    _operand(down, torch.bfloat16, at, "down")
+    _operand(up, torch.bfloat16, at, "up")
     _operand(index, torch.int32, at, "index")
     if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[0] or not _rows_ok(x) or not _rows_ok(w):
         raise ValueError("gemm_adapters: x must be [m,k] and w [k,n], row-major with unit inner strides")
     m, k = x.shape
     n = w.shape[1]
-    if (down.dim() != 3 or up.dim() != 3 or down.shape[0] != up.shape[0] or down.shape[1] != k
-            or up.shape[2] != n or down.shape[2] != up.shape[1] or down.stride(2) != 1 or up.stride(2) != 1):
+    count, rank = down.shape[0], down.shape[-1]
+    down_strides, up_strides = down.stride(), up.stride()
+    if (down.shape != (count, k, rank) or up.shape != (count, rank, n) or down_strides[-1] != 1
+            or up_strides[-1] != 1):
         raise ValueError("gemm_adapters: down must be [adapters,k,rank] and up [adapters,rank,n], unit inner strides")
-    count, _, rank = down.shape
     if tuple(index.shape) != (m,) or not index.is_contiguous():
         raise ValueError("gemm_adapters: index must be [m]")
     if scales is not None:
@@ -462,8 +467,8 @@ def gemm_adapters(x, w, down, up, index, *, scales=None, bias=None, activation=A
                         DT_FP32 if out_dtype == torch.float32 else DT_BF16, 0)
         adapters = AdaptersArgs(down.data_ptr(), up.data_ptr(), index.data_ptr(),
                                 scales.data_ptr() if scales is not None else None, room.data_ptr(),
-                                room.numel() * room.element_size(), down.stride(1), down.stride(0),
-                                up.stride(1), up.stride(0), count, rank)
+                                room.numel() * room.element_size(), down_strides[1], down_strides[0],
+                                up_strides[1], up_strides[0], count, rank)
         _check(library().trinity_sm100_gemm_adapters_bf16(ctypes.byref(args), ctypes.byref(adapters), handle))
         return o
 
@@ -487,6 +492,18 @@ def rmsnorm(x, gain=None, eps=0.0, out=None, stream=None):
     return out
 
 
+def _gain_operand(t, cols, index, name):
+    _operand(t, torch.bfloat16, index, name)
+    if t.shape != (cols,) or not t.is_contiguous():
+        raise ValueError(f"rmsnorm_residual: {name} must be [cols]")
+
+
+def _rows_operand(t, dtype, shape, index, name):
+    _operand(t, dtype, index, name)
+    if t.shape != shape or not _rows_ok(t):
+        raise ValueError(f"rmsnorm_residual: {name} must be [rows, cols] with a unit inner stride")
+
+
 def rmsnorm_residual(x, residual, *, gain=None, post_gain=None, post_norm=None, gate=None, residual_scale=1.0,
                      eps=0.0, post_eps=None, residual_out=None, out=None, stream=None):
     """The seam between two blocks: ``(h, y)`` with ``h = residual_scale * residual + gate * b`` and
@@ -505,11 +522,10 @@ def rmsnorm_residual(x, residual, *, gain=None, post_gain=None, post_norm=None, 
     if residual.shape != shape or not _rows_ok(x) or not _rows_ok(residual):
         raise ValueError("rmsnorm_residual: x and residual must be [rows, cols] with a unit inner stride")
     rows, cols = shape
-    for name, t in (("gain", gain), ("post_gain", post_gain)):
-        if t is not None:
-            _operand(t, torch.bfloat16, index, name)
-            if t.shape != (cols,) or not t.is_contiguous():
-                raise ValueError(f"rmsnorm_residual: {name} must be [cols]")
+    if gain is not None:
+        _gain_operand(gain, cols, index, "gain")
+    if post_gain is not None:
+        _gain_operand(post_gain, cols, index, "post_gain")
     if post_norm is None:
         post_norm = post_gain is not None
     elif not post_norm and post_gain is not None:
@@ -530,19 +546,24 @@ def rmsnorm_residual(x, residual, *, gain=None, post_gain=None, post_norm=None, 
         if col_stride not in (0, 1):
             raise ValueError("rmsnorm_residual: gate must have an inner stride of 0 or 1")
         gate_pointer = gate.data_ptr()
-    for name, t, dtype in (("residual_out", residual_out, residual.dtype), ("out", out, torch.bfloat16)):
-        if t is not None:
-            _operand(t, dtype, index, name)
-            if t.shape != shape or not _rows_ok(t):
-                raise ValueError(f"rmsnorm_residual: {name} must be [rows, cols] with a unit inner stride")
+    if residual_out is not None:
+        _rows_operand(residual_out, residual.dtype, shape, index, "residual_out")
+    if out is not None:
+        _rows_operand(out, torch.bfloat16, shape, index, "out")
 
     def launch(handle):
-        h = _empty_rows(residual, residual.dtype) if residual_out is None else residual_out
-        y = _empty_rows(x, torch.bfloat16) if out is None else out
+        if residual_out is None:
+            h, h_pitch = _empty_rows(residual, residual.dtype), cols
+        else:
+            h, h_pitch = residual_out, _pitch(residual_out)
+        if out is None:
+            y, y_pitch = _empty_rows(x, torch.bfloat16), cols
+        else:
+            y, y_pitch = out, _pitch(out)
         args = RmsnormResidualArgs(
             x.data_ptr(), residual.data_ptr(), gate_pointer, None if gain is None else gain.data_ptr(),
             None if post_gain is None else post_gain.data_ptr(), h.data_ptr(), y.data_ptr(), rows, cols,
-            _pitch(x), _pitch(residual), _pitch(h), _pitch(y), row_stride, col_stride, x_dtype, residual_dtype,
+            _pitch(x), _pitch(residual), h_pitch, y_pitch, row_stride, col_stride, x_dtype, residual_dtype,
             bool(post_norm), eps, eps if post_eps is None else post_eps, residual_scale)
         _check(library().trinity_sm100_rmsnorm_residual(ctypes.byref(args), handle))
         return h, y
