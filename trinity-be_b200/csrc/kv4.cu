@@ -949,6 +949,7 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       for (int n = 0; n < kNT; ++n)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
+          if (8 * n + c >= heads_here) continue;      // (for all threads: no head of the row is in this round)
           if (n | c) __syncthreads();
 #pragma unroll
           for (int o = 4; o < 32; o *= 2) sum[n][c] += __shfl_xor_sync(0xffffffffu, sum[n][c], o);
