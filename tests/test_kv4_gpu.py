@@ -66,6 +66,44 @@ def test_append_of_views(kernels, pitch, offset):
     check_cache(kernels, cache, k, v, slots, 64)
 
 
+@pytest.mark.parametrize("pad", [0, 8, 1])
+@pytest.mark.parametrize("head_dim,group", [(128, 128), (128, 64), (128, 32), (64, 64), (64, 32)])
+def test_many_rows(kernels, head_dim, group, pad):
+    """Enough rows to fill the GPU, which start on 32, 16 or 2 bytes; some of them are padding, some lie outside."""
+    kv_heads, page, tokens = 3, 48, 331000 // (3 * head_dim // 8)
+    wide = rows(tokens, 2 * kv_heads, head_dim + pad, 21)
+    wide[7, :, 5] = float("nan")
+    wide[9] *= 2.0 ** -125                         # scales that are divided by, and subnormal values
+    wide[11, :, 40] = float("inf")
+    k, v = wide[:, :kv_heads, pad:], wide[:, kv_heads:, pad:]
+    pages = tokens // page + 2
+    cache = kernels.kv4_cache(pages, kv_heads, page, head_dim, group, DEV)
+    slots = torch.randperm(pages * page, device=DEV)[:tokens]
+    left_out = torch.arange(tokens, device=DEV) % 7 == 3
+    slots[left_out] = -1
+    kernels.kv4_append(cache, k, v, slots)
+    check_cache(kernels, cache, k[~left_out], v[~left_out], slots[~left_out], group)
+    written = torch.zeros(pages * page, dtype=torch.bool, device=DEV)
+    written[slots[~left_out]] = True
+    for t in cache.tensors:
+        assert (t.transpose(1, 2).flatten(0, 1)[~written] == 0).all()
+    room = 8 if pad else 0                         # outputs inside wider rows that start on 16 bytes
+    for dtype in (BF16, torch.float32):
+        outs = [torch.full((tokens, kv_heads, head_dim + room), 7.0, dtype=dtype, device=DEV) for _ in range(2)]
+        kernels.kv4_read(cache, slots, dtype=dtype, k_out=outs[0][..., room:], v_out=outs[1][..., room:])
+        whole = kernels.kv4_read(cache, slots.abs(), dtype=dtype)
+        for out, other in zip(outs, whole):
+            assert (out[left_out][..., room:] == 0).all() and (out[..., :room] == 7).all()
+            assert same(out[~left_out][..., room:], other[~left_out])
+    assert kernels.device_status() == 0
+    slots[-1], slots[100] = pages * page, 2 ** 40
+    before = [t.clone() for t in cache.tensors]
+    kernels.kv4_append(cache, v, k, torch.where(slots < pages * page, -1, slots))
+    torch.cuda.synchronize()
+    assert kernels.device_status(clear=True) & 0xffff == 0x901
+    assert all(same(a, b) for a, b in zip(before, cache.tensors))
+
+
 def test_padding_and_slots_outside(kernels):
     k, v = rows(6, 2, 64, 7), rows(6, 2, 64, 8)
     cache = kernels.kv4_cache(2, 2, 16, 64, 32, DEV)

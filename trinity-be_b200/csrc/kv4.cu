@@ -24,10 +24,11 @@ constexpr uint32_t kSiteKv4Page = 0x903;
 // ---------------------------------------------------------------- append and read
 //
 // Bound by memory: 2 D bytes read and D / 2 + 4 D / group written per row (append).  A lane owns
-// eight channels (one 16-byte access, one 32-bit word of codes), D / 8 lanes a row, keys and
-// values in one launch; a group's extrema meet by shuffles within its 4, 8 or 16 lanes.  32771 tokens x 8
-// heads x 128 channels in groups of 32, written and read back: 84 us for 352.6 MB (0.64 of the measured
-// copy rate; instruction issue is what is left).  One token of 64 sequences: 3.2 us for both.
+// sixteen channels (one 32-byte access, two 32-bit words of codes) or eight, with keys and values in
+// one launch; a group's extrema meet by shuffles within its 2 to 16 lanes.  32771 tokens x 8 heads x
+// 128 channels in groups of 32, written and read back: 62 us for 352.6 MB (append 32.1, read 28.9: 0.84 and
+// 0.93 of the measured copy rate; with eight channels a lane and single FP32 arithmetic instruction
+// issue took 84).  One token of 64 sequences: 3.2 us for both.
 struct Kv4Rows {
   const __nv_bfloat16* in[2];      // append: keys, values
   void* out[2];                    // read: keys, values
@@ -42,9 +43,14 @@ struct Kv4Rows {
 };
 
 // Row of the cache that holds head `head` of position `slot` (the cache has fewer than 2^31 rows).
-__device__ __forceinline__ long long kv4_row(const Kv4Rows& p, uint32_t slot, uint32_t head) {
+__device__ __forceinline__ uint32_t kv4_row(const Kv4Rows& p, uint32_t slot, uint32_t head) {
   const uint32_t page = p.page_shift >= 0 ? slot >> p.page_shift : slot / uint32_t(p.page);
-  return static_cast<long long>((page * p.kv_heads + head) * p.page + (slot - page * p.page));
+  return (page * p.kv_heads + head) * p.page + (slot - page * p.page);
+}
+// Index of the (scale, zero) of a row's channel.
+template <int kD>
+__device__ __forceinline__ uint64_t kv4_pair(const Kv4Rows& p, uint32_t row, int channel) {
+  return static_cast<uint64_t>(row) * uint32_t(kD >> p.group_shift) + (channel >> p.group_shift);
 }
 // The kBatch rows (token, head) of a group of kLanes lanes, a block's rows apart; the launcher keeps
 // all lanes of a launch below 2^31.  All loads of a step are issued before the first use.
@@ -60,7 +66,7 @@ struct Kv4Batch {
       const uint32_t index = (blockIdx.x * kBatch + i) * kRows + threadIdx.x / kLanes;
       token[i] = p.heads_shift >= 0 ? index >> p.heads_shift : index / uint32_t(p.kv_heads);
       head[i] = index - token[i] * p.kv_heads;
-      live[i] = token[i] < p.tokens;
+      live[i] = token[i] < uint32_t(p.tokens);
       slot[i] = live[i] ? p.slots[token[i]] : -1;
     }
   }
@@ -69,10 +75,15 @@ struct Kv4Batch {
   }
 };
 
-// Larger of each pair of BF16 values; NaN if either is.
+// Larger, or smaller, of each pair of BF16 values; NaN if either is.
 __device__ __forceinline__ uint32_t nan_max2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t nan_min2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
 __device__ __forceinline__ float reciprocal_approx(float x) {   // 2^-23 relative
@@ -87,36 +98,102 @@ __device__ __noinline__ uint32_t divided_code(float x, float scale) {
 }
 __device__ __noinline__ float divided_spread(float spread) { return spread / 15.0f; }
 
-template <int kD, bool kVector, int kBatch>
-__global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4Rows p) {
-  constexpr int kLanes = kD / 8;
+// Two FP32 numbers an instruction (each rounded as the single ones are).
+__device__ __forceinline__ uint64_t pair_f32(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 halves_f32(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint32_t add_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+
+// 16 or 32 bytes that are not read or written again soon.
+template <int kCount>
+__device__ __forceinline__ void load_once(const void* p, uint32_t (&w)[kCount]) {
+  static_assert(kCount == 4 || kCount == 8, "");
+  if constexpr (kCount == 4)
+    asm volatile("ld.global.cs.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p));
+  else
+    asm volatile("ld.global.cs.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                 : "l"(p));
+}
+template <int kCount>
+__device__ __forceinline__ void store_once(void* p, const uint32_t (&w)[kCount]) {
+  static_assert(kCount == 4 || kCount == 8, "");
+  if constexpr (kCount == 4)
+    asm volatile("st.global.cs.v4.b32 [%4], {%0, %1, %2, %3};" ::"r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "l"(p) : "memory");
+  else
+    asm volatile("st.global.cs.v8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                 "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]), "l"(p)
+                 : "memory");
+}
+
+// Five blocks of sixteen channels a lane an SM: 32.1 us at the size above; four 35.4, six (spilling) 32.4.
+template <int kD, int kWords, bool kVector, int kBatch>
+__global__ void __launch_bounds__(256, kWords == 2 ? 5 : 1) kv4_append_kernel(const Kv4Rows p) {
+  constexpr int kChannels = 8 * kWords, kLanes = kD / kChannels;
   grid_dependents_may_launch();
   grid_dependency_wait();
   const int which = blockIdx.y, lane = threadIdx.x % kLanes;
   const Kv4Batch<kLanes, kBatch> rows(p);
-  uint4 raw[kBatch];
+  uint32_t raw[kBatch][4 * kWords];
 #pragma unroll
   for (int i = 0; i < kBatch; ++i) {
-    const __nv_bfloat16* src = p.in[which] + rows.offset(p, which, i) + lane * 8;
-    raw[i] = make_uint4(0, 0, 0, 0);
+    const __nv_bfloat16* src = p.in[which] + rows.offset(p, which, i) + lane * kChannels;
+#pragma unroll
+    for (int e = 0; e < 4 * kWords; ++e) raw[i][e] = 0;
     if (!rows.live[i]) continue;
-    if (kVector) {
-      raw[i] = __ldcs(reinterpret_cast<const uint4*>(src));
+    if constexpr (kVector) {
+      load_once(src, raw[i]);
     } else {
       const uint16_t* one = reinterpret_cast<const uint16_t*>(src);
-      raw[i] = make_uint4(one[0] | uint32_t(one[1]) << 16, one[2] | uint32_t(one[3]) << 16,
-                          one[4] | uint32_t(one[5]) << 16, one[6] | uint32_t(one[7]) << 16);
+#pragma unroll
+      for (int e = 0; e < 4 * kWords; ++e) raw[i][e] = one[2 * e] | uint32_t(one[2 * e + 1]) << 16;
     }
   }
+  const int group_lanes = 1 << p.group_shift >> (kWords == 2 ? 4 : 3);
 #pragma unroll
   for (int i = 0; i < kBatch; ++i) {      // (the shuffles need every lane of the warp, rows or not)
-    const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+    const uint32_t(&w)[4 * kWords] = raw[i];
     // (max, -min) of the group as a BF16 pair; a NaN goes through, an infinity stays one
-    uint32_t extrema = nan_max2(nan_max2(w[0], w[1]), nan_max2(w[2], w[3]));
-    const uint32_t negated = nan_max2(nan_max2(w[0] ^ 0x80008000u, w[1] ^ 0x80008000u),
-                                      nan_max2(w[2] ^ 0x80008000u, w[3] ^ 0x80008000u));
+    uint32_t extrema = w[0], smallest = w[0];
+#pragma unroll
+    for (int e = 1; e < 4 * kWords; ++e) {
+      extrema = nan_max2(extrema, w[e]);
+      smallest = nan_min2(smallest, w[e]);
+    }
+    const uint32_t negated = smallest ^ 0x80008000u;
     extrema = nan_max2(__byte_perm(extrema, negated, 0x5410), __byte_perm(extrema, negated, 0x7632));
-    for (int step = 1; step < 1 << (p.group_shift - 3); step *= 2)     // the lanes of a group are neighbours
+    for (int step = 1; step < group_lanes; step *= 2)     // the lanes of a group are neighbours
       extrema = nan_max2(extrema, __shfl_xor_sync(0xffffffffu, extrema, step));
     const float high = bf16_lo(extrema), low = -bf16_hi(extrema), spread = high - low;
     // spread / 15, correctly rounded: a product with 1 / 15 and one Newton step (the remainder is exact
@@ -126,68 +203,89 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4Rows p) {
     if (!(spread > 0x1p-90f)) fifteenth = divided_spread(spread);
     const __nv_bfloat16 scale16 = __float2bfloat16(spread < INFINITY ? fifteenth : NAN);
     const float scale = __bfloat162float(scale16);
-    float v[8];
+    uint64_t v[4 * kWords];                        // pairs of x - zero
+    const uint64_t minus_low = pair_f32(-low, -low);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      v[2 * e] = bf16_lo(w[e]) - low;
-      v[2 * e + 1] = bf16_hi(w[e]) - low;
-    }
+    for (int e = 0; e < 4 * kWords; ++e) v[e] = add_f32x2(pair_f32(bf16_lo(w[e]), bf16_hi(w[e])), minus_low);
     // code = rint((x - zero) / scale), at most 15.06 before rounding as the scale is rounded by 2^-8 at
     // most.  BF16 values and scales are so coarse that half of all warps meet a quotient of exactly k + 1/2,
     // so the quotient must be the correctly rounded one: the product with the correctly rounded
     // reciprocal, corrected once by its exact remainder (Markstein's division; an 8-bit divisor is
     // none of its exceptions).
-    uint32_t codes = 0;
+    uint32_t codes[kWords];
+#pragma unroll
+    for (int c = 0; c < kWords; ++c) codes[c] = 0;
     if (scale > 0x1p-100f) {
       constexpr float kInteger = 12582912.0f;      // 1.5 * 2^23: adding it rounds to an integer, half to even
       float inverse = reciprocal_approx(scale);
       inverse = fmaf(inverse, fmaf(-scale, inverse, 1.0f), inverse);
+      const uint64_t inverses = pair_f32(inverse, inverse), minus_scale = pair_f32(-scale, -scale);
+      const uint64_t integers = pair_f32(kInteger, kInteger);
 #pragma unroll
-      for (int e = 7; e >= 0; --e) {
-        float quotient = v[e] * inverse;
-        quotient = fmaf(fmaf(-quotient, scale, v[e]), inverse, quotient);
-        codes = codes * 16u + __float_as_uint(quotient + kInteger);   // the code in the last four bits
+      for (int e = 4 * kWords - 1; e >= 0; --e) {
+        uint64_t quotient = mul_f32x2(v[e], inverses);
+        quotient = fma_f32x2(fma_f32x2(quotient, minus_scale, v[e]), inverses, quotient);
+        const float2 sums = halves_f32(add_f32x2(quotient, integers));   // the codes in the last four bits
+        codes[e / 4] = codes[e / 4] * 16u + __float_as_uint(sums.y);
+        codes[e / 4] = codes[e / 4] * 16u + __float_as_uint(sums.x);
       }
-      codes -= 0x3f400000u;                        // what the exponents of the eight sums have added up to
+#pragma unroll
+      for (int c = 0; c < kWords; ++c) codes[c] -= 0x3f400000u;   // what the exponents of the eight sums have added up to
     } else if (scale > 0.0f) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) codes |= divided_code(v[e], scale) << (4 * e);
+      for (int e = 0; e < 4 * kWords; ++e) {
+        const float2 x = halves_f32(v[e]);
+        codes[e / 4] |= (divided_code(x.x, scale) | divided_code(x.y, scale) << 4) << (8 * (e % 4));
+      }
     }
     if (rows.slot[i] < 0) continue;
     if (rows.slot[i] >= p.positions) {
       report_timeout(kSiteKv4AppendSlot);
       continue;
     }
-    const long long row = kv4_row(p, uint32_t(rows.slot[i]), rows.head[i]);
-    reinterpret_cast<uint32_t*>(p.codes[which])[row * kLanes + lane] = codes;
-    if ((lane & ((1 << (p.group_shift - 3)) - 1)) == 0) {
+    const uint32_t row = kv4_row(p, uint32_t(rows.slot[i]), rows.head[i]);
+    uint32_t* dst = reinterpret_cast<uint32_t*>(p.codes[which]) + static_cast<uint64_t>(row) * (kD / 8) + lane * kWords;
+    if constexpr (kWords == 2)
+      *reinterpret_cast<uint2*>(dst) = make_uint2(codes[0], codes[1]);
+    else
+      *dst = codes[0];
+    if ((lane & (group_lanes - 1)) == 0) {
       __nv_bfloat162 pair;
       pair.x = scale16;
       pair.y = __float2bfloat16(low);
-      p.scales[which][row * (kD >> p.group_shift) + (lane * 8 >> p.group_shift)] = pair;
+      p.scales[which][kv4_pair<kD>(p, row, lane * kChannels)] = pair;
     }
   }
 }
 
-// The values that the codes at `slots` stand for, one rounding to the output type (the product
-// scale * code is exact in FP32).  A negative slot reads as zeros.
-template <int kD, int kBatch>
+// The values that the codes at `slots` stand for, rounded to the output type: BF16 in one fused
+// multiplication and addition, FP32 likewise (there the product is exact too).  A negative slot reads
+// as zeros.
+template <int kD, int kWords, int kBatch>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Rows p) {
-  constexpr int kLanes = kD / 8;
+  constexpr int kChannels = 8 * kWords, kLanes = kD / kChannels;
   grid_dependents_may_launch();
   grid_dependency_wait();
   const int which = blockIdx.y, lane = threadIdx.x % kLanes;
   const Kv4Batch<kLanes, kBatch> rows(p);
-  uint32_t codes[kBatch];
-  __nv_bfloat162 pair[kBatch];
+  uint32_t codes[kBatch][kWords];
+  uint32_t pair[kBatch];
 #pragma unroll
   for (int i = 0; i < kBatch; ++i) {
-    codes[i] = 0;
-    pair[i] = __floats2bfloat162_rn(0.0f, 0.0f);
+#pragma unroll
+    for (int c = 0; c < kWords; ++c) codes[i][c] = 0;
+    pair[i] = 0;
     if (rows.slot[i] >= 0 && rows.slot[i] < p.positions) {
-      const long long row = kv4_row(p, uint32_t(rows.slot[i]), rows.head[i]);
-      codes[i] = reinterpret_cast<const uint32_t*>(p.codes[which])[row * kLanes + lane];
-      pair[i] = p.scales[which][row * (kD >> p.group_shift) + (lane * 8 >> p.group_shift)];
+      const uint32_t row = kv4_row(p, uint32_t(rows.slot[i]), rows.head[i]);
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(p.codes[which]) + static_cast<uint64_t>(row) * (kD / 8) + lane * kWords;
+      if constexpr (kWords == 2) {
+        const uint2 both = *reinterpret_cast<const uint2*>(src);
+        codes[i][0] = both.x;
+        codes[i][1] = both.y;
+      } else {
+        codes[i][0] = *src;
+      }
+      pair[i] = reinterpret_cast<const uint32_t*>(p.scales[which])[kv4_pair<kD>(p, row, lane * kChannels)];
     } else if (rows.slot[i] >= 0) {
       report_timeout(kSiteKv4ReadSlot);
     }
@@ -195,25 +293,46 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Rows p) {
 #pragma unroll
   for (int i = 0; i < kBatch; ++i) {
     if (!rows.live[i]) continue;
-    const float scale = __bfloat162float(pair[i].x), zero = __bfloat162float(pair[i].y);
-    float v[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      // the code in the last mantissa bits of 2^23 (five of them reach without a shift)
-      constexpr float kInteger = 8388608.0f;
-      const int at = 4 * (e < 4 ? e : e - 4);
-      const uint32_t bits = ((e < 4 ? codes[i] : codes[i] >> 16) & (15u << at)) | __float_as_uint(kInteger);
-      v[e] = fmaf((__uint_as_float(bits) - kInteger) * (1.0f / (1 << at)), scale, zero);
-    }
-    const long long at = rows.offset(p, which, i) + lane * 8;
+    const long long at = rows.offset(p, which, i) + lane * kChannels;
     if (p.out_f32) {
-      float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out[which]) + at);
-      __stcs(dst, make_float4(v[0], v[1], v[2], v[3]));
-      __stcs(dst + 1, make_float4(v[4], v[5], v[6], v[7]));
+      const float scale = bf16_lo(pair[i]), zero = bf16_hi(pair[i]);
+#pragma unroll
+      for (int c = 0; c < kWords; ++c) {
+        uint32_t v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          // the code in the last mantissa bits of 2^23 (five of them reach without a shift); the scale
+          // times a power of two is exact, even at its smallest
+          constexpr float kInteger = 8388608.0f;
+          const int shift = 4 * (e < 4 ? e : e - 4);
+          const uint32_t bits = ((e < 4 ? codes[i][c] : codes[i][c] >> 16) & (15u << shift)) | __float_as_uint(kInteger);
+          v[e] = __float_as_uint(fmaf(__uint_as_float(bits) - kInteger, scale * (1.0f / (1 << shift)), zero));
+        }
+        float* dst = static_cast<float*>(p.out[which]) + at + 8 * c;
+        if constexpr (kWords == 2) {
+          store_once(dst, v);
+        } else {
+          store_once(dst, {v[0], v[1], v[2], v[3]});
+          store_once(dst + 4, {v[4], v[5], v[6], v[7]});
+        }
+      }
     } else {
-      __stcs(reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out[which]) + at),
-             make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
-                        pack_bf16x2(v[6], v[7])));
+      const uint32_t scales = __byte_perm(pair[i], 0, 0x1010), zeros = __byte_perm(pair[i], 0, 0x3232);
+      uint32_t out[4 * kWords];
+#pragma unroll
+      for (int c = 0; c < kWords; ++c) {
+        uint32_t v[4];                             // channels (j, j + 4)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t large = ((codes[i][c] >> (4 * j)) & 0x000f000fu) | 0x43004300u;   // 128 + code
+          v[j] = fma_bf16x2(add_bf16x2(large, 0xc300c300u), scales, zeros);
+        }
+        out[4 * c] = __byte_perm(v[0], v[1], 0x5410);
+        out[4 * c + 1] = __byte_perm(v[2], v[3], 0x5410);
+        out[4 * c + 2] = __byte_perm(v[0], v[1], 0x7632);
+        out[4 * c + 3] = __byte_perm(v[2], v[3], 0x7632);
+      }
+      store_once(static_cast<__nv_bfloat16*>(p.out[which]) + at, out);
     }
   }
 }
@@ -1138,18 +1257,25 @@ Kv4Rows kv4_rows(const trinity_sm100_kv4_cache& c, const trinity_sm100_kv4_rows&
   return p;
 }
 
-// Rows a thread takes: one while the GPU is not full of them (least latency), else four (four times the
-// bytes in flight).
-constexpr int kKv4Batch = 4;
+// What a thread takes: eight channels of one row while the GPU is not full of such threads (least
+// latency), else sixteen of two rows where rows start on 32 bytes, and eight of four where they do not
+// (four times the bytes in flight; sixteen channels take half the work on addresses for each).
 struct Kv4Grid {
-  int batch;
+  int words, batch;
   dim3 blocks;
-  Kv4Grid(long long tokens, const trinity_sm100_kv4_cache& c) {
+  Kv4Grid(long long tokens, const trinity_sm100_kv4_cache& c, bool wide) {
     const long long lanes = tokens * c.kv_heads * (c.head_dim / 8);
-    batch = lanes > 148 * 2048 ? kKv4Batch : 1;
-    blocks = dim3(unsigned((lanes + 256 * batch - 1) / (256 * batch)), 2);
+    words = lanes > 148 * 2048 && wide ? 2 : 1;
+    batch = lanes > 148 * 2048 ? 4 / words : 1;
+    blocks = dim3(unsigned((lanes + 256 * words * batch - 1) / (256 * words * batch)), 2);
   }
 };
+// Whether every row of the keys and values starts on a multiple of `bytes`.
+bool kv4_rows_start_on(int bytes, const trinity_sm100_kv4_rows& r, int element) {
+  const uintptr_t pointers = reinterpret_cast<uintptr_t>(r.k) | reinterpret_cast<uintptr_t>(r.v);
+  const long long strides = r.k_token_stride | r.v_token_stride | r.k_head_stride | r.v_head_stride;
+  return pointers % bytes == 0 && strides % (bytes / element) == 0;
+}
 
 int check_kv4_rows(const char* what, const trinity_sm100_kv4_cache& c, const trinity_sm100_kv4_rows& r) {
   if (int rc = check_kv4_cache(what, c)) return rc;
@@ -1206,19 +1332,20 @@ extern "C" int trinity_sm100_kv4_append(const trinity_sm100_kv4_cache* cache, co
   Kv4Rows p = kv4_rows(*cache, r);
   p.in[0] = static_cast<const __nv_bfloat16*>(r.k);
   p.in[1] = static_cast<const __nv_bfloat16*>(r.v);
-  // 16-byte loads where every row starts on 16 bytes
-  const bool vectors = aligned16(r.k) && aligned16(r.v) && r.k_token_stride % 8 == 0 && r.v_token_stride % 8 == 0 &&
-                       r.k_head_stride % 8 == 0 && r.v_head_stride % 8 == 0;
-  const Kv4Grid grid(r.tokens, *cache);
+  const bool vectors = kv4_rows_start_on(16, r, 2);
+  const Kv4Grid grid(r.tokens, *cache, kv4_rows_start_on(32, r, 2));
   KernelLaunch launch(grid.blocks, dim3(256), 0, static_cast<cudaStream_t>(stream_handle));
   cudaError_t e;
-#define TRINITY_KV4_APPEND(D, V) \
-  e = grid.batch == 1 ? cudaLaunchKernelEx(&launch.config, kv4_append_kernel<D, V, 1>, p) \
-                      : cudaLaunchKernelEx(&launch.config, kv4_append_kernel<D, V, kKv4Batch>, p);
+#define TRINITY_KV4_APPEND(D)                                                                            \
+  e = grid.words == 2   ? cudaLaunchKernelEx(&launch.config, kv4_append_kernel<D, 2, true, 2>, p)        \
+      : grid.batch == 4 ? (vectors ? cudaLaunchKernelEx(&launch.config, kv4_append_kernel<D, 1, true, 4>, p)   \
+                                   : cudaLaunchKernelEx(&launch.config, kv4_append_kernel<D, 1, false, 4>, p)) \
+      : vectors         ? cudaLaunchKernelEx(&launch.config, kv4_append_kernel<D, 1, true, 1>, p)        \
+                        : cudaLaunchKernelEx(&launch.config, kv4_append_kernel<D, 1, false, 1>, p);
   if (cache->head_dim == 128) {
-    if (vectors) TRINITY_KV4_APPEND(128, true) else TRINITY_KV4_APPEND(128, false)
+    TRINITY_KV4_APPEND(128)
   } else {
-    if (vectors) TRINITY_KV4_APPEND(64, true) else TRINITY_KV4_APPEND(64, false)
+    TRINITY_KV4_APPEND(64)
   }
 #undef TRINITY_KV4_APPEND
   if (e != cudaSuccess) return fail(TRINITY_SM100_E_CUDA, "kv4_append launch: %s", cudaGetErrorString(e));
@@ -1233,24 +1360,26 @@ extern "C" int trinity_sm100_kv4_read(const trinity_sm100_kv4_cache* cache, cons
   if (int rc = check_kv4_rows("kv4_read", *cache, r)) return rc;
   if (out_dtype != TRINITY_SM100_BF16 && out_dtype != TRINITY_SM100_FP32)
     return fail(TRINITY_SM100_E_INVALID, "kv4_read: unknown output dtype %d", out_dtype);
-  const int unit = out_dtype == TRINITY_SM100_FP32 ? 4 : 8;
-  if (!aligned16(r.k) || !aligned16(r.v) || r.k_token_stride % unit || r.v_token_stride % unit || r.k_head_stride % unit ||
-      r.v_head_stride % unit)
-    return fail(TRINITY_SM100_E_INVALID, "kv4_read: output rows must start on 16 bytes");
+  const int element = out_dtype == TRINITY_SM100_FP32 ? 4 : 2;
+  if (!kv4_rows_start_on(16, r, element)) return fail(TRINITY_SM100_E_INVALID, "kv4_read: output rows must start on 16 bytes");
   if (int rc = require_sm100(nullptr)) return rc;
   Kv4Rows p = kv4_rows(*cache, r);
   p.out[0] = r.k;
   p.out[1] = r.v;
   p.out_f32 = out_dtype == TRINITY_SM100_FP32;
-  const Kv4Grid grid(r.tokens, *cache);
+  const Kv4Grid grid(r.tokens, *cache, kv4_rows_start_on(32, r, element));
   KernelLaunch launch(grid.blocks, dim3(256), 0, static_cast<cudaStream_t>(stream_handle));
   cudaError_t e;
-  if (cache->head_dim == 128)
-    e = grid.batch == 1 ? cudaLaunchKernelEx(&launch.config, kv4_read_kernel<128, 1>, p)
-                        : cudaLaunchKernelEx(&launch.config, kv4_read_kernel<128, kKv4Batch>, p);
-  else
-    e = grid.batch == 1 ? cudaLaunchKernelEx(&launch.config, kv4_read_kernel<64, 1>, p)
-                        : cudaLaunchKernelEx(&launch.config, kv4_read_kernel<64, kKv4Batch>, p);
+#define TRINITY_KV4_READ(D)                                                                        \
+  e = grid.words == 2   ? cudaLaunchKernelEx(&launch.config, kv4_read_kernel<D, 2, 2>, p)           \
+      : grid.batch == 4 ? cudaLaunchKernelEx(&launch.config, kv4_read_kernel<D, 1, 4>, p)           \
+                        : cudaLaunchKernelEx(&launch.config, kv4_read_kernel<D, 1, 1>, p);
+  if (cache->head_dim == 128) {
+    TRINITY_KV4_READ(128)
+  } else {
+    TRINITY_KV4_READ(64)
+  }
+#undef TRINITY_KV4_READ
   if (e != cudaSuccess) return fail(TRINITY_SM100_E_CUDA, "kv4_read launch: %s", cudaGetErrorString(e));
   count_launch();
   return check_launch("kv4_read");
