@@ -88,6 +88,21 @@ def test_assignments(kernels, kind, count, m):
     check(kernels.gemm_adapters(x, w, down, up, index, scales=scales), *expected(x, w, down, up, index, scales, None))
 
 
+@pytest.mark.parametrize("most", [15, 16, 17, 31, 32, 33, 47, 48, 49, 63, 64])
+@pytest.mark.parametrize("rank,n", [(16, 328), (64, 264), (128, 520)])
+def test_shares_of_a_tile(kernels, most, rank, n):
+    """Rows of one adapter scattered over a tile of 64 rows in every number of sixteens, others and none between;
+    a bias reaches the rows without an adapter too; few tiles of rows and many."""
+    for m in (64, 333):
+        x, w, down, up, scales, bias = make(m, 136, n, rank, 4, most)
+        index = indexes("mixed", m, 3, most)
+        for row0 in range(0, m, 64):
+            places = row0 + torch.randperm(64, generator=torch.Generator().manual_seed(row0 + most))[:most]
+            index[places[places < m].to(DEV)] = 3
+        check(kernels.gemm_adapters(x, w, down, up, index, scales=scales, bias=bias),
+              *expected(x, w, down, up, index, scales, bias))
+
+
 @pytest.mark.parametrize("m", [4735, 4736, 5000])
 @pytest.mark.parametrize("kind", ["mixed", "sorted"])
 def test_prompts(kernels, m, kind):

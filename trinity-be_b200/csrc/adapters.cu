@@ -7,18 +7,20 @@
 //   2. expand   delta[i] = t[i] up[a] + bias            [m, n], rounded to BF16 once
 //   3. the GEMM kernel with delta as its matrix side operand (added in FP32)
 // Both small kernels work on tiles of rows.  A tile's rows may have any adapters; the distinct ones are
-// taken in turn, each multiplied with all rows of the tile, and every row keeps only the result of
+// taken in turn.  Shrink multiplies each with all rows of the tile and every row keeps only the result of
 // its own adapter (a selection, not a product with zero: an adapter that holds infinities or NaN
-// reaches its own rows only).  Sorted prompts have one or two adapters in a tile; decode batches of
+// reaches its own rows only); expand gathers the adapter's rows.  Sorted prompts have one or two adapters in a tile; decode batches of
 // sixteen rows sixteen at most, where the weights' bytes and not the products are what takes time.
 //
 // Bound by memory with few rows: the weight (the GEMM's part) and the adapters that the rows name, read
 // once each.  16 rows x 8192 x 8192 with 12 adapters of rank 16: 39 us (floor 21; GEMM 29, the small
-// kernels 8 each, in part beside it).  61 rows x 4096 x 28672, 24 adapters of rank 64: 73 us (floor 52).
+// kernels 8 each, in part beside it).  61 rows x 4096 x 28672, 24 adapters of rank 64: 67 us (floor 52).
 // 8192^3 with rank 32: 800 to 823 us, of which the GEMM 707 to 720 under its power cap.
 //
 // Rounding t and delta to BF16 costs 2^-8 of the adapter's own contribution each, as the
 // intermediates of the other chained products of this library do.
+#include <type_traits>
+
 #include "host_common.h"
 #include "sm100_ptx.cuh"
 
@@ -236,20 +238,32 @@ __host__ __device__ constexpr int expand_smem_bytes() {
   return 1024 + kExpandRows * kRank * 2 + expand_slabs<kRank, kCols>() * kRank * kCols * 2 + kExpandRows * (kCols + 8) * 2;
 }
 
+// Blocks an SM that the registers must allow for (shared memory may allow for fewer).
+template <int kRank, int kCols>
+__host__ __device__ constexpr int expand_per_sm() {
+  return kCols == 128 ? (kRank < 128 ? 4 : 2) : kRank < 64 ? 2 : 1;
+}
+
 // delta of 64 rows.  The work on a tile of rows is a sequence of slabs, (kCols columns, adapter) with the
 // adapters innermost; the gridDim.x blocks of a tile take equal runs of it, with one thread keeping a ring
-// of slabs filled across the columns.  Warps take 32 columns each.  A block writes, of the columns of a
-// slab, the rows of the adapters that its run covered (rows without one go with the first adapter): every
-// element is written once.
+// of slabs filled across the columns.  Warps take 32 columns each.  The rows that have an adapter are
+// gathered (ldmatrix takes any row addresses) into as few tiles of sixteen as hold them, so that a slab
+// costs one tile's products where its adapter has up to sixteen rows, wherever they lie: 24 adapters on 61 rows,
+// rank 64, 28672 columns take 23 us for 88 MB; with products of every tile of rows in place, of which each row
+// kept its own, 31 us (the fetches alone take 21).  A block writes, of the columns of a slab, the rows
+// of the adapters that its run covered (rows without one go with the first adapter): every element is
+// written once.
 template <int kRank, int kCols>
-__global__ void __launch_bounds__(kCols, kCols == 128 ? 4 : 2)
+__global__ void __launch_bounds__(kCols, expand_per_sm<kRank, kCols>())
 adapter_expand_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant__ CUtensorMap map_up,
                       const AdapterParams p) {
   constexpr int kRowT = kRank < 64 ? kRank * 2 : 128;
   constexpr int kTile = kExpandRows * kRank * 2, kSlab = kRank * kCols * 2, kSlabs = expand_slabs<kRank, kCols>();
   constexpr int kPitch = (kCols + 8) * 2;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ int of_row[kExpandRows], distinct[kExpandRows], place[kExpandRows], found;   // place of a row's adapter in distinct
+  __shared__ int of_row[kExpandRows], distinct[kExpandRows], found;
+  __shared__ __align__(16) int place[kExpandRows];        // of a row's adapter in distinct; kExpandRows: none
+  __shared__ int order[kExpandRows], start[kExpandRows + 1];   // the rows by place, and where each place's begin
   __shared__ __align__(8) uint64_t full[kSlabs], t_full;
   const uint32_t ts = (smem_u32(smem_raw) + 1023u) & ~1023u, us = ts + kTile;
   uint8_t* staging = smem_raw + (ts - smem_u32(smem_raw)) + kTile + kSlabs * kSlab;
@@ -279,11 +293,30 @@ adapter_expand_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_co
   };
   if (threadIdx.x == 0 && adapters)
     for (int q = begin; q < end && q < begin + kSlabs - 1; ++q) fetch(q);
-  for (int i = threadIdx.x; i < kExpandRows; i += kCols) {
-    int at = 0;
+  if (threadIdx.x < kExpandRows) {
+    int at = of_row[threadIdx.x] < 0 ? kExpandRows : 0;
     for (int o = 1; o < adapters; ++o)
-      if (of_row[i] == distinct[o]) at = o;
-    place[i] = at;
+      if (of_row[threadIdx.x] == distinct[o]) at = o;
+    place[threadIdx.x] = at;
+  }
+  __syncthreads();
+  if (threadIdx.x < kExpandRows) {
+    const int mine = place[threadIdx.x];
+    int before = 0, same = 0, named = 0;      // rows of places before this row's, of this place before this row, with a place
+#pragma unroll 4
+    for (int i = 0; i < kExpandRows; i += 4) {
+      const int4 four = *reinterpret_cast<const int4*>(place + i);
+      const int other[4] = {four.x, four.y, four.z, four.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        before += other[e] < mine;
+        same += other[e] == mine && i + e < int(threadIdx.x);
+        named += other[e] < kExpandRows;
+      }
+    }
+    order[before + same] = threadIdx.x;
+    if (same == 0 && mine < kExpandRows) start[mine] = before;
+    if (threadIdx.x == 0) start[adapters] = named;
   }
   grid_dependency_wait();
   bool ok = true;
@@ -296,16 +329,55 @@ adapter_expand_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_co
     }
     ok = mbar_wait(smem_u32(&t_full), 0, 0xA21);
   }
-  float out[4][4][4];     // [16 rows][8 columns][fragment]
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) out[i][j][e] = 0.0f;
   int from = begin % steps;            // first adapter of the run on the present columns
   int columns = begin / steps, ordinal = from, s = 0;      // of slab q: its columns, adapter and stage
   uint32_t parity = 0;
+  float bias[4][2];                    // of the lane's columns
+  // kTiles tiles of sixteen of the rows that have the adapter (from number `first` on, before number
+  // `behind`) times the slab, rounded into the warp's columns of the staging tile
+  auto products = [&](auto tiles, uint32_t slab, int first, int behind) {
+    constexpr int kTiles = decltype(tiles)::value;
+    float acc[kTiles][4][4];
+    int row[kTiles];                   // whose address the lane gives to ldmatrix
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+      row[i] = order[min(first + i * 16 + (lane & 15), behind - 1)];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.0f;
+    }
+#pragma unroll
+    for (int k16 = 0; k16 < kRank; k16 += 16) {
+      uint32_t b[2][4];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        load_matrices<true>(slab + swizzled((k16 + (lane & 15)) * 128 + (warp % 2) * 64 + j * 32 + (lane >> 4) * 16, 128), b[j]);
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i) {
+        uint32_t a[4];
+        load_matrices<false>(ts + k16 / 64 * kExpandRows * 128 +
+                             swizzled(row[i] * kRowT + (k16 % 64 + (lane >> 4) * 8) * 2, kRowT), a);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          mma_bf16_16816(acc[i][2 * j], a, b[j][0], b[j][1]);
+          mma_bf16_16816(acc[i][2 * j + 1], a, b[j][2], b[j][3]);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int at = first + i * 16 + half * 8 + g;
+        if (at >= behind) continue;
+        uint8_t* dst = staging + order[at] * kPitch + (warp * 32 + 2 * t) * 2;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<uint32_t*>(dst + j * 16) =
+              pack_bf16x2(acc[i][j][2 * half] + bias[j][0], acc[i][j][2 * half + 1] + bias[j][1]);
+      }
+  };
   for (int q = begin; q < end; ++q, s = s + 1 == kSlabs ? 0 : s + 1, parity ^= s == 0 ? 1u : 0u) {
     if (q != begin && ++ordinal == steps) {
       ordinal = 0;
@@ -314,92 +386,43 @@ adapter_expand_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_co
     if (adapters && ok) ok = mbar_wait(smem_u32(full + s), parity, 0xA22);
     __syncthreads();                   // everyone is through with the slab before, which is filled again
     if (threadIdx.x == 0 && adapters && q + kSlabs - 1 < end) fetch(q + kSlabs - 1);
+    const int col0 = columns * kCols;
+    if (ordinal == from) {             // new columns
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int col = col0 + warp * 32 + j * 8 + 2 * t;
+        const bool some = p.bias && col < p.n;
+        bias[j][0] = some ? __bfloat162float(p.bias[col]) : 0.0f;
+        bias[j][1] = some ? __bfloat162float(p.bias[col + 1]) : 0.0f;
+      }
+    }
     if (adapters) {
       const uint32_t slab = us + s * kSlab + warp / 2 * kRank * 128;      // the half with this warp's columns
-      const int adapter = distinct[ordinal];
-      uint32_t whole = 0;              // tiles of sixteen rows that are all this adapter's: no selection
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (__all_sync(0xffffffffu, of_row[i * 16 + g] == adapter && of_row[i * 16 + g + 8] == adapter)) whole |= 1u << i;
-      if (whole) {
-#pragma unroll
-        for (int k16 = 0; k16 < kRank; k16 += 16) {
-          uint32_t b[2][4];
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-            load_matrices<true>(slab + swizzled((k16 + (lane & 15)) * 128 + (warp % 2) * 64 + j * 32 + (lane >> 4) * 16, 128), b[j]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (!(whole >> i & 1u)) continue;
-            uint32_t a[4];
-            load_matrices<false>(ts + k16 / 64 * kExpandRows * 128 +
-                                 swizzled((i * 16 + (lane & 15)) * kRowT + (k16 % 64 + (lane >> 4) * 8) * 2, kRowT), a);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              mma_bf16_16816(out[i][2 * j], a, b[j][0], b[j][1]);
-              mma_bf16_16816(out[i][2 * j + 1], a, b[j][2], b[j][3]);
-            }
-          }
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (i * 16 >= rows) break;
-        if (whole >> i & 1u) continue;
-        const bool low = of_row[i * 16 + g] == adapter, high = of_row[i * 16 + g + 8] == adapter;
-        if (!__any_sync(0xffffffffu, low || high)) continue;
-        float acc[4][4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[j][e] = 0.0f;
-#pragma unroll
-        for (int k16 = 0; k16 < kRank; k16 += 16) {
-          uint32_t a[4];
-          load_matrices<false>(ts + k16 / 64 * kExpandRows * 128 +
-                               swizzled((i * 16 + (lane & 15)) * kRowT + (k16 % 64 + (lane >> 4) * 8) * 2, kRowT), a);
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            uint32_t b[4];
-            load_matrices<true>(slab + swizzled((k16 + (lane & 15)) * 128 + (warp % 2) * 64 + j * 32 + (lane >> 4) * 16, 128), b);
-            mma_bf16_16816(acc[2 * j], a, b[0], b[1]);
-            mma_bf16_16816(acc[2 * j + 1], a, b[2], b[3]);
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (low) { out[i][j][0] = acc[j][0]; out[i][j][1] = acc[j][1]; }
-          if (high) { out[i][j][2] = acc[j][2]; out[i][j][3] = acc[j][3]; }
-        }
-      }
+      const int first = start[ordinal], behind = start[ordinal + 1];
+      if (behind - first <= 16)
+        products(std::integral_constant<int, 1>(), slab, first, behind);
+      else if (behind - first <= 32)
+        products(std::integral_constant<int, 2>(), slab, first, behind);
+      else
+        products(std::integral_constant<int, 4>(), slab, first, behind);
     }
     if (ordinal + 1 < steps && q + 1 < end) continue;
-    // the run leaves these columns: each warp turns its 32 columns through shared memory and writes them
-    const int col0 = columns * kCols;
+    // the run leaves these columns: rows without an adapter (which get the bias), then all, each warp its 32 columns
+    if (from == 0)
+      for (int at = (adapters ? start[adapters] : 0) + g; at < kExpandRows; at += 8)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int col = warp * 32 + j * 8 + 2 * t;
-      float b0 = 0.0f, b1 = 0.0f;
-      if (p.bias && col0 + col < p.n) {
-        b0 = __bfloat162float(p.bias[col0 + col]);
-        b1 = __bfloat162float(p.bias[col0 + col + 1]);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        *reinterpret_cast<uint32_t*>(staging + (i * 16 + g) * kPitch + col * 2) = pack_bf16x2(out[i][j][0] + b0, out[i][j][1] + b1);
-        *reinterpret_cast<uint32_t*>(staging + (i * 16 + g + 8) * kPitch + col * 2) = pack_bf16x2(out[i][j][2] + b0, out[i][j][3] + b1);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) out[i][j][e] = 0.0f;
-      }
-    }
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<uint32_t*>(staging + order[at] * kPitch + (warp * 32 + j * 8 + 2 * t) * 2) = pack_bf16x2(bias[j][0], bias[j][1]);
     __syncwarp();
     const int c = warp * 32 + (lane & 3) * 8;
     if (col0 + c < p.n)
 #pragma unroll
-      for (int r = lane >> 2; r < kExpandRows; r += 8)
-        if (r < rows && place[r] >= from && place[r] <= ordinal)
+      for (int r = lane >> 2; r < kExpandRows; r += 8) {
+        const int at = place[r] < kExpandRows ? place[r] : 0;
+        if (r < rows && at >= from && at <= ordinal)
           *reinterpret_cast<uint4*>(p.delta + static_cast<long long>(row0 + r) * p.n + col0 + c) =
               *reinterpret_cast<const uint4*>(staging + r * kPitch + c * 2);
+      }
     __syncwarp();
     from = 0;
   }
@@ -454,7 +477,7 @@ int launch_expand(const AdapterParams& p, int sm_count, cudaStream_t stream) {
   if (int rc = make_tensor_map_3d(&map_up, p.up, 2, p.n, p.rank, p.count, p.ld_up * 2, p.stride_up * 2, 64, kRank, 1, 128)) return rc;
   // as many blocks as are resident together, an equal number for every tile of rows
   const int tiles = (p.m + kExpandRows - 1) / kExpandRows, columns = (p.n + kCols - 1) / kCols;
-  const int resident = sm_count * min(kCols == 128 ? 4 : 2, 227 * 1024 / (kSmem + 2048));
+  const int resident = sm_count * min(expand_per_sm<kRank, kCols>(), 227 * 1024 / (kSmem + 2048));
   const long long slabs = static_cast<long long>(columns) * min(p.count, min(kExpandRows, p.m));
   const int blocks = int(max(1ll, min(slabs, static_cast<long long>(resident / tiles))));
   KernelLaunch launch(dim3(blocks, tiles), dim3(kCols), kSmem, stream);
