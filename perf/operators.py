@@ -24,18 +24,12 @@ own = False
 _DTYPES = {"bf16": torch.bfloat16, "fp32": torch.float32}
 
 
-_loaded = None
-
-
 def _kernels():
-    global _loaded
-    if _loaded is None:
-        package = str(Path(__file__).resolve().parents[1] / "trinity-be_b200")
-        if package not in sys.path:
-            sys.path.insert(0, package)
-        from trinity_lowering import kernels
-        _loaded = kernels
-    return _loaded
+    package = str(Path(__file__).resolve().parents[1] / "trinity-be_b200")
+    if package not in sys.path:
+        sys.path.insert(0, package)
+    from trinity_lowering import kernels
+    return kernels
 
 
 # ------------------------------------------------------------------------------------- cases
