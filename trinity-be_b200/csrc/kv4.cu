@@ -393,6 +393,7 @@ constexpr int kKv4RowUnits = 2;
 // groups of scales each need more registers and shared memory.
 __host__ __device__ constexpr int kv4_per_sm(int groups, int head_tiles) { return head_tiles > 1 ? 2 : 3; }
 constexpr uint32_t kKv4Lag = 2;
+constexpr float kKv4NoScore = -3e38f;     // reference point before the first score: below any but -infinity
 constexpr int kKv4Threads = kKv4Warps * 32;
 
 struct Kv4Attend {
@@ -823,7 +824,7 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           for (int e = 0; e < 4; ++e) acc[n][i][e] = 0.0f;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          ref[n][c] = -INFINITY;
+          ref[n][c] = kKv4NoScore;
           sum[n][c] = 0.0f;
 #pragma unroll
           for (int i = 0; i < kNG; ++i) zeros[n][c][i] = 0.0f;
@@ -1102,7 +1103,7 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 #pragma unroll
           for (int w = 0; w < kKv4Warps; ++w) {
             const float mw = join_ml[(w * 4 + place) * 2], lw = join_ml[(w * 4 + place) * 2 + 1];
-            const float f = mw == -INFINITY ? (lw == 0.0f ? 0.0f : 1.0f) : exp2f(mw - m);
+            const float f = exp2f(mw - m);
             const float4 x = *reinterpret_cast<const float4*>(join + (w * 4 + place) * kPitch + channel);
             total = fmaf(lw, f, total);
             o.x = fmaf(x.x, f, o.x);
