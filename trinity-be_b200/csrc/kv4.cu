@@ -375,12 +375,14 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Rows p) {
 //   the second sum is FP32.  (Without the 8 both sums would be some 3 where the values average to 0: over
 //   262144 positions that cancellation cost 2.5 times the output's own rounding.  One product of the
 //   weights with a constant operand gives what the 8 takes off every channel; it is added to the
-//   accumulators every fourth tile.)  p_t scale_v[t] enters as FP16 (2^-12, far below the output's rounding): p_t is at most 2^15
-//   (see the maximum below) and scale_v is divided by a power of two, a running bound of the
-//   scales seen, which the accumulators follow like they follow the maximum.
+//   accumulators every fourth tile.)  p_t scale_v[t] enters as FP16 (2^-11, an eighth of the
+//   output's rounding).  What must fit FP16 is the product, so the reference point of a head's exponentials follows
+//   the largest product of weight and value magnitude, not the largest weight: a loud value that
+//   hardly weighs anything takes no bits from the others, and values may have any size that
+//   FP32 sums of the weights allow.
 //
 // Measured: 64 sequences x 4096 positions x 8 cached heads (287 MB) 70 us, 2 x 262144 with sixteen query
-// heads to a cached one (604 MB) 189 us, 200 sequences of 0 to 8191 positions 27 us, one of 1023 9.8 us.
+// heads to a cached one (604 MB) 192 us, 200 sequences of 0 to 8191 positions 27 us, one of 1023 9.8 us.
 // When the first took 77, it took 60 without the arithmetic and 64 without the copies: what bounds it is
 // the latency of a warp's chain of products, exponentials and products at the twelve (eight) warps that
 // the registers allow.  Tiles of 64 positions (85 to 90 us) and four blocks an SM with two stages (84)
@@ -393,6 +395,12 @@ constexpr int kKv4RowUnits = 2;
 // groups of scales each need more registers and shared memory.
 __host__ __device__ constexpr int kv4_per_sm(int groups, int head_tiles) { return head_tiles > 1 ? 2 : 3; }
 constexpr uint32_t kKv4Lag = 2;
+// The largest exponential times value magnitude is 2^kKv4Top when the reference point is set, and 2^kKv4Room
+// times that at most before it is set again; times kKv4Unit it is an FP16 number (below 2^15).  The
+// factor keeps the exponentials themselves inside FP32's range where values are large: those of values of 2^100
+// are some 2^-73, and what is below 2^-126 is lost.  Magnitudes below kKv4Smallest count as that
+// (sums of the weights of values that are all zero must not overflow).
+constexpr float kKv4Top = 27.0f, kKv4Room = 8.0f, kKv4Unit = 0x1p-20f, kKv4Smallest = 0x1p-60f;
 constexpr float kKv4NoScore = -3e38f;     // reference point before the first score: below any but -infinity
 constexpr int kKv4Threads = kKv4Warps * 32;
 
@@ -560,6 +568,11 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
 __device__ __forceinline__ float exp2_approx(float x) {   // 2^-22 relative; results below 2^-126 are 0
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float max_or_nan(float a, float b) {   // NaN if either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
 template <bool kTrans>
@@ -815,7 +828,6 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           for (int i = 0; i < kNG; ++i) zero_factor[n][c][i] = factors[n * 8 + 2 * t + c][1 + i];
         }
       float acc[kNT][kMT][4], zeros[kNT][2][kNG], ref[kNT][2], sum[kNT][2];
-      float limit = 0.0f, inverse_limit = 0.0f;        // power of two above every value scale so far
 #pragma unroll
       for (int n = 0; n < kNT; ++n) {
 #pragma unroll
@@ -927,57 +939,50 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
                   for (int i = 0; i < kNG; ++i) value_pair[u][r][i] = 0;
                 }
           }
-          // The reference point of a head's exponentials is 2^7 below the largest score when it was last
-          // set, and is set again only when a score exceeds that one by 2^8 or more (most tiles need
-          // neither the shuffles nor the rescaling): exponentials stay below 2^15, and FP16 keeps
-          // those down to 2^-31 of the largest.
+          // The reference point of a head's exponentials lies kKv4Top below the largest score plus logarithm of
+          // the value's magnitude (an upper bound: the exponent and one) when it was last set, and is set
+          // again only when one exceeds that by kKv4Room (most tiles need neither the shuffles nor the
+          // rescaling).  FP16 keeps products of weight and scale down to 2^-30 of the largest of weight and
+          // magnitude.  A group whose scale is NaN is NaN in the result whatever it weighs: its
+          // zero, which may be infinite, does not count.
+          float level[kKv4Sub][2];
+#pragma unroll
+          for (int u = 0; u < kKv4Sub; ++u)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              float size = kKv4Smallest;
+#pragma unroll
+              for (int i = 0; i < kNG; ++i)
+                size = fmaxf(size, max_or_nan(fabsf(bf16_lo(value_pair[u][r][i])), fabsf(bf16_hi(value_pair[u][r][i]))));
+              level[u][r] = __uint_as_float(0x4b000000u | __float_as_uint(size) >> 23) - (8388608.0f + 126.0f);
+            }
           bool raise = false;
 #pragma unroll
-          for (int u = 0; u < kKv4Sub; ++u) {
+          for (int u = 0; u < kKv4Sub; ++u)
 #pragma unroll
             for (int n = 0; n < kNT; ++n)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) raise |= score[u][n][e] > ref[n][e & 1] + 15.0f;
-#pragma unroll
-            for (int r = 0; r < 2; ++r)
-#pragma unroll
-              for (int i = 0; i < kNG; ++i) raise |= bf16_lo(value_pair[u][r][i]) > limit;
-          }
+              for (int e = 0; e < 4; ++e)
+                raise |= score[u][n][e] + level[u][e >> 1] > ref[n][e & 1] + (kKv4Top + kKv4Room);
           if (__any_sync(0xffffffffu, raise)) {
-            float most = 0.0f;
-#pragma unroll
-            for (int u = 0; u < kKv4Sub; ++u)
-#pragma unroll
-              for (int r = 0; r < 2; ++r)
-#pragma unroll
-                for (int i = 0; i < kNG; ++i) most = fmaxf(most, bf16_lo(value_pair[u][r][i]));
-#pragma unroll
-            for (int o = 4; o < 32; o *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-            float rescale = 1.0f;
-            if (most > limit) {
-              const uint32_t power = min((__float_as_uint(most) & 0x7f800000u) + 0x00800000u, 0x7e800000u);
-              inverse_limit = __uint_as_float(0x7f000000u - power);      // 2^-k for limit 2^k
-              rescale = limit * inverse_limit;
-              limit = __uint_as_float(power);
-            }
 #pragma unroll
             for (int n = 0; n < kNT; ++n)
 #pragma unroll
               for (int c = 0; c < 2; ++c) {
                 float m = -INFINITY;
 #pragma unroll
-                for (int u = 0; u < kKv4Sub; ++u) m = fmaxf(m, fmaxf(score[u][n][c], score[u][n][2 + c]));
+                for (int u = 0; u < kKv4Sub; ++u)
+                  m = fmaxf(m, fmaxf(score[u][n][c] + level[u][0], score[u][n][2 + c] + level[u][1]));
 #pragma unroll
                 for (int o = 4; o < 32; o *= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
                 float f = 1.0f;
-                if (m - 7.0f > ref[n][c]) {
-                  f = exp2_approx(ref[n][c] - (m - 7.0f));
-                  ref[n][c] = m - 7.0f;
+                if (m - kKv4Top > ref[n][c]) {
+                  f = exp2_approx(ref[n][c] - (m - kKv4Top));
+                  ref[n][c] = m - kKv4Top;
                 }
                 sum[n][c] *= f;
 #pragma unroll
                 for (int i = 0; i < kNG; ++i) zeros[n][c][i] *= f;
-                f *= rescale;
 #pragma unroll
                 for (int i = 0; i < kNG; ++i) {
                   shift[n][i][c] *= f;
@@ -1005,8 +1010,8 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
             for (int i = 0; i < kNG; ++i)
 #pragma unroll
               for (int r = 0; r < 2; ++r) {
-                const float scale = bf16_lo(value_pair[u][r][i]) * inverse_limit;
-              const float zero = fmaf(8.0f, bf16_lo(value_pair[u][r][i]), bf16_hi(value_pair[u][r][i]));
+                const float scale = bf16_lo(value_pair[u][r][i]) * kKv4Unit;
+                const float zero = fmaf(8.0f, bf16_lo(value_pair[u][r][i]), bf16_hi(value_pair[u][r][i]));
 #pragma unroll
                 for (int n = 0; n < kNT; ++n) {
                   const __half2 h = __floats2half2_rn(weight[n][2 * r] * scale, weight[n][2 * r + 1] * scale);
@@ -1078,7 +1083,7 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 #pragma unroll
             for (int o = 4; o < 32; o *= 2) zeros[n][c][i] += __shfl_xor_sync(0xffffffffu, zeros[n][c][i], o);
           float* mine = join + (warp * 4 + t) * kPitch + g * 4;
-          const float even = limit * 0x1p24f, odd = limit * 0x1p20f;
+          constexpr float even = 0x1p24f / kKv4Unit, odd = 0x1p20f / kKv4Unit;     // the units of codes and weights
 #pragma unroll
           for (int j = 0; j < kChunks; ++j) {
             const float zero = zeros[n][c][j * kNG / kChunks];
