@@ -137,7 +137,7 @@ TRINITY_SM100_API int trinity_sm100_gemm_batched_bf16(const trinity_sm100_gemm* 
  * gemm: bias mode none or column vector, any activation but the gated one; k and n multiples of 8, as are
  * pitches and strides; rank a multiple of 8 up to 128.  Only the adapters that index names are read,
  * and one that holds infinities or NaN reaches no rows but its own.  scales * (a @ down) and the
- * adapter's contribution (with the bias) are rounded to BF16 once each; all sums are FP32.
+ * adapter's contribution are rounded to BF16 once each; all sums are FP32, the bias's among them.
  */
 typedef struct trinity_sm100_adapters {
   const void* down;

@@ -4,8 +4,8 @@
 //
 // Three launches of one stream:
 //   1. shrink   t[i] = scale[a] * (x[i] down[a])        [m, rank], rounded to BF16 once
-//   2. expand   delta[i] = t[i] up[a] + bias            [m, n], rounded to BF16 once
-//   3. the GEMM kernel with delta as its matrix side operand (added in FP32)
+//   2. expand   delta[i] = t[i] up[a]                   [m, n], rounded to BF16 once
+//   3. the GEMM kernel with delta as its matrix side operand (it and the bias are added in FP32)
 // Both small kernels work on tiles of rows.  A tile's rows may have any adapters; the distinct ones are
 // taken in turn.  Shrink multiplies each with all rows of the tile and every row keeps only the result of
 // its own adapter (a selection, not a product with zero: an adapter that holds infinities or NaN
@@ -38,7 +38,6 @@ struct AdapterParams {
   const __nv_bfloat16* up;
   const int* index;
   const float* scales;         // null: 1
-  const __nv_bfloat16* bias;   // null: none
   __nv_bfloat16* t;            // [m, padded rank]
   __nv_bfloat16* delta;        // [m, n]
   long long ldx, ld_down, stride_down, ld_up, stride_up;
@@ -332,7 +331,6 @@ adapter_expand_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_co
   int from = begin % steps;            // first adapter of the run on the present columns
   int columns = begin / steps, ordinal = from, s = 0;      // of slab q: its columns, adapter and stage
   uint32_t parity = 0;
-  float bias[4][2];                    // of the lane's columns
   // kTiles tiles of sixteen of the rows that have the adapter (from number `first` on, before number
   // `behind`) times the slab, rounded into the warp's columns of the staging tile
   auto products = [&](auto tiles, uint32_t slab, int first, int behind) {
@@ -375,7 +373,7 @@ adapter_expand_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_co
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           *reinterpret_cast<uint32_t*>(dst + j * 16) =
-              pack_bf16x2(acc[i][j][2 * half] + bias[j][0], acc[i][j][2 * half + 1] + bias[j][1]);
+              pack_bf16x2(acc[i][j][2 * half], acc[i][j][2 * half + 1]);
       }
   };
   for (int q = begin; q < end; ++q, s = s + 1 == kSlabs ? 0 : s + 1, parity ^= s == 0 ? 1u : 0u) {
@@ -387,15 +385,6 @@ adapter_expand_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_co
     __syncthreads();                   // everyone is through with the slab before, which is filled again
     if (threadIdx.x == 0 && adapters && q + kSlabs - 1 < end) fetch(q + kSlabs - 1);
     const int col0 = columns * kCols;
-    if (ordinal == from) {             // new columns
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int col = col0 + warp * 32 + j * 8 + 2 * t;
-        const bool some = p.bias && col < p.n;
-        bias[j][0] = some ? __bfloat162float(p.bias[col]) : 0.0f;
-        bias[j][1] = some ? __bfloat162float(p.bias[col + 1]) : 0.0f;
-      }
-    }
     if (adapters) {
       const uint32_t slab = us + s * kSlab + warp / 2 * kRank * 128;      // the half with this warp's columns
       const int first = start[ordinal], behind = start[ordinal + 1];
@@ -407,12 +396,12 @@ adapter_expand_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_co
         products(std::integral_constant<int, 4>(), slab, first, behind);
     }
     if (ordinal + 1 < steps && q + 1 < end) continue;
-    // the run leaves these columns: rows without an adapter (which get the bias), then all, each warp its 32 columns
+    // the run leaves these columns: rows without an adapter (which get nothing), then all, each warp its 32 columns
     if (from == 0)
       for (int at = (adapters ? start[adapters] : 0) + g; at < kExpandRows; at += 8)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          *reinterpret_cast<uint32_t*>(staging + order[at] * kPitch + (warp * 32 + j * 8 + 2 * t) * 2) = pack_bf16x2(bias[j][0], bias[j][1]);
+          *reinterpret_cast<uint32_t*>(staging + order[at] * kPitch + (warp * 32 + j * 8 + 2 * t) * 2) = 0u;
     __syncwarp();
     const int c = warp * 32 + (lane & 3) * 8;
     if (col0 + c < p.n)
@@ -543,7 +532,6 @@ extern "C" int trinity_sm100_gemm_adapters_bf16(const trinity_sm100_gemm* gemm, 
   p.up = static_cast<const __nv_bfloat16*>(a.up);
   p.index = static_cast<const int*>(a.index);
   p.scales = static_cast<const float*>(a.scales);
-  p.bias = g.bias_mode == TRINITY_SM100_BIAS_COL_VECTOR ? static_cast<const __nv_bfloat16*>(g.bias) : nullptr;
   p.t = static_cast<__nv_bfloat16*>(a.workspace);
   p.delta = reinterpret_cast<__nv_bfloat16*>(static_cast<uint8_t*>(a.workspace) + adapter_t_bytes(g.m, a.rank));
   p.ldx = g.lda;
@@ -574,7 +562,9 @@ extern "C" int trinity_sm100_gemm_adapters_bf16(const trinity_sm100_gemm* gemm, 
   // shrink kernel after everything before that one had completed: x and the weight may be read at
   // once, so the GEMM begins beside the small kernels where an SM is free, and waits in its epilogue.
   g_late_wait_for_next_launch = true;
+  g_column_bias_for_next_launch = g.bias_mode == TRINITY_SM100_BIAS_COL_VECTOR ? g.bias : nullptr;
   const int launched = trinity_sm100_gemm_bf16(&with_delta, stream_handle);
   g_late_wait_for_next_launch = false;
+  g_column_bias_for_next_launch = nullptr;
   return launched;
 }

@@ -99,6 +99,7 @@ struct GemmParams {
   // The previous kernel of the stream produces the side operand only, and everything before that one had
   // completed when it let this one start: the operands are read at once, only the epilogue waits.
   int late_wait;
+  const __nv_bfloat16* column_bias;   // a column vector beside a matrix side operand (null: none)
   void* out;               // split form: the output, which its epilogue stores without a tensor map
   long long ldo;           // ... and its row pitch in elements
 };
@@ -239,6 +240,7 @@ __device__ __forceinline__ bool reduce_owned_tile(const GemmParams& p, const Gem
 
 // Set by the adapters entry point around its call of the GEMM entry point (same thread).
 thread_local bool g_late_wait_for_next_launch = false;
+thread_local const void* g_column_bias_for_next_launch = nullptr;
 
 // (the split form leaves the epilogue loop of the other forms unreachable in its instantiations)
 #pragma nv_diag_suppress 128
@@ -480,6 +482,7 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a,
       const int z = kBatched ? unit / p.tiles_per_batch : 0;
       locate_tile<kPair>(p, kBatched ? unit - z * p.tiles_per_batch : unit, rank, m_blk, n_blk, tile);
       const __nv_bfloat16* bias_base = p.bias + (kBatched ? z * p.stride_bias : 0);
+      const __nv_bfloat16* column_bias = p.bias_mode == TRINITY_SM100_BIAS_COL_VECTOR ? bias_base : p.column_bias;
       const int m0 = m_blk * kBM;
       const int n0 = n_blk * kOutN;
       const uint32_t acc = local_tile & 1u;
@@ -603,14 +606,8 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a,
           }
           if (out_row >= p.m) continue;
           const bool whole = gcol + 8 <= p.n;
-          if (p.bias_mode == TRINITY_SM100_BIAS_ROW_VECTOR) {
-            const float b = __bfloat162float(bias_base[out_row]);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] += b;
-          } else if (p.bias_mode != TRINITY_SM100_BIAS_NONE) {
-            const __nv_bfloat16* src = p.bias_mode == TRINITY_SM100_BIAS_COL_VECTOR
-                                           ? bias_base + gcol
-                                           : bias_base + static_cast<long long>(out_row) * p.ld_bias + gcol;
+          // eight columns of a side operand
+          auto add = [&](const __nv_bfloat16* src) {
             if (whole) {
               const uint4 b = __ldg(reinterpret_cast<const uint4*>(src));
               const uint32_t w[4] = {b.x, b.y, b.z, b.w};
@@ -624,6 +621,14 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a,
               for (int j = 0; j < 8; ++j)
                 if (gcol + j < p.n) x[j] += __bfloat162float(src[j]);
             }
+          };
+          if (column_bias) add(column_bias + gcol);
+          if (p.bias_mode == TRINITY_SM100_BIAS_ROW_VECTOR) {
+            const float b = __bfloat162float(bias_base[out_row]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] += b;
+          } else if (p.bias_mode == TRINITY_SM100_BIAS_MATRIX) {
+            add(bias_base + static_cast<long long>(out_row) * p.ld_bias + gcol);
           }
           if (!kGated && p.activation != TRINITY_SM100_ACT_NONE) {
 #pragma unroll
@@ -694,9 +699,9 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a,
             for (int j = 0; j < 32; ++j) x[j] = __uint_as_float(v[j]);
           }
           const int gcol = n0 + col;
-          if (p.bias_mode == TRINITY_SM100_BIAS_COL_VECTOR) {
+          if (column_bias) {
             if (gcol + 32 <= p.n) {
-              const uint4* src = reinterpret_cast<const uint4*>(bias_base + gcol);
+              const uint4* src = reinterpret_cast<const uint4*>(column_bias + gcol);
 #pragma unroll
               for (int v4 = 0; v4 < 4; ++v4) {
                 const uint4 b = __ldg(src + v4);
@@ -710,9 +715,10 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a,
             } else {
 #pragma unroll
               for (int j = 0; j < 32; ++j)
-                if (gcol + j < p.n) x[j] += __bfloat162float(bias_base[gcol + j]);
+                if (gcol + j < p.n) x[j] += __bfloat162float(column_bias[gcol + j]);
             }
-          } else if (p.bias_mode == TRINITY_SM100_BIAS_ROW_VECTOR) {
+          }
+          if (p.bias_mode == TRINITY_SM100_BIAS_ROW_VECTOR) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) x[j] += row_bias;
           } else if (staged_bias) {
@@ -1010,6 +1016,7 @@ int launch_gemm(const trinity_sm100_gemm& g, int sm_count, cudaStream_t stream, 
   p.split_rows = g.m <= 16 ? 16 : g.m <= 32 ? 32 : 64;
   p.split_a_rows = g.m <= 32 ? 32 : 64;
   p.late_wait = g_late_wait_for_next_launch ? 1 : 0;
+  p.column_bias = static_cast<const __nv_bfloat16*>(g_column_bias_for_next_launch);
   p.out = g.out;
   p.ldo = g.ldo;
   GemmPeers peers = {};
