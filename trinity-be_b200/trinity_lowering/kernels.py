@@ -275,6 +275,14 @@ def _operand(t, dtype, index, name):
         raise ValueError(f"{name}: expected a tensor of {dtype} on cuda:{max(index, 0)}, got {t.device} {t.dtype}")
 
 
+def _workspace_operand(t, index, what):
+    """A workspace of any type; the kernels write its ``numel() * element_size()`` bytes from its first on."""
+    if t.get_device() != index:
+        raise ValueError(f"{what}: the workspace is on another device")
+    if not t.is_contiguous():
+        raise ValueError(f"{what}: the workspace must be contiguous")
+
+
 def _rows_ok(t):
     """A [rows, cols] tensor with a unit inner stride (of no meaning when there is one column)."""
     return t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] == 1)
@@ -453,8 +461,8 @@ def gemm_adapters(x, w, down, up, index, *, scales=None, bias=None, activation=A
             raise ValueError("gemm_adapters: out must be a row-major [m,n] tensor")
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise ValueError("gemm_adapters: out dtype must be bf16 or fp32")
-    if workspace is not None and workspace.get_device() != at:
-        raise ValueError("gemm_adapters: the workspace is on another device")
+    if workspace is not None:
+        _workspace_operand(workspace, at, "gemm_adapters")
 
     def launch(handle):
         o = torch.empty((m, n), dtype=out_dtype, device=device) if out is None else out
@@ -794,8 +802,8 @@ def kv4_decode(q, cache, page_table, lengths, scale, *, out=None, lse=None, work
         _operand(lse, torch.float32, index, "lse")
         if lse.shape != (batch, heads) or not lse.is_contiguous():
             raise ValueError("kv4_decode: lse must be a contiguous [batch, heads] tensor")
-    if workspace is not None and workspace.get_device() != index:
-        raise ValueError("kv4_decode: the workspace is on another device")
+    if workspace is not None:
+        _workspace_operand(workspace, index, "kv4_decode")
 
     def launch(handle):
         o = _empty_rows(q, torch.bfloat16) if out is None else out
