@@ -505,7 +505,7 @@ extern "C" int trinity_sm100_gemm_adapters_bf16(const trinity_sm100_gemm* gemm, 
     return fail(TRINITY_SM100_E_UNSUPPORTED, "gemm_adapters: the gated form takes no adapters");
   if (g.bias_mode != TRINITY_SM100_BIAS_NONE && g.bias_mode != TRINITY_SM100_BIAS_COL_VECTOR)
     return fail(TRINITY_SM100_E_UNSUPPORTED, "gemm_adapters: bias mode %d (a vector over the columns is supported)", g.bias_mode);
-  if (!a.down || !a.up || !a.index || !a.workspace) return fail(TRINITY_SM100_E_INVALID, "gemm_adapters: null operand");
+  if (!a.down || !a.up || !a.index) return fail(TRINITY_SM100_E_INVALID, "gemm_adapters: null operand");
   if (a.count <= 0) return fail(TRINITY_SM100_E_INVALID, "gemm_adapters: no adapters");
   if (a.rank <= 0 || a.rank % 8 || a.rank > 128)
     return fail(TRINITY_SM100_E_UNSUPPORTED, "gemm_adapters: rank %d (multiples of 8 up to 128)", a.rank);
@@ -521,6 +521,8 @@ extern "C" int trinity_sm100_gemm_adapters_bf16(const trinity_sm100_gemm* gemm, 
     return fail(TRINITY_SM100_E_INVALID, "gemm_adapters: a pointer is not aligned to its element type");
   if (g.m > 65535ll * 16 || g.n > INT32_MAX - 256)
     return fail(TRINITY_SM100_E_UNSUPPORTED, "gemm_adapters: too many rows (%lld)", (long long)g.m);
+  // (behind the checks of the extents: the size of the workspace is 0 for those that are refused)
+  if (!a.workspace) return fail(TRINITY_SM100_E_INVALID, "gemm_adapters: null workspace");
   const size_t need = trinity_sm100_gemm_adapters_workspace_bytes(g.m, g.n, a.rank);
   if (a.workspace_bytes < need)
     return fail(TRINITY_SM100_E_INVALID, "gemm_adapters: workspace of %zu bytes, %zu needed", a.workspace_bytes, need);

@@ -1405,7 +1405,7 @@ extern "C" int trinity_sm100_kv4_decode(const trinity_sm100_kv4_cache* cache, co
   const trinity_sm100_kv4_cache& c = *cache;
   const trinity_sm100_kv4_decode_args& a = *args;
   if (int rc = check_kv4_cache("kv4_decode", c)) return rc;
-  if (!a.q || !a.out || !a.page_table || !a.lengths || !a.workspace) return fail(TRINITY_SM100_E_INVALID, "kv4_decode: null pointer");
+  if (!a.q || !a.out || !a.page_table || !a.lengths) return fail(TRINITY_SM100_E_INVALID, "kv4_decode: null pointer");
   if (a.batch <= 0 || a.heads <= 0 || a.max_pages <= 0) return fail(TRINITY_SM100_E_INVALID, "kv4_decode: empty extent");
   if (a.heads % c.kv_heads)
     return fail(TRINITY_SM100_E_INVALID, "kv4_decode: %d query heads do not divide over %d cached ones", a.heads, c.kv_heads);
@@ -1423,6 +1423,8 @@ extern "C" int trinity_sm100_kv4_decode(const trinity_sm100_kv4_cache* cache, co
   if (((static_cast<long long>(a.max_pages) * c.page + kKv4Tile - 1) / kKv4Tile + kKv4RowUnits) * c.kv_heads * head_blocks > INT32_MAX)
     return fail(TRINITY_SM100_E_UNSUPPORTED, "kv4_decode: a sequence of up to %lld positions is too long for %d heads",
                 static_cast<long long>(a.max_pages) * c.page, a.heads);
+  // (behind the checks of the layout: the size of the workspace is 0 for one that is refused)
+  if (!a.workspace) return fail(TRINITY_SM100_E_INVALID, "kv4_decode: null workspace");
   int sm_count = 0;
   if (int rc = require_sm100(&sm_count)) return rc;
   const size_t need = trinity_sm100_kv4_decode_workspace_bytes(a.heads, c.kv_heads, c.head_dim);

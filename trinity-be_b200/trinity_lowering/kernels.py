@@ -771,7 +771,9 @@ def kv4_decode_workspace_bytes(heads, kv_heads, head_dim):
     key = (torch._C._cuda_getDevice(), heads, kv_heads, head_dim)
     size = _kv4_workspaces.get(key)
     if size is None:
-        size = _kv4_workspaces[key] = int(library().trinity_sm100_kv4_decode_workspace_bytes(heads, kv_heads, head_dim))
+        size = int(library().trinity_sm100_kv4_decode_workspace_bytes(heads, kv_heads, head_dim))
+        if size:      # 0: no such layout, or the device could not be asked
+            _kv4_workspaces[key] = size
     return size
 
 
