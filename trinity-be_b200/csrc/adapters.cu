@@ -514,7 +514,7 @@ extern "C" int trinity_sm100_gemm_adapters_bf16(const trinity_sm100_gemm* gemm, 
   if (a.ld_down < a.rank || a.ld_up < g.n) return fail(TRINITY_SM100_E_INVALID, "gemm_adapters: leading dimension smaller than the row");
   if (a.count > 1 && (a.stride_down <= 0 || a.stride_up <= 0))
     return fail(TRINITY_SM100_E_INVALID, "gemm_adapters: strides between adapters must be positive");
-  if (a.ld_down % 8 || a.ld_up % 8 || a.stride_down % 8 || a.stride_up % 8 || !aligned16(a.down) || !aligned16(a.up) ||
+  if (a.ld_down % 8 || a.ld_up % 8 || (a.count > 1 && (a.stride_down % 8 || a.stride_up % 8)) || !aligned16(a.down) || !aligned16(a.up) ||
       !aligned16(a.workspace))
     return fail(TRINITY_SM100_E_INVALID, "gemm_adapters: adapter rows and the workspace must start on 16 bytes");
   if (reinterpret_cast<uintptr_t>(a.index) % 4 || reinterpret_cast<uintptr_t>(a.scales) % 4)

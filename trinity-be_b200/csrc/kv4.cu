@@ -1276,10 +1276,12 @@ struct Kv4Grid {
     blocks = dim3(unsigned((lanes + 256 * words * batch - 1) / (256 * words * batch)), 2);
   }
 };
-// Whether every row of the keys and values starts on a multiple of `bytes`.
-bool kv4_rows_start_on(int bytes, const trinity_sm100_kv4_rows& r, int element) {
+// Whether every row of the keys and values starts on a multiple of `bytes` (the stride of an axis with
+// one entry has no meaning).
+bool kv4_rows_start_on(int bytes, const trinity_sm100_kv4_rows& r, int element, int kv_heads) {
   const uintptr_t pointers = reinterpret_cast<uintptr_t>(r.k) | reinterpret_cast<uintptr_t>(r.v);
-  const long long strides = r.k_token_stride | r.v_token_stride | r.k_head_stride | r.v_head_stride;
+  const long long strides = (r.tokens > 1 ? r.k_token_stride | r.v_token_stride : 0) |
+                            (kv_heads > 1 ? r.k_head_stride | r.v_head_stride : 0);
   return pointers % bytes == 0 && strides % (bytes / element) == 0;
 }
 
@@ -1338,8 +1340,8 @@ extern "C" int trinity_sm100_kv4_append(const trinity_sm100_kv4_cache* cache, co
   Kv4Rows p = kv4_rows(*cache, r);
   p.in[0] = static_cast<const __nv_bfloat16*>(r.k);
   p.in[1] = static_cast<const __nv_bfloat16*>(r.v);
-  const bool vectors = kv4_rows_start_on(16, r, 2);
-  const Kv4Grid grid(r.tokens, *cache, kv4_rows_start_on(32, r, 2));
+  const bool vectors = kv4_rows_start_on(16, r, 2, cache->kv_heads);
+  const Kv4Grid grid(r.tokens, *cache, kv4_rows_start_on(32, r, 2, cache->kv_heads));
   KernelLaunch launch(grid.blocks, dim3(256), 0, static_cast<cudaStream_t>(stream_handle));
   cudaError_t e;
 #define TRINITY_KV4_APPEND(D)                                                                            \
@@ -1367,13 +1369,13 @@ extern "C" int trinity_sm100_kv4_read(const trinity_sm100_kv4_cache* cache, cons
   if (out_dtype != TRINITY_SM100_BF16 && out_dtype != TRINITY_SM100_FP32)
     return fail(TRINITY_SM100_E_INVALID, "kv4_read: unknown output dtype %d", out_dtype);
   const int element = out_dtype == TRINITY_SM100_FP32 ? 4 : 2;
-  if (!kv4_rows_start_on(16, r, element)) return fail(TRINITY_SM100_E_INVALID, "kv4_read: output rows must start on 16 bytes");
+  if (!kv4_rows_start_on(16, r, element, cache->kv_heads)) return fail(TRINITY_SM100_E_INVALID, "kv4_read: output rows must start on 16 bytes");
   if (int rc = require_sm100(nullptr)) return rc;
   Kv4Rows p = kv4_rows(*cache, r);
   p.out[0] = r.k;
   p.out[1] = r.v;
   p.out_f32 = out_dtype == TRINITY_SM100_FP32;
-  const Kv4Grid grid(r.tokens, *cache, kv4_rows_start_on(32, r, element));
+  const Kv4Grid grid(r.tokens, *cache, kv4_rows_start_on(32, r, element, cache->kv_heads));
   KernelLaunch launch(grid.blocks, dim3(256), 0, static_cast<cudaStream_t>(stream_handle));
   cudaError_t e;
 #define TRINITY_KV4_READ(D)                                                                        \
@@ -1410,7 +1412,7 @@ extern "C" int trinity_sm100_kv4_decode(const trinity_sm100_kv4_cache* cache, co
   if (a.heads % c.kv_heads)
     return fail(TRINITY_SM100_E_INVALID, "kv4_decode: %d query heads do not divide over %d cached ones", a.heads, c.kv_heads);
   if (a.table_stride < a.max_pages) return fail(TRINITY_SM100_E_INVALID, "kv4_decode: table stride smaller than its row");
-  if (!aligned16(a.q) || a.q_batch_stride % 8 || a.q_head_stride % 8)
+  if (!aligned16(a.q) || (a.batch > 1 && a.q_batch_stride % 8) || (a.heads > 1 && a.q_head_stride % 8))
     return fail(TRINITY_SM100_E_INVALID, "kv4_decode: query rows must start on 16 bytes");
   if (!aligned16(a.out) || !aligned16(a.workspace)) return fail(TRINITY_SM100_E_INVALID, "kv4_decode: pointers must be 16-byte aligned");
   if (reinterpret_cast<uintptr_t>(a.page_table) % 4 || reinterpret_cast<uintptr_t>(a.lengths) % 4 ||

@@ -289,10 +289,9 @@ def _rows_ok(t):
 
 
 def _pitch(t):
-    """Row pitch of a [rows, cols] tensor in elements (of no meaning when there is one row)."""
+    """Row pitch of a [rows, cols] tensor in elements (a single row has none that means anything: its width)."""
     rows, cols = t.shape
-    pitch = t.stride(0)
-    return pitch if rows > 1 or pitch > cols else cols
+    return t.stride(0) if rows > 1 else cols
 
 
 def _empty_rows(like, dtype):
