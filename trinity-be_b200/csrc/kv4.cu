@@ -381,8 +381,8 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Rows p) {
 //   hardly weighs anything takes no bits from the others, and values may have any size that
 //   FP32 sums of the weights allow.
 //
-// Measured: 64 sequences x 4096 positions x 8 cached heads (287 MB) 70 us, 2 x 262144 with sixteen query
-// heads to a cached one (604 MB) 192 us, 200 sequences of 0 to 8191 positions 27 us, one of 1023 9.8 us.
+// Measured: 64 sequences x 4096 positions x 8 cached heads (287 MB) 71.5 us, 2 x 262144 with sixteen query
+// heads to a cached one (604 MB) 189 us, 200 sequences of 0 to 8191 positions 25 us, one of 1023 9.4 us.
 // When the first took 77, it took 60 without the arithmetic and 64 without the copies: what bounds it is
 // the latency of a warp's chain of products, exponentials and products at the twelve (eight) warps that
 // the registers allow.  Tiles of 64 positions (85 to 90 us) and four blocks an SM with two stages (84)
@@ -1143,28 +1143,38 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   }
 }
 
-// Joins the parts of a row that was cut; one block an entry of `cuts`.  A warp takes one head and
-// every kGroups-th part, lanes the channels; the groups meet in shared memory, all in a fixed order.
-template <int kD, int kHeads, int kGroups>
-__global__ void __launch_bounds__(32 * kHeads * kGroups) kv4_join_kernel(const Kv4Attend p, int blocks) {
-  constexpr int kPerLane = kD / 32, kJoinThreads = 32 * kHeads * kGroups;
-  __shared__ float sums[kGroups][kHeads][kD], ml_shared[kGroups][kHeads][2];
+// Joins the parts of a row that was cut, in a fixed order; blockIdx.x counts the entries of `cuts`.  How many parts a
+// row has depends on the lengths, which only the device knows (one long sequence among many short ones is
+// spread over almost all blocks), so a block decides what it does: of a row of up to kFewParts parts the
+// first block of each eight heads takes one head a warp, and the others leave; of a longer one every block takes
+// kJoinHeads heads, with the parts dealt out to its warps, which meet in shared memory.  (When the host chose, by the
+// average number of parts: one sequence of 131072 positions beside 63 of 16 took 50 us, now 25; 200 sequences of
+// 0 to 8191 28 and 25, 2 x 262144 192 and 189; 64 x 4096 70 and 71.5, for the blocks that leave.)
+constexpr int kJoinWarps = 8, kJoinHeads = 2, kFewParts = 16;
+template <int kD, int kHeads>
+__global__ void __launch_bounds__(32 * kJoinWarps) kv4_join_kernel(const Kv4Attend p, int blocks) {
+  constexpr int kPerLane = kD / 32;
+  __shared__ float sums[kJoinWarps][kD], ml_shared[kJoinWarps][2];
   grid_dependents_may_launch();
   grid_dependency_wait();
   const int4 cut = p.cuts[blockIdx.x];
   if (!cut.w) return;
   const int first = cut.w - 1, last = cut.z;
-  const int head = (threadIdx.x >> 5) % kHeads, group = (threadIdx.x >> 5) / kHeads, lane = threadIdx.x & 31;
+  const bool few = last - first < kFewParts;
+  const int heads_here = few ? kJoinWarps : kJoinHeads, groups = kJoinWarps / heads_here;
+  if (int(blockIdx.y) * heads_here >= kHeads) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int head = blockIdx.y * heads_here + warp % heads_here, group = warp / heads_here;
   const float* parts_ml = p.parts + static_cast<long long>(blocks) * 2 * kHeads * kD;
   float m = -INFINITY, total = 0.0f, o[kPerLane];
 #pragma unroll
   for (int e = 0; e < kPerLane; ++e) o[e] = 0.0f;
   constexpr int kBatch = 8;      // parts whose loads are in flight together
-  for (int c0 = first + group; c0 <= last; c0 += kBatch * kGroups) {
+  for (int c0 = first + group; c0 <= last; c0 += kBatch * groups) {
     float x[kBatch][kPerLane], mc[kBatch], lc[kBatch];
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      const int c = c0 + u * kGroups;
+      const int c = c0 + u * groups;
       const long long at = (static_cast<long long>(c) * 2 + (c == first ? 1 : 0)) * kHeads + head;
       mc[u] = -INFINITY;
       lc[u] = 0.0f;
@@ -1200,28 +1210,26 @@ __global__ void __launch_bounds__(32 * kHeads * kGroups) kv4_join_kernel(const K
     m = top;
   }
 #pragma unroll
-  for (int e = 0; e < kPerLane; ++e) sums[group][head][lane * kPerLane + e] = o[e];
+  for (int e = 0; e < kPerLane; ++e) sums[warp][lane * kPerLane + e] = o[e];
   if (lane == 0) {
-    ml_shared[group][head][0] = m;
-    ml_shared[group][head][1] = total;
+    ml_shared[warp][0] = m;
+    ml_shared[warp][1] = total;
   }
   __syncthreads();
   const int kv = cut.y / p.head_blocks, hb = cut.y - kv * p.head_blocks;
-  const int head0 = kv * p.group_heads + hb * kHeads;
-  for (int i = threadIdx.x; i < kHeads * kD; i += kJoinThreads) {
+  const int in_group0 = hb * kHeads + blockIdx.y * heads_here;       // first head of the block, within its cached head
+  for (int i = threadIdx.x; i < heads_here * kD; i += 32 * kJoinWarps) {
     const int h = i / kD, channel = i - h * kD;
-    if (hb * kHeads + h >= p.group_heads) break;
+    if (in_group0 + h >= p.group_heads) break;
     float top = -INFINITY, all = 0.0f, sum = 0.0f;
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g) top = fmaxf(top, ml_shared[g][h][0]);
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-      const float mg = ml_shared[g][h][0], lg = ml_shared[g][h][1];
+    for (int w = h; w < kJoinWarps; w += heads_here) top = fmaxf(top, ml_shared[w][0]);
+    for (int w = h; w < kJoinWarps; w += heads_here) {
+      const float mg = ml_shared[w][0], lg = ml_shared[w][1];
       const float f = mg == -INFINITY ? (lg == 0.0f ? 0.0f : 1.0f) : exp2f(mg - top);
       all = fmaf(lg, f, all);
-      sum = fmaf(sums[g][h][channel], f, sum);
+      sum = fmaf(sums[w][channel], f, sum);
     }
-    const long long at = static_cast<long long>(cut.x) * p.heads + head0 + h;
+    const long long at = static_cast<long long>(cut.x) * p.heads + kv * p.group_heads + in_group0 + h;
     p.out[at * kD + channel] = __float2bfloat16(all == 0.0f ? 0.0f : sum / all);
     if (p.lse && channel == 0) p.lse[at] = (top + log2f(all)) * 0.69314718055994531f;
   }
@@ -1308,14 +1316,9 @@ int launch_kv4_attend(const Kv4Attend& p, const CUtensorMap& map_k, const CUtens
     count_launch();
   }
   if (blocks > 1) {
-    // Few rows for many blocks: a row may have many parts, which four (or two) groups of warps share.  Else
-    // it has ten at most, and small blocks leave sooner.
-    const long long rows = static_cast<long long>(p.batch) * p.kv_heads * p.head_blocks;
-    constexpr int kManyGroups = kNT == 1 ? 4 : 2;
-    const bool many = rows * 8 < blocks;
-    KernelLaunch launch(dim3(p.cuts_by_row ? unsigned(rows) : unsigned(blocks)), dim3(32 * 8 * kNT * (many ? kManyGroups : 1)), 0, stream);
-    cudaError_t e = many ? cudaLaunchKernelEx(&launch.config, kv4_join_kernel<kD, 8 * kNT, kManyGroups>, p, blocks)
-                         : cudaLaunchKernelEx(&launch.config, kv4_join_kernel<kD, 8 * kNT, 1>, p, blocks);
+    const unsigned rows = unsigned(p.batch) * p.kv_heads * p.head_blocks;
+    KernelLaunch launch(dim3(p.cuts_by_row ? rows : unsigned(blocks), 8 * kNT / kJoinHeads), dim3(32 * kJoinWarps), 0, stream);
+    cudaError_t e = cudaLaunchKernelEx(&launch.config, kv4_join_kernel<kD, 8 * kNT>, p, blocks);
     if (e != cudaSuccess) return fail(TRINITY_SM100_E_CUDA, "kv4_join launch: %s", cudaGetErrorString(e));
     count_launch();
   }
