@@ -104,6 +104,8 @@ struct GemmParams {
   long long ldo;           // ... and its row pitch in elements
 };
 
+constexpr int kBarrierBytes = 256;   // barriers and counters behind the staging buffers
+
 // In a CTA pair each CTA stages only half of the tile's B columns.
 template <int kBN, bool kPair = false>
 __host__ __device__ constexpr int stage_bytes() {
@@ -111,7 +113,7 @@ __host__ __device__ constexpr int stage_bytes() {
 }
 template <int kBN, int kStages, bool kPair = false>
 __host__ __device__ constexpr int gemm_smem_bytes() {
-  return 1024 + kStages * stage_bytes<kBN, kPair>() + kStagingBytes + 256;
+  return 1024 + kStages * stage_bytes<kBN, kPair>() + kStagingBytes + kBarrierBytes;
 }
 
 // Rasterisation: groups of `group_rows` tile rows are walked column by column so that the
@@ -296,6 +298,7 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a,
   constexpr bool kCanStageBias = !kOutF32 && !kGated && !kFused && !kBatched && !kSplit;
   const bool staged_bias = kCanStageBias && p.bias_mode == TRINITY_SM100_BIAS_MATRIX;
   auto bias_bar = [&](int quad, uint32_t buffer) { return stored_count + 24u + 8u * (quad * 2 + buffer); };
+  static_assert(8 * (2 * kStages + 4) + 8 + 24 + 8 * 8 <= kBarrierBytes, "the barriers outgrow their place in shared memory");
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
