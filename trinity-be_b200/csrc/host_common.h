@@ -36,7 +36,9 @@ int mla_prepare_device();
 // blocks may start while the previous kernel of the stream is still draining.  Every kernel
 // launched this way runs only its set-up (barriers, tensor memory, descriptor prefetch) before
 // `griddepcontrol.wait`, which returns once the previous kernel has completed and its writes are
-// visible; nothing before the wait reads or writes memory another kernel produces.
+// visible; nothing before the wait reads or writes memory that a kernel still running may produce.
+// (In the chain of the adapters the first kernel waits for all that lies before it, so the second reads
+// the adapters, and the GEMM behind it its operands, before their own waits; each says so.)
 struct KernelLaunch {
   cudaLaunchConfig_t config;
   cudaLaunchAttribute attributes[2];

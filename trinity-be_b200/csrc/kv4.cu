@@ -391,9 +391,9 @@ constexpr int kKv4Tile = 128;          // positions in a stage
 constexpr int kKv4Warps = 4;
 constexpr int kKv4Sub = kKv4Tile / (16 * kKv4Warps);   // groups of 16 positions a warp takes of each tile
 constexpr int kKv4RowUnits = 2;
-// Resident blocks an SM: three (twelve warps of 168 registers), or two where sixteen heads with four
-// groups of scales each need more registers and shared memory.
-__host__ __device__ constexpr int kv4_per_sm(int groups, int head_tiles) { return head_tiles > 1 ? 2 : 3; }
+// Resident blocks an SM: three (twelve warps of up to 168 registers), or two with sixteen heads, whose accumulators
+// take 226 to 255 registers and which hold twice the queries.
+__host__ __device__ constexpr int kv4_per_sm(int head_tiles) { return head_tiles > 1 ? 2 : 3; }
 constexpr uint32_t kKv4Lag = 2;
 // The largest exponential times value magnitude is 2^kKv4Top when the reference point is set, and 2^kKv4Room
 // times that at most before it is set again; times kKv4Unit it is an FP16 number (below 2^15).  The
@@ -615,7 +615,7 @@ __host__ __device__ constexpr int kv4_query_bytes() {
 template <int kD, int kNG, int kNT>
 __host__ __device__ constexpr int kv4_stages() {
   // what a block's share of an SM's 228 KB leaves beside the system's 1 KB a block, static variables and alignment
-  return (228 * 1024 / kv4_per_sm(kNG, kNT) - 3 * 1024 - kv4_join_bytes<kD>() - kv4_query_bytes<kD, kNT>()) / kv4_stage_bytes<kD, kNG>();
+  return (228 * 1024 / kv4_per_sm(kNT) - 3 * 1024 - kv4_join_bytes<kD>() - kv4_query_bytes<kD, kNT>()) / kv4_stage_bytes<kD, kNG>();
 }
 template <int kD, int kNG, int kNT>
 __host__ __device__ constexpr int kv4_smem_bytes() {
@@ -624,7 +624,7 @@ __host__ __device__ constexpr int kv4_smem_bytes() {
 }
 
 template <int kD, int kNG, int kNT>
-__global__ void __launch_bounds__(kKv4Threads, kv4_per_sm(kNG, kNT))
+__global__ void __launch_bounds__(kKv4Threads, kv4_per_sm(kNT))
 kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                   const Kv4Attend p) {
   constexpr int kRow = kD / 2;                         // bytes of codes a position
@@ -1277,10 +1277,10 @@ Kv4Rows kv4_rows(const trinity_sm100_kv4_cache& c, const trinity_sm100_kv4_rows&
 struct Kv4Grid {
   int words, batch;
   dim3 blocks;
-  Kv4Grid(long long tokens, const trinity_sm100_kv4_cache& c, bool wide) {
-    const long long lanes = tokens * c.kv_heads * (c.head_dim / 8);
-    words = lanes > 148 * 2048 && wide ? 2 : 1;
-    batch = lanes > 148 * 2048 ? 4 / words : 1;
+  Kv4Grid(long long tokens, const trinity_sm100_kv4_cache& c, bool wide, int sm_count) {
+    const long long lanes = tokens * c.kv_heads * (c.head_dim / 8), resident = 2048ll * sm_count;
+    words = lanes > resident && wide ? 2 : 1;
+    batch = lanes > resident ? 4 / words : 1;
     blocks = dim3(unsigned((lanes + 256 * words * batch - 1) / (256 * words * batch)), 2);
   }
 };
@@ -1325,7 +1325,7 @@ int launch_kv4_attend(const Kv4Attend& p, const CUtensorMap& map_k, const CUtens
   return check_launch("kv4_decode");
 }
 
-int kv4_blocks(int sm_count, int groups, int block_heads) { return kv4_per_sm(groups, block_heads / 8) * sm_count; }
+int kv4_blocks(int sm_count, int block_heads) { return kv4_per_sm(block_heads / 8) * sm_count; }
 
 }  // namespace
 }  // namespace trinity_sm100
@@ -1339,12 +1339,13 @@ extern "C" int trinity_sm100_kv4_append(const trinity_sm100_kv4_cache* cache, co
   if (int rc = check_kv4_rows("kv4_append", *cache, r)) return rc;
   if (reinterpret_cast<uintptr_t>(r.k) % 2 || reinterpret_cast<uintptr_t>(r.v) % 2)
     return fail(TRINITY_SM100_E_INVALID, "kv4_append: a pointer is not aligned to its element type");
-  if (int rc = require_sm100(nullptr)) return rc;
+  int sm_count = 0;
+  if (int rc = require_sm100(&sm_count)) return rc;
   Kv4Rows p = kv4_rows(*cache, r);
   p.in[0] = static_cast<const __nv_bfloat16*>(r.k);
   p.in[1] = static_cast<const __nv_bfloat16*>(r.v);
   const bool vectors = kv4_rows_start_on(16, r, 2, cache->kv_heads);
-  const Kv4Grid grid(r.tokens, *cache, kv4_rows_start_on(32, r, 2, cache->kv_heads));
+  const Kv4Grid grid(r.tokens, *cache, kv4_rows_start_on(32, r, 2, cache->kv_heads), sm_count);
   KernelLaunch launch(grid.blocks, dim3(256), 0, static_cast<cudaStream_t>(stream_handle));
   cudaError_t e;
 #define TRINITY_KV4_APPEND(D)                                                                            \
@@ -1373,12 +1374,13 @@ extern "C" int trinity_sm100_kv4_read(const trinity_sm100_kv4_cache* cache, cons
     return fail(TRINITY_SM100_E_INVALID, "kv4_read: unknown output dtype %d", out_dtype);
   const int element = out_dtype == TRINITY_SM100_FP32 ? 4 : 2;
   if (!kv4_rows_start_on(16, r, element, cache->kv_heads)) return fail(TRINITY_SM100_E_INVALID, "kv4_read: output rows must start on 16 bytes");
-  if (int rc = require_sm100(nullptr)) return rc;
+  int sm_count = 0;
+  if (int rc = require_sm100(&sm_count)) return rc;
   Kv4Rows p = kv4_rows(*cache, r);
   p.out[0] = r.k;
   p.out[1] = r.v;
   p.out_f32 = out_dtype == TRINITY_SM100_FP32;
-  const Kv4Grid grid(r.tokens, *cache, kv4_rows_start_on(32, r, element, cache->kv_heads));
+  const Kv4Grid grid(r.tokens, *cache, kv4_rows_start_on(32, r, element, cache->kv_heads), sm_count);
   KernelLaunch launch(grid.blocks, dim3(256), 0, static_cast<cudaStream_t>(stream_handle));
   cudaError_t e;
 #define TRINITY_KV4_READ(D)                                                                        \
@@ -1400,7 +1402,7 @@ extern "C" size_t trinity_sm100_kv4_decode_workspace_bytes(int32_t heads, int32_
   int sm_count = 0;
   if (heads <= 0 || kv_heads <= 0 || head_dim <= 0 || heads % kv_heads || require_sm100(&sm_count)) return 0;
   const int group_heads = heads / kv_heads;
-  const size_t blocks = kv4_blocks(sm_count, 1, 8);      // the most that any grouping uses
+  const size_t blocks = kv4_blocks(sm_count, 8);      // the most that any layout uses
   return blocks * 2 * (group_heads > 8 ? 16 : 8) * (size_t(head_dim) + 2) * 4 + blocks * sizeof(int4);
 }
 
@@ -1465,7 +1467,7 @@ extern "C" int trinity_sm100_kv4_decode(const trinity_sm100_kv4_cache* cache, co
   const uint32_t box_lines = p.box * (c.head_dim / 2) / 128;
   if (int rc = make_tensor_map_3d(&map_k, c.k_codes, 2, 64, lines, 1, 128, 128 * lines, 64, box_lines, 1, 128)) return rc;
   if (int rc = make_tensor_map_3d(&map_v, c.v_codes, 2, 64, lines, 1, 128, 128 * lines, 64, box_lines, 1, 128)) return rc;
-  const int blocks = kv4_blocks(sm_count, c.head_dim / c.group, block_heads);
+  const int blocks = kv4_blocks(sm_count, block_heads);
   p.cuts_by_row = static_cast<long long>(a.batch) * c.kv_heads * head_blocks <= blocks ? 1 : 0;
   p.cuts = reinterpret_cast<int4*>(p.parts + static_cast<size_t>(blocks) * 2 * block_heads * (c.head_dim + 2));
   cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
