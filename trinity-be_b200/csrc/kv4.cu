@@ -381,8 +381,8 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Rows p) {
 //   hardly weighs anything takes no bits from the others, and values may have any size that
 //   FP32 sums of the weights allow.
 //
-// Measured: 64 sequences x 4096 positions x 8 cached heads (287 MB) 71.5 us, 2 x 262144 with sixteen query
-// heads to a cached one (604 MB) 189 us, 200 sequences of 0 to 8191 positions 25 us, one of 1023 9.4 us.
+// Measured: 64 sequences x 4096 positions x 8 cached heads (287 MB) 72 us, 2 x 262144 with sixteen query
+// heads to a cached one (604 MB) 189 us, 200 sequences of 0 to 8191 positions 25 us, one of 1023 9.5 us.
 // When the first took 77, it took 60 without the arithmetic and 64 without the copies: what bounds it is
 // the latency of a warp's chain of products, exponentials and products at the twelve (eight) warps that
 // the registers allow.  Tiles of 64 positions (85 to 90 us) and four blocks an SM with two stages (84)
@@ -402,6 +402,8 @@ constexpr uint32_t kKv4Lag = 2;
 // (sums of the weights of values that are all zero must not overflow).
 constexpr float kKv4Top = 27.0f, kKv4Room = 8.0f, kKv4Unit = 0x1p-20f, kKv4Smallest = 0x1p-60f;
 constexpr float kKv4NoScore = -3e38f;     // reference point before the first score: below any but -infinity
+// Reference points from here on are too coarse for sums with them: such heads take the exact way at every tile.
+constexpr float kKv4Coarse = 0x1p22f;
 constexpr int kKv4Threads = kKv4Warps * 32;
 
 struct Kv4Attend {
@@ -958,6 +960,10 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
             }
           bool raise = false;
 #pragma unroll
+          for (int n = 0; n < kNT; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) raise |= !(fabsf(ref[n][c]) < kKv4Coarse);
+#pragma unroll
           for (int u = 0; u < kKv4Sub; ++u)
 #pragma unroll
             for (int n = 0; n < kNT; ++n)
@@ -969,16 +975,23 @@ kv4_attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
             for (int n = 0; n < kNT; ++n)
 #pragma unroll
               for (int c = 0; c < 2; ++c) {
-                float m = -INFINITY;
+                // the largest score, and relative to it (exactly) the largest score and logarithm
+                float m = -INFINITY, top = -INFINITY;
 #pragma unroll
-                for (int u = 0; u < kKv4Sub; ++u)
-                  m = fmaxf(m, fmaxf(score[u][n][c] + level[u][0], score[u][n][2 + c] + level[u][1]));
+                for (int u = 0; u < kKv4Sub; ++u) m = fmaxf(m, fmaxf(score[u][n][c], score[u][n][2 + c]));
 #pragma unroll
                 for (int o = 4; o < 32; o *= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                float f = 1.0f;
-                if (m - kKv4Top > ref[n][c]) {
-                  f = exp2_approx(ref[n][c] - (m - kKv4Top));
-                  ref[n][c] = m - kKv4Top;
+#pragma unroll
+                for (int u = 0; u < kKv4Sub; ++u)
+                  top = fmaxf(top, fmaxf((score[u][n][c] - m) + level[u][0], (score[u][n][2 + c] - m) + level[u][1]));
+#pragma unroll
+                for (int o = 4; o < 32; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                float next = m + (top - kKv4Top), f = 1.0f;
+                if ((m - next) + top > kKv4Top + kKv4Room)        // rounded too far down (scores of 2^28)
+                  next = __int_as_float(__float_as_int(next) + (next < 0.0f ? -1 : 1));
+                if (next > ref[n][c]) {
+                  f = exp2_approx(ref[n][c] - next);
+                  ref[n][c] = next;
                 }
                 sum[n][c] *= f;
 #pragma unroll
