@@ -15,7 +15,7 @@
 // Bound by memory with few rows: the weight (the GEMM's part) and the adapters that the rows name, read
 // once each.  16 rows x 8192 x 8192 with 12 adapters of rank 16: 39 us (floor 21; GEMM 29, the small
 // kernels 8 each, in part beside it).  61 rows x 4096 x 28672, 24 adapters of rank 64: 67 us (floor 52).
-// 8192^3 with rank 32: 800 to 823 us, of which the GEMM 707 to 720 under its power cap.
+// 8192^3 with rank 32: 818 to 860 us (950 to 1000 in passes issued one by one), of which the GEMM 717 under its power cap.
 //
 // Rounding t and delta to BF16 costs 2^-8 of the adapter's own contribution each, as the
 // intermediates of the other chained products of this library do.

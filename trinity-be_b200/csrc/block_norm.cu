@@ -7,9 +7,10 @@
 // Bound by memory: x, the residual and a full gate are read once, residual_out and out written
 // once.  A row is spread over kThreads lanes (32..1024) of 16 elements each (8 where the layout
 // allows only one at a time); the lane keeps its part of the row in registers through both sums, so
-// nothing is read twice.  Warps in flight decide: with 16-byte accesses 48 warps an SM (40 registers
-// a thread) take 169 us for 32768 x 4096 BF16 (1074 MB, 0.97 of the measured copy rate), 36 warps
-// 184 us and 56 warps (spilling) 205 us.  All arithmetic is FP32; the two roundings are those of the
+// nothing is read twice.  Warps in flight decide: with 16-byte accesses 48 warps an SM (40 registers a
+// thread, and 20 to 32 bytes of spills) take 170 us for 32768 x 4096 BF16 (1074 MB, 0.96 of the measured copy
+// rate; 187 to 195 in passes issued one by one), 36 warps 184 us and 56 warps (spilling more) 205 us.  With FP32
+// operands, 32 warps: 240 us for an FP32 stream (1611 MB), 279 with x in FP32 too.  All arithmetic is FP32; the two roundings are those of the
 // two outputs (out is computed from the unrounded h).
 #include "host_common.h"
 #include "sm100_ptx.cuh"
@@ -89,11 +90,11 @@ __device__ __forceinline__ const void* element_of(const void* base, long long of
               : static_cast<const void*>(static_cast<const __nv_bfloat16*>(base) + offset);
 }
 
-// kW = 8: 16-byte accesses (every row of every operand starts on 16 bytes); kW = 1: any layout.
-// kElements a lane.
 // Threads an SM is to hold, which bounds the registers of each (see above; FP32 operands need more).
 template <int kW, bool kF32>
 constexpr int seam_resident() { return kW == 1 ? 2048 : kF32 ? 1024 : 1536; }
+// kW = 8: 16-byte accesses (every row of every operand starts on 16 bytes); kW = 1: any layout.
+// kElements a lane.
 template <int kThreads, int kW, int kElements, bool kXF32, bool kResF32>
 __global__ void __launch_bounds__(kThreads > kRowBlock ? kThreads : kRowBlock, (kElements > 8 && kW == 1 ? 1 : seam_resident<kW, kXF32 || kResF32>() / (kThreads > kRowBlock ? kThreads : kRowBlock)))
 rmsnorm_residual_kernel(const SeamParams p) {

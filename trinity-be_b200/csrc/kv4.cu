@@ -26,8 +26,8 @@ constexpr uint32_t kSiteKv4Page = 0x903;
 // Bound by memory: 2 D bytes read and D / 2 + 4 D / group written per row (append).  A lane owns
 // sixteen channels (one 32-byte access, two 32-bit words of codes) or eight, with keys and values in
 // one launch; a group's extrema meet by shuffles within its 2 to 16 lanes.  32771 tokens x 8 heads x
-// 128 channels in groups of 32, written and read back: 62 us for 352.6 MB (append 32.1, read 28.9: 0.84 and
-// 0.93 of the measured copy rate; with eight channels a lane and single FP32 arithmetic instruction
+// 128 channels in groups of 32, written and read back: 63 us for 352.6 MB (append 32.7, read 29.0: 0.82 and
+// 0.93 of the measured copy rate; read in FP32 48.7 us for 311 MB; with eight channels a lane and single FP32 arithmetic instruction
 // issue took 84).  One token of 64 sequences: 3.2 us for both.
 struct Kv4Rows {
   const __nv_bfloat16* in[2];      // append: keys, values
@@ -157,7 +157,7 @@ __device__ __forceinline__ void store_once(void* p, const uint32_t (&w)[kCount])
                  : "memory");
 }
 
-// Five blocks of sixteen channels a lane an SM: 32.1 us at the size above; four 35.4, six (spilling) 32.4.
+// Five blocks of sixteen channels a lane an SM: 32.1 to 32.7 us at the size above; four 35.4, six (spilling) 32.4.
 template <int kD, int kWords, bool kVector, int kBatch>
 __global__ void __launch_bounds__(256, kWords == 2 ? 5 : 1) kv4_append_kernel(const Kv4Rows p) {
   constexpr int kChannels = 8 * kWords, kLanes = kD / kChannels;
@@ -392,7 +392,7 @@ constexpr int kKv4Warps = 4;
 constexpr int kKv4Sub = kKv4Tile / (16 * kKv4Warps);   // groups of 16 positions a warp takes of each tile
 constexpr int kKv4RowUnits = 2;
 // Resident blocks an SM: three (twelve warps of up to 168 registers), or two with sixteen heads, whose accumulators
-// take 226 to 255 registers and which hold twice the queries.
+// take 212 to 255 registers and which hold twice the queries.
 __host__ __device__ constexpr int kv4_per_sm(int head_tiles) { return head_tiles > 1 ? 2 : 3; }
 constexpr uint32_t kKv4Lag = 2;
 // The largest exponential times value magnitude is 2^kKv4Top when the reference point is set, and 2^kKv4Room
