@@ -427,7 +427,8 @@ TRINITY_SM100_API int trinity_sm100_kv4_read(const trinity_sm100_kv4_cache* cach
  * Beside the final rounding to BF16 the products of weights and value scales are rounded by 2^-11, or by
  * 2^-28 of the row's largest product of weight and value magnitude where that is more; everything
  * else is FP32.  Finite inputs give finite results as long as |scale| times the largest query element stays
- * below 2^113 and the scores below 2^28 (from 2^20 on the rounding of FP32 scores shows in the weights).  Where a row holds values of 2^100 and more, positions that weigh less than 2^-25 of the
+ * below 2^113 and the scores below 2^28 (from 2^20 on the rounding of FP32 scores shows in the
+ * weights).  Where a row holds values of 2^100 and more, positions that weigh less than 2^-25 of the
  * heaviest may be lost; values below 2^-60 are good to 2^-88.
  */
 typedef struct trinity_sm100_kv4_decode_args {

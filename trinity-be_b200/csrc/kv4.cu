@@ -27,8 +27,8 @@ constexpr uint32_t kSiteKv4Page = 0x903;
 // sixteen channels (one 32-byte access, two 32-bit words of codes) or eight, with keys and values in
 // one launch; a group's extrema meet by shuffles within its 2 to 16 lanes.  32771 tokens x 8 heads x
 // 128 channels in groups of 32, written and read back: 63 us for 352.6 MB (append 32.7, read 29.0: 0.82 and
-// 0.93 of the measured copy rate; read in FP32 48.7 us for 311 MB; with eight channels a lane and single FP32 arithmetic instruction
-// issue took 84).  One token of 64 sequences: 3.2 us for both.
+// 0.93 of the measured copy rate; read in FP32 48.7 us for 311 MB; with eight channels a lane and single
+// FP32 arithmetic instruction issue took 84).  One token of 64 sequences: 3.1 us for both.
 struct Kv4Rows {
   const __nv_bfloat16* in[2];      // append: keys, values
   void* out[2];                    // read: keys, values
